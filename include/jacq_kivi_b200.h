@@ -231,6 +231,102 @@ int kivi_b200_gemv_f16(const kivi_f16* w, const kivi_f16* x, kivi_f16* y_f16, fl
  * healthy run) to *failures_out; synchronises the device. */
 int kivi_b200_gemm_wait_failures(uint32_t* failures_out);
 
+/* ------------------------------------------------------------------ 8-bit block-scaled cache (q8) --
+ * A paged KV cache in 8 bits with ONE fp32 scale for K and one for V per page and kv head, beside the int4 KIVI
+ * cache: half its compression, a quarter of a per cent of parameters, and an error that does not depend on
+ * per-channel statistics. No counterpart in the reference. Layout, for B = block_size tokens per page:
+ *
+ *   k_pages, v_pages  8-bit [num_blocks, NKV, B, D]   int8 or e4m3 codes; value = code * scale
+ *   scales            f32   [num_blocks, NKV, 2]      K scale, V scale
+ *   k_tail, v_tail    f16   [num_slots, NKV, B, D]    the tokens of a sequence's last, incomplete block
+ *
+ * Token j of a sequence is row j % B of logical page j / B. A sequence of T tokens holds T / B complete pages in
+ * 8 bits (block table entries 0 .. T / B - 1) and T % B rows, 0 .. T % B - 1, of its tail slot in fp16: a block is
+ * quantised once, from its fp16 rows, when its last token arrives, so no value is ever rounded twice.
+ *   scale = max|x| * fp32(1/127) (e4m3: fp32(1/448)), code = x / scale rounded to nearest even
+ * An all-zero block has scale 0. A block that holds an infinity or a NaN gets scale NaN and zero codes: every
+ * query that sees one of its tokens yields NaN, queries that do not are unaffected. */
+enum kivi_q8_format { KIVI_Q8_INT8 = 0, KIVI_Q8_E4M3 = 1 };
+
+typedef struct kivi_q8_geometry {
+    int32_t num_q_heads;
+    int32_t num_kv_heads;  /* num_q_heads % num_kv_heads == 0 */
+    int32_t head_dim;      /* 64, 128 or 256 */
+    int32_t block_size;    /* 16, 32, 64 or 128 */
+    int32_t format;        /* kivi_q8_format */
+} kivi_q8_geometry;
+
+typedef struct kivi_q8_cache {
+    uint8_t* k_pages;
+    uint8_t* v_pages;
+    float* scales;
+    kivi_f16* k_tail;
+    kivi_f16* v_tail;
+    int32_t num_blocks;
+    int32_t num_slots;
+} kivi_q8_cache;
+
+int kivi_b200_q8_validate_geometry(const kivi_q8_geometry* geom);
+
+/* Append rows new_offsets[i] .. new_offsets[i+1]-1 of new_k / new_v to sequence i, which held start_seq_lens[i]
+ * tokens. Token rows are [NKV, D] contiguous, k_stride / v_stride fp16 elements apart (multiples of 8), so that slices
+ * of a fused projection's output go in as they are. total_new: rows of new_k and new_v; a sequence whose offsets do
+ * not lie inside them, whose length or count lies outside 0 .. max_start_seq_len / max_new_per_seq, or whose slot or
+ * pages lie outside the pools is left untouched and counted. Sequences of one call must not share a slot or a page. */
+int kivi_b200_q8_cache_write(const kivi_q8_geometry* geom, const kivi_q8_cache* cache,
+                             const kivi_f16* new_k, const kivi_f16* new_v, int64_t k_stride, int64_t v_stride,
+                             const int32_t* block_tables, int max_blocks_per_seq,
+                             const int32_t* start_seq_lens, const int32_t* new_offsets, const int32_t* slot_ids,
+                             int batch, int total_new, int max_new_per_seq, int max_start_seq_len,
+                             cudaStream_t stream);
+
+/* The values the cache holds, as fp16: rows row_offsets[i] .. row_offsets[i+1]-1 of k_out / v_out
+ * ([total_rows, NKV, D], contiguous) receive tokens first_rows[i] .. of sequence i, which holds seq_lens[i] tokens.
+ * Rows behind the sequence's last token become zeros; the rows of sequences the call rejects (as above) are left. */
+int kivi_b200_q8_cache_read(const kivi_q8_geometry* geom, const kivi_q8_cache* cache,
+                            const int32_t* block_tables, int max_blocks_per_seq, const int32_t* seq_lens,
+                            const int32_t* slot_ids, const int32_t* row_offsets, const int32_t* first_rows,
+                            int batch, int total_rows, int max_rows_per_seq, kivi_f16* k_out, kivi_f16* v_out,
+                            cudaStream_t stream);
+
+/* Bytes of workspace kivi_b200_q8_attention needs (0: none; also 0 for arguments it would refuse). */
+size_t kivi_b200_q8_attention_workspace_bytes(const kivi_q8_geometry* geom, int batch, int max_q_per_seq,
+                                              int max_seq_len, int window, int sinks, int with_mass);
+
+/* Attention of the last tokens of every sequence over the cache. q f16 [total_q, NH, D], token rows q_stride elements
+ * apart (a multiple of 8); sequence i owns rows q_offsets[i] .. q_offsets[i+1]-1 (q_offsets NULL: one row each,
+ * total_q = batch), the queries of its last tokens, already written to the cache: with n rows and T = seq_lens[i]
+ * tokens, row r is token T - n + r. Token i sees token j when j <= i and (j < sinks or j > i - window); window 0 is no
+ * window, and sinks then says nothing. scale multiplies q.k; 0 stands for 1 / sqrt(D). A row that sees nothing gives
+ * zeros. out_f16 or out_f32 [total_q, NH, D], contiguous; exactly one is not NULL.
+ * page_mass (or NULL) f32 [batch, NKV, mass_width], single-token calls only (q_offsets NULL): entry [i, h, p] grows by the
+ * softmax weight that the query heads of kv head h gave the tokens of logical page p; mass_width * B >= max_seq_len.
+ * Lengths are on the device: a longer one than max_seq_len counts as max_seq_len, a negative one as 0; page and slot
+ * ids outside the pools are read as 0 and counted; a sequence whose q rows lie outside 0 .. total_q is skipped. */
+int kivi_b200_q8_attention(const kivi_q8_geometry* geom, const kivi_q8_cache* cache, const kivi_f16* q,
+                           int64_t q_stride, const int32_t* q_offsets, int total_q, const int32_t* block_tables,
+                           int max_blocks_per_seq, const int32_t* seq_lens, const int32_t* slot_ids, int batch,
+                           int max_q_per_seq, int max_seq_len, int window, int sinks, float scale,
+                           float* page_mass, int mass_width, float* out_f32, kivi_f16* out_f16,
+                           void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
+/* Keep `budget` complete pages of every sequence that has more: its first `first` and last `recent` ones and, of the
+ * others, those of the largest page_mass summed over the kv heads (in 64 bits, then rounded to fp32; equal ones:
+ * the lowest page first; NaN ranks below everything). first + recent <= budget. Nothing is moved: the kept pages'
+ * table entries close up in their order, the tail stays. All outputs are written whole and may not alias the inputs:
+ *   new_tables [batch, max_blocks_per_seq]: 0 behind the kept pages;  new_lens [batch]
+ *   new_mass [batch, NKV, mass_width]: the kept pages' columns and the open block's, 0 behind them
+ *   freed [batch, max_blocks_per_seq]: ids of the evicted pages in order, -1 behind them;  freed_counts [batch]
+ * mass_width * block_size >= max_seq_len; lengths are clamped to 0 .. max_seq_len. */
+int kivi_b200_q8_evict(int num_kv_heads, int block_size, const int32_t* block_tables, int max_blocks_per_seq,
+                       const int32_t* seq_lens, const float* page_mass, int mass_width, int batch, int max_seq_len,
+                       int budget, int first, int recent, int32_t* new_tables, int32_t* new_lens, float* new_mass,
+                       int32_t* freed, int32_t* freed_counts, cudaStream_t stream);
+
+/* Sequences (write, read) and ids (attention) refused since the library was loaded on the current device; 0 in any
+ * healthy run. Synchronises the device. */
+int kivi_b200_q8_rejected_indices(uint32_t* count_out);
+
 /* ------------------------------------------------------------------ ABI v1 (reference lane) -- */
 
 /* ---------------------------------------------------------------------------------------------

@@ -6,7 +6,7 @@ shared object has not been built (``python -m jacq_b200.build``).
 from __future__ import annotations
 
 import ctypes
-from ctypes import c_float, c_int, c_int32, c_size_t, c_uint32, c_void_p
+from ctypes import c_float, c_int, c_int32, c_int64, c_size_t, c_uint32, c_void_p
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libjacq_kivi_b200.so"
@@ -29,6 +29,19 @@ class KiviCacheStruct(ctypes.Structure):
     _fields_ = [(n, c_void_p) for n in
                 ("k_code_pages", "k_scale_pages", "k_zero_pages", "v_code_pages", "v_scale_pages",
                  "v_zero_pages", "k_residual_scratch", "v_residual_scratch")] + \
+               [("num_blocks", c_int32), ("num_slots", c_int32)]
+
+
+class KiviQ8Geometry(ctypes.Structure):
+    """``kivi_q8_geometry`` of the header."""
+
+    _fields_ = [(n, c_int32) for n in ("num_q_heads", "num_kv_heads", "head_dim", "block_size", "format")]
+
+
+class KiviQ8CacheStruct(ctypes.Structure):
+    """``kivi_q8_cache`` of the header."""
+
+    _fields_ = [(n, c_void_p) for n in ("k_pages", "v_pages", "scales", "k_tail", "v_tail")] + \
                [("num_blocks", c_int32), ("num_slots", c_int32)]
 
 
@@ -114,6 +127,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kivi_b200_bias_rope": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_float, _P]),
     "kivi_b200_silu_mul": (c_int, [_P, _P, c_int, c_int, _P]),
     "kivi_b200_argmax": (c_int, [_P, _P, c_int, c_int, _P, c_size_t, _P]),
+    "kivi_b200_q8_validate_geometry": (c_int, [ctypes.POINTER(KiviQ8Geometry)]),
+    "kivi_b200_q8_cache_write": (c_int, [ctypes.POINTER(KiviQ8Geometry), ctypes.POINTER(KiviQ8CacheStruct), _P, _P, c_int64,
+                                         c_int64, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, _P]),
+    "kivi_b200_q8_cache_read": (c_int, [ctypes.POINTER(KiviQ8Geometry), ctypes.POINTER(KiviQ8CacheStruct), _P, c_int, _P, _P,
+                                        _P, _P, c_int, c_int, c_int, _P, _P, _P]),
+    "kivi_b200_q8_attention_workspace_bytes": (c_size_t, [ctypes.POINTER(KiviQ8Geometry)] + [c_int] * 6),
+    "kivi_b200_q8_attention": (c_int, [ctypes.POINTER(KiviQ8Geometry), ctypes.POINTER(KiviQ8CacheStruct), _P, c_int64, _P,
+                                       c_int, _P, c_int, _P, _P, c_int, c_int, c_int, c_int, c_int, c_float, _P, c_int, _P,
+                                       _P, _P, c_size_t, _P]),
+    "kivi_b200_q8_evict": (c_int, [c_int, c_int, _P, c_int, _P, _P] + [c_int] * 6 + [_P] * 6),
+    "kivi_b200_q8_rejected_indices": (c_int, [ctypes.POINTER(c_uint32)]),
     "jac_launch": (None, [_P, _P] + _V1_CACHE + [c_int, _P, _P]),
     "jac_launch_tp2_local": (None, [_P, _P] + _V1_CACHE + [c_int, _P, _P]),
     "jac_launch_batched": (None, [_P, _P, _P] + _V1_CACHE + [c_int, _P, _P]),

@@ -1,0 +1,636 @@
+// Attention over the 8-bit block-scaled cache: one query token per sequence (serving), short runs and prompts.
+//
+//   s_ij = scale * ks(page of j) * (q_i . kc_j),  out_i = sum_j p_ij vs(page of j) vc_j / sum_j p_ij,  p = 2^(s log2e - m)
+//
+// kc, vc are codes: both formats are exact in fp16, and a page has ONE scale, so neither K nor V is ever scaled element
+// by element: K's scale multiplies the 16 x rows score tile, V's goes into the probabilities. The products run on
+// mma.sync m16n8k16 with tokens (QK) and channels (PV) as the 16 side and the query rows as the 8 side. What bounds a
+// single-token call is HBM: 2 D bytes per token and kv head against 4 D flops per query row.
+//
+// No shared-memory tile is exchanged between lanes. The order of the contraction index is free, and so is the order of
+// the output channels, so lane (g, t) = (lane / 4, lane % 4) takes of a 16-token tile exactly the bytes its fragments
+// need, in 16-byte pieces: K rows g and g + 8, channels 16 (t + 4 j) ..; V tokens 2t, 2t+1, 2t+8, 2t+9, channels
+// (D / 8) g .. . Every warp-level copy covers whole 32-byte sectors, a lane reads back only what it asked for itself,
+// and cp.async's per-thread groups are the only synchronisation of the ring.
+//
+// A sequence's context is cut into `parts`, one CTA each, that form a thread-block cluster: they merge through
+// distributed shared memory, so a call needs no second launch and no workspace.
+#include <cooperative_groups.h>
+#include <cfloat>
+
+#include "q8_common.cuh"
+
+namespace kivi {
+namespace {
+
+namespace cg = cooperative_groups;
+
+constexpr int kWarps = 4;
+constexpr float kUnset = -3.0e38f;     // running maximum before any visible token
+constexpr float kLazy = 8.0f;          // the maximum is raised when a score tops it by 2^8
+constexpr float kHeadroom = 64.0f;     // probabilities in fp16 carry 2^6: p vs <= 2^8 2^6 < 65504, 2^20 below 1 stay normal
+
+__device__ unsigned int g_q8_attn_rejected;
+
+__device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+template <int D>
+struct Tile {
+    static constexpr int KC = D / 64;            // 16-byte pieces of a K row per lane
+    static constexpr int MT = D / 16;            // channel tiles of the output
+    static constexpr int VP = D == 256 ? 2 : 1;  // pieces of a V row per lane
+    static constexpr int VB = D == 64 ? 8 : 16;  // bytes of a piece
+    static constexpr int VW = VB / 4;            // words (4 channels) of a piece
+    static constexpr int K_BYTES = 2 * KC * 512;
+    static constexpr int V_BYTES = 4 * VP * VB * 32;
+    static constexpr int SCALE_BYTES = 256;      // every lane its own copy: nothing is exchanged
+    static constexpr int STAGE = K_BYTES + V_BYTES + SCALE_BYTES;
+};
+
+// Channel of output tile mt, half hf (rows g / g + 8 of the fragment) on lanes of group g.
+template <int D>
+__device__ __forceinline__ int channel_of(int g, int mt, int hf) {
+    if constexpr (D == 256) return (mt < 8 ? 0 : 128) + 16 * g + 2 * (mt & 7) + hf;
+    else return (D / 8) * g + 2 * mt + hf;
+}
+
+// The keys a block of query rows sees: [0, sinks) and [low, end), as 16-token tiles.
+struct View {
+    int len, n;          // tokens, query rows' tokens
+    int pos0, pos1;      // positions of the block's first and last query token
+    int low0, low1;      // first windowed key of those two
+    int end;             // keys [0, end) are at most seen
+    int paged;           // tokens held in pages
+    int ns, w0, tiles;   // page tiles: 0 .. ns - 1, then w0 ..; `tiles` in all
+    int tail_tiles;
+};
+__device__ __forceinline__ View make_view(const Q8AttnParams& p, int len, int n, int tok0, int tok1) {
+    View v;
+    v.len = len; v.n = n;
+    v.pos0 = len - n + tok0; v.pos1 = len - n + tok1;
+    v.low0 = max(0, p.window == 0x7fffffff ? 0 : v.pos0 - p.window + 1);
+    v.low1 = max(0, p.window == 0x7fffffff ? 0 : v.pos1 - p.window + 1);
+    v.end = max(0, v.pos1 + 1);
+    v.paged = len >> p.cache.log2b << p.cache.log2b;
+    const int qt = (min(v.end, v.paged) + 15) >> 4;
+    v.ns = min((min(p.sinks, v.low0) + 15) >> 4, qt);
+    v.w0 = min(v.low0 >> 4, qt);
+    if (v.ns >= v.w0) { v.ns = 0; v.w0 = 0; }
+    v.tiles = v.ns + qt - v.w0;
+    v.tail_tiles = v.end > v.paged ? (v.end - v.paged + 15) >> 4 : 0;
+    return v;
+}
+
+template <int D, int FMT, int NT, bool MASS, int S>
+__global__ void __launch_bounds__(kWarps * 32) q8_attention_kernel(const Q8AttnParams p) {
+    using T = Tile<D>;
+    constexpr int R = 8 * NT;
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ float s_m[kWarps][R], s_l[kWarps][R];
+    __shared__ float c_m[R], c_l[R];             // this CTA's merged state, read by its cluster
+    __shared__ float f_m[R], f_il[R];            // the unit's final maximum and 1 / sum
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int nkv = p.cache.nkv, block = 1 << p.cache.log2b;
+    const int part = blockIdx.x % p.parts;
+    int unit = blockIdx.x / p.parts;
+    const int rb = unit % p.row_blocks + p.row_block0;
+    unit /= p.row_blocks;
+    const int h = unit % nkv, seq = unit / nkv;
+
+    // ---- what this unit is
+    int len = p.seq.lens[seq];
+    len = min(max(len, 0), p.max_seq);
+    int row0 = seq, n = 1;
+    if (p.q_offsets) {
+        row0 = p.q_offsets[seq];
+        n = min(p.q_offsets[seq + 1] - row0, p.max_q);
+        if (row0 < 0 || n < 0 || row0 > p.total_q - n) n = 0;
+    }
+    const int rows = n * p.qpk;
+    if (rb * R >= rows) return;                  // uniform over the cluster
+    const int tok0 = rb * R / p.qpk, tok1 = min(rb * R + R, rows) - 1;
+    const View v = make_view(p, len, n, tok0, tok1 / p.qpk);
+    const int items = v.tiles + v.tail_tiles;
+    const int i0 = (int)((long long)items * part / p.parts), i1 = (int)((long long)items * (part + 1) / p.parts);
+
+    // ---- query rows as B fragments, in the channel order of the K pieces
+    uint32_t qf[NT][T::MT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int r = rb * R + 8 * nt + g;
+        const __half* row = p.q + (long long)(row0 + r / p.qpk) * p.q_stride + (size_t)(h * p.qpk + r % p.qpk) * D + 16 * t;
+#pragma unroll
+        for (int j = 0; j < T::KC; ++j) {
+            uint4 a = make_uint4(0u, 0u, 0u, 0u), b = a;
+            if (r < rows) {
+                a = *reinterpret_cast<const uint4*>(row + 64 * j);
+                b = *reinterpret_cast<const uint4*>(row + 64 * j + 8);
+            }
+            qf[nt][4 * j][0] = a.x; qf[nt][4 * j][1] = a.y; qf[nt][4 * j + 1][0] = a.z; qf[nt][4 * j + 1][1] = a.w;
+            qf[nt][4 * j + 2][0] = b.x; qf[nt][4 * j + 2][1] = b.y; qf[nt][4 * j + 3][0] = b.z; qf[nt][4 * j + 3][1] = b.w;
+        }
+    }
+    // keys that the lane's score columns (rows 2t, 2t + 1 of each 8) see
+    int hi[NT][2], lo[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int r = rb * R + 8 * nt + 2 * t + c;
+            hi[nt][c] = r < rows ? len - n + r / p.qpk : -1;
+            lo[nt][c] = p.window == 0x7fffffff ? 0 : hi[nt][c] - p.window + 1;
+        }
+
+    float o[NT][T::MT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int mt = 0; mt < T::MT; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.0f;
+        m[nt][0] = m[nt][1] = kUnset;
+        l[nt][0] = l[nt][1] = 0.0f;
+    }
+    // V's scales enter the fp16 probabilities relative to vref, a power of two not below any met so far (0: none yet)
+    float vref = 0.0f, vmul = 0.0f;
+
+    // Scores of a tile -> probabilities as B fragments pb; also the running state.
+    auto softmax = [&](float (&s)[NT][4], float f, float vs, int key0, int item, uint32_t (&pb)[NT][2]) {
+        const bool whole = key0 + 15 <= v.pos0 && (key0 >= v.low1 || key0 + 16 <= p.sinks);
+        bool raise = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                s[nt][e] *= f;
+                if (!whole) {
+                    const int key = key0 + g + (e >> 1) * 8, c = e & 1;
+                    if (key > hi[nt][c] || (key < lo[nt][c] && key >= p.sinks)) s[nt][e] = -INFINITY;
+                }
+                raise |= s[nt][e] > m[nt][e & 1] + kLazy;
+            }
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    float top = fmaxf(s[nt][c], s[nt][c + 2]);
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                    const float mn = fmaxf(m[nt][c], top), a = fast_exp2(m[nt][c] - mn);
+                    m[nt][c] = mn;
+                    l[nt][c] *= a;
+#pragma unroll
+                    for (int mt = 0; mt < T::MT; ++mt) { o[nt][mt][c] *= a; o[nt][mt][c + 2] *= a; }
+                }
+        }
+        if (vs > vref) {   // uniform over the warp; false for a NaN scale, which goes through as it is
+            const float next = __uint_as_float((__float_as_uint(vs) & 0x7f800000u) + 0x00800000u), a = vref / next;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int mt = 0; mt < T::MT; ++mt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[nt][mt][e] *= a;
+            vref = next;
+            vmul = kHeadroom / next;
+        }
+        const float w = vs * vmul;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float e[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) e[k] = fast_exp2(s[nt][k] - m[nt][k & 1]);
+            l[nt][0] += e[0] + e[2];
+            l[nt][1] += e[1] + e[3];
+            if constexpr (MASS) {
+                float a = e[0] + e[2], b = e[1] + e[3];
+#pragma unroll
+                for (int x = 4; x < 32; x *= 2) {
+                    a += __shfl_xor_sync(0xffffffffu, a, x);
+                    b += __shfl_xor_sync(0xffffffffu, b, x);
+                }
+                if (g == 0) {
+                    float4* dst = reinterpret_cast<float4*>(p.page_ws + ((size_t)(seq * nkv + h) * p.ws_tiles + item) * R + 8 * nt + 2 * t);
+                    *dst = make_float4(a, m[nt][0], b, m[nt][1]);
+                }
+            }
+            // a probability of a masked key is 0 whatever the page's scale is
+            if (!whole) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) e[k] = s[nt][k] == -INFINITY ? 0.0f : e[k] * w;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) e[k] *= w;
+            }
+            pb[nt][0] = movmatrix_trans(pack_half2(e[0], e[1]));
+            pb[nt][1] = movmatrix_trans(pack_half2(e[2], e[3]));
+        }
+        return whole;
+    };
+    // Whether a token of a partly visible tile is seen by no row of this block.
+    auto unseen = [&](int key) { return key >= v.end || (key < v.low0 && key >= p.sinks); };
+
+    // ---- page tiles: a ring of S stages per warp, filled by the lanes for themselves
+    const uint32_t ring = smem_u32(smem) + (uint32_t)warp * S * T::STAGE;
+    const int q1 = min(i1, v.tiles);
+    const int* table = p.seq.tables + (size_t)seq * p.seq.width;
+    const int sub_mask = (block >> 4) - 1, sub_log = p.cache.log2b - 4;
+    auto tile_of = [&](int item) { return item < v.ns ? item : item - v.ns + v.w0; };
+    auto id_of = [&](int item) {
+        if (item >= q1) return 0;
+        const int page = tile_of(item) >> sub_log;
+        int id = page < p.seq.width ? table[page] : -1;
+        if (!index_in_pool(id, p.cache.num_blocks)) {
+            if (lane == 0) atomicAdd(&g_q8_attn_rejected, 1u);
+            id = 0;
+        }
+        return id;
+    };
+    const size_t page_bytes = (size_t)nkv * block * D;
+    const uint8_t* kbase = p.cache.k + (size_t)h * block * D + g * D + 16 * t;
+    const uint8_t* vbase = p.cache.v + (size_t)h * block * D + 2 * t * D + T::VB * g;
+    auto issue = [&](int item, int id, int stage) {
+        if (item < q1) {
+            const size_t at = (size_t)id * page_bytes + (size_t)(tile_of(item) & sub_mask) * (16 * D);
+            const uint8_t *k = kbase + at, *vv = vbase + at;
+            uint32_t dst = ring + (uint32_t)stage * T::STAGE + lane * 16;
+#pragma unroll
+            for (int j = 0; j < T::KC; ++j) {
+                cp_async16_32(dst + (2 * j) * 512, k + 64 * j);
+                cp_async16_32(dst + (2 * j + 1) * 512, k + 8 * D + 64 * j);
+            }
+            dst += T::K_BYTES - (T::VB == 8 ? lane * 8 : 0);
+#pragma unroll
+            for (int j = 0; j < T::VP; ++j)
+#pragma unroll
+                for (int k4 = 0; k4 < 4; ++k4) {
+                    const uint8_t* src = vv + ((k4 & 1) + (k4 >> 1) * 8) * D + 128 * j;
+                    if constexpr (T::VB == 8) cp_async8(dst + k4 * 256, src);
+                    else cp_async16_32(dst + (4 * j + k4) * 512, src);
+                }
+            cp_async8(ring + (uint32_t)stage * T::STAGE + T::K_BYTES + T::V_BYTES + lane * 8,
+                      p.cache.scales + (size_t)id * nkv + h);
+        }
+        cp_async_commit();
+    };
+    {
+        int ids[S];
+#pragma unroll
+        for (int s = 0; s < S; ++s) ids[s] = id_of(i0 + warp + s * kWarps);
+#pragma unroll
+        for (int s = 0; s < S - 1; ++s) issue(i0 + warp + s * kWarps, ids[s], s);
+        int next_id = ids[S - 1], stage = 0;
+        for (int item = i0 + warp; item < q1; item += kWarps) {
+            issue(item + (S - 1) * kWarps, next_id, stage == 0 ? S - 1 : stage - 1);
+            next_id = id_of(item + S * kWarps);
+            cp_async_wait<S - 1>();
+            const uint32_t src = ring + (uint32_t)stage * T::STAGE + lane * 16;
+            const uint2 sc = lds64(src + T::K_BYTES + T::V_BYTES - lane * 8);
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < T::KC; ++j) {
+                const uint4 a = lds128(src + (2 * j) * 512), b = lds128(src + (2 * j + 1) * 512);
+                const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t a0, a1, a2, a3;
+                    q8_unpack<FMT>(aw[i], a0, a2);
+                    q8_unpack<FMT>(bw[i], a1, a3);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma16816(s[nt], a0, a1, a2, a3, qf[nt][4 * j + i][0], qf[nt][4 * j + i][1]);
+                }
+            }
+            uint32_t pb[NT][2];
+            const int key0 = tile_of(item) * 16;
+            const bool whole = softmax(s, __uint_as_float(sc.x) * p.scale_log2, __uint_as_float(sc.y), key0, item, pb);
+#pragma unroll
+            for (int j = 0; j < T::VP; ++j) {
+                uint32_t w[4][T::VW];
+#pragma unroll
+                for (int k4 = 0; k4 < 4; ++k4) {
+                    if constexpr (T::VB == 8) {
+                        const uint2 x = lds64(src + T::K_BYTES - lane * 8 + k4 * 256);
+                        w[k4][0] = x.x; w[k4][1] = x.y;
+                    } else {
+                        const uint4 x = lds128(src + T::K_BYTES + (4 * j + k4) * 512);
+                        w[k4][0] = x.x; w[k4][1] = x.y; w[k4][2] = x.z; w[k4][3] = x.w;
+                    }
+                    if (!whole && unseen(key0 + 2 * t + (k4 & 1) + (k4 >> 1) * 8)) {
+#pragma unroll
+                        for (int i = 0; i < T::VW; ++i) w[k4][i] = 0u;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < T::VW; ++i) {
+                    uint32_t ab[4], cd[4];
+                    q8_unpack_pairs<FMT>(w[0][i], w[1][i], ab);
+                    q8_unpack_pairs<FMT>(w[2][i], w[3][i], cd);
+                    const int mt = 8 * j + 2 * i;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma16816(o[nt][mt], ab[0], ab[1], cd[0], cd[1], pb[nt][0], pb[nt][1]);
+                        mma16816(o[nt][mt + 1], ab[2], ab[3], cd[2], cd[3], pb[nt][0], pb[nt][1]);
+                    }
+                }
+            }
+            stage = stage == S - 1 ? 0 : stage + 1;
+        }
+    }
+
+    // ---- tail tiles: fp16 rows straight from global memory (at most B / 16 of them per sequence)
+    if (i1 > v.tiles) {
+        int slot = q8_slot(p.seq, seq);
+        if (!index_in_pool(slot, p.cache.num_slots)) {
+            if (lane == 0 && warp == 0) atomicAdd(&g_q8_attn_rejected, 1u);
+            slot = 0;
+        }
+        const __half* kt = p.cache.k_tail + ((size_t)slot * nkv + h) * block * D;
+        const __half* vt = p.cache.v_tail + ((size_t)slot * nkv + h) * block * D;
+        int first = i0 + warp;                    // this warp's items, as in the ring
+        if (first < v.tiles) first += (v.tiles - first + kWarps - 1) / kWarps * kWarps;
+        for (int item = first; item < i1; item += kWarps) {
+            const int r0 = (item - v.tiles) * 16, key0 = v.paged + r0;
+            auto word4 = [&](const __half* base, int row, int chan) {   // 8 channels of a token, zero unless it is seen
+                if (unseen(v.paged + row)) return make_uint4(0u, 0u, 0u, 0u);
+                return *reinterpret_cast<const uint4*>(base + (size_t)row * D + chan);
+            };
+            float s[NT][4];
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < T::KC; ++j)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint4 a = word4(kt, r0 + g, 16 * t + 64 * j + 8 * half), b = word4(kt, r0 + g + 8, 16 * t + 64 * j + 8 * half);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma16816(s[nt], a.x, b.x, a.y, b.y, qf[nt][4 * j + 2 * half][0], qf[nt][4 * j + 2 * half][1]);
+                        mma16816(s[nt], a.z, b.z, a.w, b.w, qf[nt][4 * j + 2 * half + 1][0], qf[nt][4 * j + 2 * half + 1][1]);
+                    }
+                }
+            uint32_t pb[NT][2];
+            softmax(s, p.scale_log2, 1.0f, key0, item, pb);
+#pragma unroll
+            for (int e = 0; e < T::MT / 4; ++e) {   // 8 channels of a token per 16-byte word: output tiles 4 e .. 4 e + 3
+                const int chan = D == 64 ? 8 * g : 16 * g + 8 * (e & 1) + 128 * (e >> 1);
+                uint4 x[4];
+                bool odd = false;
+#pragma unroll
+                for (int k4 = 0; k4 < 4; ++k4) {
+                    x[k4] = word4(vt, r0 + 2 * t + (k4 & 1) + (k4 >> 1) * 8, chan);
+                    const uint32_t w[4] = {x[k4].x, x[k4].y, x[k4].z, x[k4].w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) odd |= (w[i] & 0x7c00u) == 0x7c00u || (w[i] & 0x7c000000u) == 0x7c000000u;
+                }
+                uint32_t a[4][4];                   // [tile][fragment register]
+                auto pairs = [&](const uint4& y0, const uint4& y1, int reg) {
+                    const uint32_t w0[4] = {y0.x, y0.y, y0.z, y0.w}, w1[4] = {y1.x, y1.y, y1.z, y1.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        a[i][reg] = __byte_perm(w0[i], w1[i], 0x5410);
+                        a[i][reg + 1] = __byte_perm(w0[i], w1[i], 0x7632);
+                    }
+                };
+                pairs(x[0], x[1], 0);
+                pairs(x[2], x[3], 2);
+                // An infinity or NaN in V must reach the rows that see its token and no other, but 0 * NaN is NaN: such
+                // elements leave the product, and a second product counts the weight that fell on them.
+                const bool any_odd = __any_sync(0xffffffffu, odd);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t bad[4] = {0u, 0u, 0u, 0u};
+                    if (any_odd) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            if ((a[i][k] & 0x7c00u) == 0x7c00u) { a[i][k] &= 0xffff0000u; bad[k] |= 0x3c00u; }
+                            if ((a[i][k] & 0x7c000000u) == 0x7c000000u) { a[i][k] &= 0x0000ffffu; bad[k] |= 0x3c000000u; }
+                        }
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        mma16816(o[nt][4 * e + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[nt][0], pb[nt][1]);
+                        if (any_odd) {
+                            float hit[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma16816(hit, bad[0], bad[1], bad[2], bad[3], pb[nt][0], pb[nt][1]);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) if (hit[k] != 0.0f) o[nt][4 * e + i][k] = __int_as_float(0x7fc00000);
+                        }
+                    }
+                }
+            }
+        }
+    }
+
+    // ---- merge: the CTA's warps through shared memory (over the ring), then the cluster's CTAs
+    cp_async_wait<0>();
+    const float back = vref / kHeadroom;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float x = l[nt][c];
+            x += __shfl_xor_sync(0xffffffffu, x, 4);
+            x += __shfl_xor_sync(0xffffffffu, x, 8);
+            x += __shfl_xor_sync(0xffffffffu, x, 16);
+            if (g == 0) { s_m[warp][8 * nt + 2 * t + c] = m[nt][c]; s_l[warp][8 * nt + 2 * t + c] = x; }
+        }
+    __syncthreads();                              // rings are drained, states are there
+    float* so = reinterpret_cast<float*>(smem);   // [kWarps][R][D]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            const int r = 8 * nt + 2 * t + c;
+            float top = s_m[0][r];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][r]);
+            const float a = back * fast_exp2(m[nt][c] - top);
+#pragma unroll
+            for (int mt = 0; mt < T::MT; ++mt)
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) so[(warp * R + r) * D + channel_of<D>(g, mt, hf)] = o[nt][mt][2 * hf + c] * a;
+        }
+    if (threadIdx.x < R) {
+        const int r = threadIdx.x;
+        float top = s_m[0][r], sum = 0.0f;
+        for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][r]);
+        for (int w = 0; w < kWarps; ++w) sum += s_l[w][r] * fast_exp2(s_m[w][r] - top);
+        c_m[r] = top; c_l[r] = sum;
+    }
+    __syncthreads();
+    constexpr int VEC = R * D / 4;                // float4 elements of the unit's output
+    float4* sv = reinterpret_cast<float4*>(smem);
+    if (p.parts > 1) {
+        for (int e = threadIdx.x; e < VEC; e += kWarps * 32) {
+            float4 x = sv[e];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) {
+                const float4 y = sv[w * VEC + e];
+                x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+            }
+            sv[e] = x;
+        }
+        cg::this_cluster().sync();
+    }
+    if (threadIdx.x < R) {
+        const int r = threadIdx.x;
+        float top = c_m[r], sum = c_l[r];
+        if (p.parts > 1) {
+            auto cluster = cg::this_cluster();
+            for (int c = 0; c < p.parts; ++c) top = fmaxf(top, *cluster.map_shared_rank(&c_m[r], c));
+            sum = 0.0f;
+            for (int c = 0; c < p.parts; ++c)
+                sum += *cluster.map_shared_rank(&c_l[r], c) * fast_exp2(*cluster.map_shared_rank(&c_m[r], c) - top);
+        }
+        f_m[r] = top;
+        f_il[r] = sum != 0.0f ? 1.0f / sum : 0.0f;   // a row that saw nothing has sum 0 and o 0
+    }
+    __syncthreads();
+    const int ranks = p.parts, share = (VEC + ranks - 1) / ranks;
+    for (int e = part * share + threadIdx.x; e < min(VEC, (part + 1) * share); e += kWarps * 32) {
+        const int r = e / (D / 4), row = rb * R + r;
+        if (row >= rows) continue;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (p.parts > 1) {
+            auto cluster = cg::this_cluster();
+            for (int c = 0; c < p.parts; ++c) {
+                const float a = fast_exp2(*cluster.map_shared_rank(&c_m[r], c) - f_m[r]);
+                const float4 y = *cluster.map_shared_rank(&sv[e], c);
+                x.x += a * y.x; x.y += a * y.y; x.z += a * y.z; x.w += a * y.w;
+            }
+        } else {
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+                const float4 y = sv[w * VEC + e];
+                x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+            }
+        }
+        const float il = f_il[r];
+        x.x *= il; x.y *= il; x.z *= il; x.w *= il;
+        const size_t at = ((size_t)(row0 + row / p.qpk) * nkv * p.qpk + h * p.qpk + row % p.qpk) * D + (e % (D / 4)) * 4;
+        if (p.out_h) *reinterpret_cast<uint2*>(p.out_h + at) = make_uint2(pack_half2(x.x, x.y), pack_half2(x.z, x.w));
+        else *reinterpret_cast<float4*>(p.out + at) = x;
+    }
+    if constexpr (MASS) {
+        // page p's tiles, whichever CTA of the cluster met them (their sums are visible since the cluster's barrier)
+        __syncthreads();
+        const int pages = (v.len + block - 1) >> p.cache.log2b;
+        const float2* ws = p.page_ws + (size_t)(seq * nkv + h) * p.ws_tiles * R;
+        float* mass = p.mass + ((size_t)seq * nkv + h) * p.mass_width;
+        const int top_row = min(R, rows - rb * R);
+        for (int page = part * kWarps * 32 + threadIdx.x; page < pages; page += p.parts * kWarps * 32) {
+            float sum = 0.0f;
+            const int t0 = page << sub_log;
+            for (int k = 0; k <= sub_mask; ++k) {
+                int item;
+                if (t0 * 16 < v.paged) {
+                    const int tile = t0 + k;
+                    if (tile < v.ns) item = tile;
+                    else if (tile >= v.w0 && tile - v.w0 + v.ns < v.tiles) item = tile - v.w0 + v.ns;
+                    else continue;
+                } else {
+                    if (k >= v.tail_tiles) break;
+                    item = v.tiles + k;
+                }
+                for (int r = 0; r < top_row; ++r) {
+                    const float2 x = __ldcg(ws + (size_t)item * R + r);
+                    sum += x.x * fast_exp2(x.y - f_m[r]) * f_il[r];
+                }
+            }
+            if (sum != 0.0f) mass[page] += sum;
+        }
+    }
+    if (p.parts > 1) cg::this_cluster().sync();   // nobody leaves while a peer may still read its shared memory
+}
+
+constexpr int stages_of(int d) { return d == 64 ? 6 : d == 128 ? 4 : 3; }
+
+template <int D, int FMT, int NT, bool MASS>
+cudaError_t launch(const Q8AttnParams& p, cudaStream_t stream) {
+    constexpr int S = stages_of(D);
+    constexpr size_t ring = (size_t)kWarps * S * Tile<D>::STAGE, merge = (size_t)kWarps * 8 * NT * D * 4;
+    constexpr size_t smem = ring > merge ? ring : merge;
+    auto kernel = q8_attention_kernel<D, FMT, NT, MASS, S>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess && p.parts > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((size_t)p.seq.batch * p.cache.nkv * p.row_blocks * p.parts));
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)p.parts;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.parts > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+template <int D, int FMT>
+cudaError_t launch_rows(Q8AttnParams p, bool wide, cudaStream_t stream) {
+    const int r = wide ? 16 : 8, rows = p.max_q * p.qpk, blocks = (rows + r - 1) / r;
+    if (!p.mass) {
+        p.row_blocks = blocks; p.row_block0 = 0;
+        return wide ? launch<D, FMT, 2, false>(p, stream) : launch<D, FMT, 1, false>(p, stream);
+    }
+    // page masses of a kv head grow by one block of query heads at a time: its own launch, so nothing races
+    p.row_blocks = 1;
+    for (p.row_block0 = 0; p.row_block0 < blocks; ++p.row_block0) {
+        const cudaError_t e = wide ? launch<D, FMT, 2, true>(p, stream) : launch<D, FMT, 1, true>(p, stream);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+// Tiles of the longest unit the launch allows.
+int most_tiles(const Q8Cache& c, int max_q, int max_seq, int window, int sinks) {
+    const int block = 1 << c.log2b;
+    long long keys = max_seq;
+    if (window != 0x7fffffff && (long long)window + max_q + sinks + 48 < keys) keys = (long long)window + max_q + sinks + 48;
+    (void)block;
+    return (int)((keys + 15) / 16) + 2;
+}
+
+// Parts a unit's context is cut into: a power of two up to 16, the CTAs of a cluster. A part should keep two tiles per
+// warp, and cutting stops when the units fill the resident slots (three CTAs per multiprocessor).
+int plan_parts(long long units, int tiles) {
+    int parts = 1;
+    while (parts < 16 && units * parts * 2 <= 3LL * sm_count() && tiles >= parts * 2 * kWarps) parts *= 2;
+    return parts;
+}
+
+}  // namespace
+
+size_t q8_attention_workspace(const Q8Cache& c, int qpk, int batch, int max_q, int max_seq, int window, int sinks, bool mass) {
+    if (!mass) return 0;
+    const int r = qpk > 8 ? 16 : 8;
+    return (size_t)batch * c.nkv * most_tiles(c, max_q, max_seq, window, sinks) * r * sizeof(float2);
+}
+
+cudaError_t launch_q8_attention(const Q8AttnParams& args, int d, int fmt, cudaStream_t stream) {
+    Q8AttnParams p = args;
+    const int rows = p.max_q * p.qpk;
+    const bool wide = rows > 8;
+    p.ws_tiles = most_tiles(p.cache, p.max_q, p.max_seq, p.window, p.sinks);
+    const long long blocks = p.mass ? 1 : (rows + (wide ? 15 : 7)) / (wide ? 16 : 8);
+    p.parts = plan_parts((long long)p.seq.batch * p.cache.nkv * blocks, p.ws_tiles);
+    const bool i8 = fmt == KIVI_Q8_INT8;
+    switch (d) {
+        case 64: return i8 ? launch_rows<64, KIVI_Q8_INT8>(p, wide, stream) : launch_rows<64, KIVI_Q8_E4M3>(p, wide, stream);
+        case 128: return i8 ? launch_rows<128, KIVI_Q8_INT8>(p, wide, stream) : launch_rows<128, KIVI_Q8_E4M3>(p, wide, stream);
+        default: return i8 ? launch_rows<256, KIVI_Q8_INT8>(p, wide, stream) : launch_rows<256, KIVI_Q8_E4M3>(p, wide, stream);
+    }
+}
+
+cudaError_t q8_attention_rejected(unsigned int* count) { return cudaMemcpyFromSymbol(count, g_q8_attn_rejected, sizeof(*count)); }
+
+}  // namespace kivi

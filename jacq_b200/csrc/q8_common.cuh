@@ -1,0 +1,107 @@
+// Shared by the kernels of the 8-bit block-scaled cache: its pointers, how a launch finds a sequence, conversions.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "kivi_common.cuh"
+
+namespace kivi {
+
+constexpr float kQ8RecipInt8 = 1.0f / 127.0f;
+constexpr float kQ8RecipE4m3 = 1.0f / 448.0f;
+
+struct Q8Cache {
+    uint8_t* k; uint8_t* v;        // [num_blocks, NKV, B, D] codes
+    float2* scales;                // [num_blocks, NKV] (K, V)
+    __half* k_tail; __half* v_tail;  // [num_slots, NKV, B, D]
+    int num_blocks, num_slots;
+    int nkv, log2b;
+};
+
+struct Q8Seqs {
+    const int* tables; int width;  // [batch, width]
+    const int* lens;               // [batch]
+    const int* slots;              // [batch] or nullptr: slot i
+    int batch;
+};
+
+__device__ __forceinline__ int q8_slot(const Q8Seqs& s, int i) { return s.slots ? s.slots[i] : i; }
+
+// Sequences and ids a launch refused (kivi_b200_q8_rejected_indices adds the files' counters up).
+cudaError_t q8_cache_rejected(unsigned int* count);
+cudaError_t q8_attention_rejected(unsigned int* count);
+
+// Two codes (the low 16 bits of `codes`) as a pair of fp16 values; every e4m3 value is an fp16 value.
+__device__ __forceinline__ uint32_t q8_e4m3_pair(uint16_t codes) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(codes));
+    return r;
+}
+// Two int8 codes that were biased to 1024 + 128 + code by a byte permute under 0x64: minus 1152 is exact.
+__device__ __forceinline__ uint32_t q8_int8_pair(uint32_t biased) {
+    const __half2 bias = __halves2half2(__ushort_as_half((unsigned short)0xE480), __ushort_as_half((unsigned short)0xE480));
+    const __half2 x = __hadd2(*reinterpret_cast<const __half2*>(&biased), bias);
+    return *reinterpret_cast<const uint32_t*>(&x);
+}
+
+// Codes c0 c1 c2 c3 of one word as the pairs (c0, c1) and (c2, c3).
+template <int FMT>
+__device__ __forceinline__ void q8_unpack(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if constexpr (FMT == KIVI_Q8_INT8) {
+        w ^= 0x80808080u;
+        lo = q8_int8_pair(__byte_perm(w, 0x64646464u, 0x4140));
+        hi = q8_int8_pair(__byte_perm(w, 0x64646464u, 0x4342));
+    } else {
+        lo = q8_e4m3_pair((uint16_t)w);
+        hi = q8_e4m3_pair((uint16_t)(w >> 16));
+    }
+}
+
+// Words a and b of two tokens, the same four channels: pairs (a_c, b_c) for c = 0 .. 3.
+template <int FMT>
+__device__ __forceinline__ void q8_unpack_pairs(uint32_t a, uint32_t b, uint32_t (&p)[4]) {
+    const uint32_t x = __byte_perm(a, b, 0x5140), y = __byte_perm(a, b, 0x7362);
+    q8_unpack<FMT>(x, p[0], p[1]);
+    q8_unpack<FMT>(y, p[2], p[3]);
+}
+
+// Host launchers.
+struct Q8WriteParams {
+    Q8Cache cache; Q8Seqs seq;     // seq.lens: tokens before the call
+    const __half* new_k; const __half* new_v;
+    long long k_stride, v_stride;
+    const int* offsets;
+    int total_new, max_new, max_start;
+};
+struct Q8ReadParams {
+    Q8Cache cache; Q8Seqs seq;
+    const int* offsets; const int* first;
+    int total_rows, max_rows;
+    __half* k_out; __half* v_out;
+};
+struct Q8AttnParams {
+    Q8Cache cache; Q8Seqs seq;
+    const __half* q; long long q_stride;
+    const int* q_offsets;          // or nullptr: one row each
+    int total_q, max_q, max_seq;
+    int qpk, window, sinks;        // window 0x7fffffff: none
+    float scale_log2;              // scale * log2(e)
+    float* mass; int mass_width;
+    float2* page_ws; int ws_tiles; // mass: (sum, maximum) of every visited 16-token tile, per row
+    float* out; __half* out_h;
+    int parts, row_blocks, row_block0;
+};
+struct Q8EvictParams {
+    const int* tables; int width;
+    const int* lens; const float* mass; int mass_width;
+    int nkv, log2b, batch, max_seq, budget, first, recent;
+    int* new_tables; int* new_lens; float* new_mass; int* freed; int* freed_counts;
+};
+cudaError_t launch_q8_write(const Q8WriteParams& p, int d, int fmt, cudaStream_t stream);
+cudaError_t launch_q8_read(const Q8ReadParams& p, int d, int fmt, cudaStream_t stream);
+cudaError_t launch_q8_attention(const Q8AttnParams& p, int d, int fmt, cudaStream_t stream);
+size_t q8_attention_workspace(const Q8Cache& c, int qpk, int batch, int max_q, int max_seq, int window, int sinks, bool mass);
+cudaError_t launch_q8_evict(const Q8EvictParams& p, cudaStream_t stream);
+int q8_evict_max_pages();
+
+}  // namespace kivi
