@@ -7,11 +7,12 @@
 // mma.sync m16n8k16 with tokens (QK) and channels (PV) as the 16 side and the query rows as the 8 side. What bounds a
 // single-token call is HBM: 2 D bytes per token and kv head against 4 D flops per query row.
 //
-// No shared-memory tile is exchanged between lanes. The order of the contraction index is free, and so is the order of
-// the output channels, so lane (g, t) = (lane / 4, lane % 4) takes of a 16-token tile exactly the bytes its fragments
-// need, in 16-byte pieces: K rows g and g + 8, channels 16 (t + 4 j) ..; V tokens 2t, 2t+1, 2t+8, 2t+9, channels
-// (D / 8) g .. . Every warp-level copy covers whole 32-byte sectors, a lane reads back only what it asked for itself,
-// and cp.async's per-thread groups are the only synchronisation of the ring.
+// The order of the contraction index is free, and so is the order of the output channels, so lane (g, t) = (lane / 4,
+// lane % 4) takes of a 16-token tile the bytes its fragments need in 16-byte pieces: K rows g and g + 8, channels
+// 16 (t + 4 j) ..; V tokens 2t, 2t+1, 2t+8, 2t+9, channels (D / 8) g .. . The warp copies a tile as whole 128-byte lines
+// into its own ring (copying the pieces straight to the lanes that use them, in half lines, capped the kernel at
+// 5.0 TB/s however many warps there were), under a swizzle that frees the reads of bank conflicts; cp.async groups and
+// __syncwarp are the only synchronisation.
 //
 // A sequence's context is cut into `parts`, one CTA each, that form a thread-block cluster: they merge through
 // distributed shared memory, so a call needs no second launch and no workspace.
@@ -25,7 +26,6 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarps = 4;
 constexpr float kUnset = -3.0e38f;     // running maximum before any visible token
 constexpr float kLazy = 8.0f;          // the maximum is raised when a score tops it by 2^8
 constexpr float kHeadroom = 64.0f;     // probabilities in fp16 carry 2^6: p vs <= 2^8 2^6 < 65504, 2^20 below 1 stay normal
@@ -46,10 +46,13 @@ struct Tile {
     static constexpr int VP = D == 256 ? 2 : 1;  // pieces of a V row per lane
     static constexpr int VB = D == 64 ? 8 : 16;  // bytes of a piece
     static constexpr int VW = VB / 4;            // words (4 channels) of a piece
-    static constexpr int K_BYTES = 2 * KC * 512;
-    static constexpr int V_BYTES = 4 * VP * VB * 32;
-    static constexpr int SCALE_BYTES = 256;      // every lane its own copy: nothing is exchanged
-    static constexpr int STAGE = K_BYTES + V_BYTES + SCALE_BYTES;
+    static constexpr int BYTES = 16 * D;         // K or V codes of a tile
+    static constexpr int CPR = D / 16;           // 16-byte chunks of a row
+    static constexpr int STAGE = 2 * BYTES + 16; // K, V, scales
+    // A row's chunks are stored under an exclusive or with a function of the row, so that the reads below spread over
+    // the banks: K reads touch rows g and chunks t + 4 j, V reads rows 2 t .. and chunks g.
+    static __device__ __forceinline__ int k_swizzle(int row) { return D == 64 ? 0 : (row & 1) << 2; }
+    static __device__ __forceinline__ int v_swizzle(int row) { return D == 64 ? (row >> 1) & 3 : ((row >> 1) & 3) << 1; }
 };
 
 // Channel of output tile mt, half hf (rows g / g + 8 of the fragment) on lanes of group g.
@@ -86,8 +89,11 @@ __device__ __forceinline__ View make_view(const Q8AttnParams& p, int len, int n,
     return v;
 }
 
-template <int D, int FMT, int NT, bool MASS, int S>
-__global__ void __launch_bounds__(kWarps * 32) q8_attention_kernel(const Q8AttnParams p) {
+constexpr int stages_of(int d) { return d == 64 ? 4 : 3; }
+constexpr int ctas_of(int d, int nt) { return d == 64 ? (nt == 1 ? 5 : 4) : d == 128 ? (nt == 1 ? 4 : 3) : 2; }
+
+template <int D, int FMT, int NT, bool MASS, int kWarps, int S>
+__global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? ctas_of(D, NT) : 1) q8_attention_kernel(const Q8AttnParams p) {
     using T = Tile<D>;
     constexpr int R = 8 * NT;
     extern __shared__ __align__(16) unsigned char smem[];
@@ -208,16 +214,14 @@ __global__ void __launch_bounds__(kWarps * 32) q8_attention_kernel(const Q8AttnP
             l[nt][0] += e[0] + e[2];
             l[nt][1] += e[1] + e[3];
             if constexpr (MASS) {
-                float a = e[0] + e[2], b = e[1] + e[3];
-#pragma unroll
-                for (int x = 4; x < 32; x *= 2) {
-                    a += __shfl_xor_sync(0xffffffffu, a, x);
-                    b += __shfl_xor_sync(0xffffffffu, b, x);
-                }
-                if (g == 0) {
-                    float4* dst = reinterpret_cast<float4*>(p.page_ws + ((size_t)(seq * nkv + h) * p.ws_tiles + item) * R + 8 * nt + 2 * t);
-                    *dst = make_float4(a, m[nt][0], b, m[nt][1]);
-                }
+                // sums over the 16 tokens: lanes of even g end up with column 2t's, those of odd g with column 2t + 1's
+                const bool odd = g & 1;
+                const float a = e[0] + e[2], b = e[1] + e[3];
+                float x = (odd ? b : a) + __shfl_xor_sync(0xffffffffu, odd ? a : b, 4);
+                x += __shfl_xor_sync(0xffffffffu, x, 8);
+                x += __shfl_xor_sync(0xffffffffu, x, 16);
+                if (g < 2)
+                    p.page_ws[((size_t)(seq * nkv + h) * p.ws_tiles + item) * R + 8 * nt + 2 * t + g] = make_float2(x, g ? m[nt][1] : m[nt][0]);
             }
             // a probability of a masked key is 0 whatever the page's scale is
             if (!whole) {
@@ -241,62 +245,68 @@ __global__ void __launch_bounds__(kWarps * 32) q8_attention_kernel(const Q8AttnP
     const int* table = p.seq.tables + (size_t)seq * p.seq.width;
     const int sub_mask = (block >> 4) - 1, sub_log = p.cache.log2b - 4;
     auto tile_of = [&](int item) { return item < v.ns ? item : item - v.ns + v.w0; };
-    auto id_of = [&](int item) {
-        if (item >= q1) return 0;
-        const int page = tile_of(item) >> sub_log;
-        int id = page < p.seq.width ? table[page] : -1;
-        if (!index_in_pool(id, p.cache.num_blocks)) {
-            if (lane == 0) atomicAdd(&g_q8_attn_rejected, 1u);
-            id = 0;
-        }
+    // Page ids of the warp's tiles, 32 at a time, one per lane, a block of 32 ahead of their use: the load's latency and
+    // the check against the pool are paid once per 32 tiles.
+    auto load_ids = [&](int k0) {
+        const int item = i0 + warp + (k0 + lane) * kWarps;
+        const int page = item < q1 ? tile_of(item) >> sub_log : 0;
+        return item < q1 && page < p.seq.width ? table[page] : item < q1 ? -1 : 0;
+    };
+    auto checked = [&](int id) {
+        if (!index_in_pool(id, p.cache.num_blocks)) { atomicAdd(&g_q8_attn_rejected, 1u); id = 0; }
         return id;
     };
     const size_t page_bytes = (size_t)nkv * block * D;
-    const uint8_t* kbase = p.cache.k + (size_t)h * block * D + g * D + 16 * t;
-    const uint8_t* vbase = p.cache.v + (size_t)h * block * D + 2 * t * D + T::VB * g;
+    const uint8_t* kbase = p.cache.k + (size_t)h * block * D + lane * 16;
+    const uint8_t* vbase = p.cache.v + (size_t)h * block * D + lane * 16;
+    // chunk 32 i + lane of a tile: row (32 i + lane) / CPR; rows of later i are a multiple of 2 on (of 8 at D = 64, where
+    // the swizzle depends on three bits of the row; of 4 and 2 at D = 128 and 256)
+    auto swizzled = [&](int i, bool is_v) {
+        const int row = (32 * i + lane) / T::CPR, chunk = lane % T::CPR;
+        return (uint32_t)(row * D + ((chunk ^ (is_v ? T::v_swizzle(row) : T::k_swizzle(row))) << 4));
+    };
     auto issue = [&](int item, int id, int stage) {
         if (item < q1) {
-            const size_t at = (size_t)id * page_bytes + (size_t)(tile_of(item) & sub_mask) * (16 * D);
+            const size_t at = (size_t)id * page_bytes + (size_t)(tile_of(item) & sub_mask) * T::BYTES;
             const uint8_t *k = kbase + at, *vv = vbase + at;
-            uint32_t dst = ring + (uint32_t)stage * T::STAGE + lane * 16;
+            const uint32_t dst = ring + (uint32_t)stage * T::STAGE;
 #pragma unroll
-            for (int j = 0; j < T::KC; ++j) {
-                cp_async16_32(dst + (2 * j) * 512, k + 64 * j);
-                cp_async16_32(dst + (2 * j + 1) * 512, k + 8 * D + 64 * j);
-            }
-            dst += T::K_BYTES - (T::VB == 8 ? lane * 8 : 0);
+            for (int i = 0; i < T::BYTES / 512; ++i) cp_async16_32(dst + swizzled(i, false), k + 512 * i);
 #pragma unroll
-            for (int j = 0; j < T::VP; ++j)
-#pragma unroll
-                for (int k4 = 0; k4 < 4; ++k4) {
-                    const uint8_t* src = vv + ((k4 & 1) + (k4 >> 1) * 8) * D + 128 * j;
-                    if constexpr (T::VB == 8) cp_async8(dst + k4 * 256, src);
-                    else cp_async16_32(dst + (4 * j + k4) * 512, src);
-                }
-            cp_async8(ring + (uint32_t)stage * T::STAGE + T::K_BYTES + T::V_BYTES + lane * 8,
-                      p.cache.scales + (size_t)id * nkv + h);
+            for (int i = 0; i < T::BYTES / 512; ++i) cp_async16_32(dst + T::BYTES + swizzled(i, true), vv + 512 * i);
+            if (lane == 0) cp_async8(dst + 2 * T::BYTES, p.cache.scales + (size_t)id * nkv + h);
         }
         cp_async_commit();
     };
+    // where this lane's pieces lie in a stage
+    const uint32_t k_at = g * D + ((t ^ T::k_swizzle(g)) << 4);
+    const uint32_t v_at = T::BYTES + 2 * t * D + (D == 64 ? (((g >> 1) ^ T::v_swizzle(2 * t)) << 4) + (g & 1) * 8 : (g ^ T::v_swizzle(2 * t)) << 4);
     {
-        int ids[S];
+        int ids = checked(load_ids(0)), ids_next = load_ids(32), asked = 0;
+        auto issue_next = [&](int stage) {
+            const int id = __shfl_sync(0xffffffffu, ids, asked & 31);
+            issue(i0 + warp + asked * kWarps, id, stage);
+            if ((++asked & 31) == 0) { ids = checked(ids_next); ids_next = load_ids(asked + 32); }
+        };
 #pragma unroll
-        for (int s = 0; s < S; ++s) ids[s] = id_of(i0 + warp + s * kWarps);
-#pragma unroll
-        for (int s = 0; s < S - 1; ++s) issue(i0 + warp + s * kWarps, ids[s], s);
-        int next_id = ids[S - 1], stage = 0;
+        for (int s = 0; s < S - 1; ++s) issue_next(s);
+        int stage = 0;
         for (int item = i0 + warp; item < q1; item += kWarps) {
-            issue(item + (S - 1) * kWarps, next_id, stage == 0 ? S - 1 : stage - 1);
-            next_id = id_of(item + S * kWarps);
+            issue_next(stage == 0 ? S - 1 : stage - 1);
             cp_async_wait<S - 1>();
-            const uint32_t src = ring + (uint32_t)stage * T::STAGE + lane * 16;
-            const uint2 sc = lds64(src + T::K_BYTES + T::V_BYTES - lane * 8);
-            float s[NT][4];
+            __syncwarp();                          // the other lanes' copies have landed too
+            const uint32_t src = ring + (uint32_t)stage * T::STAGE;
+            const uint2 sc = lds64(src + 2 * T::BYTES);
+            float s[NT][4], s2[NT][4];   // two sums, so that half as many products wait on one another
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.0f;
 #pragma unroll
             for (int j = 0; j < T::KC; ++j) {
-                const uint4 a = lds128(src + (2 * j) * 512), b = lds128(src + (2 * j + 1) * 512);
+                // piece t + 4 j: the swizzle flips bit 2 of the chunk, that is j's low bit
+                const uint32_t at = src + (k_at ^ (uint32_t)((j & 1) << 6)) + (j >> 1) * 128;
+                const uint4 a = lds128(at), b = lds128(at + 8 * D);
                 const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -304,9 +314,14 @@ __global__ void __launch_bounds__(kWarps * 32) q8_attention_kernel(const Q8AttnP
                     q8_unpack<FMT>(aw[i], a0, a2);
                     q8_unpack<FMT>(bw[i], a1, a3);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma16816(s[nt], a0, a1, a2, a3, qf[nt][4 * j + i][0], qf[nt][4 * j + i][1]);
+                    for (int nt = 0; nt < NT; ++nt)
+                        mma16816(i & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, qf[nt][4 * j + i][0], qf[nt][4 * j + i][1]);
                 }
             }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[nt][e] += s2[nt][e];
             uint32_t pb[NT][2];
             const int key0 = tile_of(item) * 16;
             const bool whole = softmax(s, __uint_as_float(sc.x) * p.scale_log2, __uint_as_float(sc.y), key0, item, pb);
@@ -316,10 +331,10 @@ __global__ void __launch_bounds__(kWarps * 32) q8_attention_kernel(const Q8AttnP
 #pragma unroll
                 for (int k4 = 0; k4 < 4; ++k4) {
                     if constexpr (T::VB == 8) {
-                        const uint2 x = lds64(src + T::K_BYTES - lane * 8 + k4 * 256);
+                        const uint2 x = lds64(src + v_at + ((k4 & 1) + (k4 >> 1) * 8) * D);
                         w[k4][0] = x.x; w[k4][1] = x.y;
                     } else {
-                        const uint4 x = lds128(src + T::K_BYTES + (4 * j + k4) * 512);
+                        const uint4 x = lds128(src + v_at + ((k4 & 1) + (k4 >> 1) * 8) * D + j * 128);
                         w[k4][0] = x.x; w[k4][1] = x.y; w[k4][2] = x.z; w[k4][3] = x.w;
                     }
                     if (!whole && unseen(key0 + 2 * t + (k4 & 1) + (k4 >> 1) * 8)) {
@@ -341,6 +356,7 @@ __global__ void __launch_bounds__(kWarps * 32) q8_attention_kernel(const Q8AttnP
                 }
             }
             stage = stage == S - 1 ? 0 : stage + 1;
+            __syncwarp();                          // every lane has read the stage that the next copies go to
         }
     }
 
@@ -442,7 +458,9 @@ __global__ void __launch_bounds__(kWarps * 32) q8_attention_kernel(const Q8AttnP
             if (g == 0) { s_m[warp][8 * nt + 2 * t + c] = m[nt][c]; s_l[warp][8 * nt + 2 * t + c] = x; }
         }
     __syncthreads();                              // rings are drained, states are there
-    float* so = reinterpret_cast<float*>(smem);   // [kWarps][R][D]
+    // Accumulators lie in fragment order, [warp][accumulator][lane]: neighbouring lanes in neighbouring banks.
+    constexpr int ACC = NT * T::MT * 4, VEC = ACC * 32;
+    float* so = reinterpret_cast<float*>(smem);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -455,27 +473,25 @@ __global__ void __launch_bounds__(kWarps * 32) q8_attention_kernel(const Q8AttnP
 #pragma unroll
             for (int mt = 0; mt < T::MT; ++mt)
 #pragma unroll
-                for (int hf = 0; hf < 2; ++hf) so[(warp * R + r) * D + channel_of<D>(g, mt, hf)] = o[nt][mt][2 * hf + c] * a;
+                for (int hf = 0; hf < 2; ++hf)
+                    so[warp * VEC + ((nt * T::MT + mt) * 4 + 2 * hf + c) * 32 + lane] = o[nt][mt][2 * hf + c] * a;
         }
     if (threadIdx.x < R) {
         const int r = threadIdx.x;
         float top = s_m[0][r], sum = 0.0f;
+#pragma unroll
         for (int w = 1; w < kWarps; ++w) top = fmaxf(top, s_m[w][r]);
+#pragma unroll
         for (int w = 0; w < kWarps; ++w) sum += s_l[w][r] * fast_exp2(s_m[w][r] - top);
         c_m[r] = top; c_l[r] = sum;
     }
     __syncthreads();
-    constexpr int VEC = R * D / 4;                // float4 elements of the unit's output
-    float4* sv = reinterpret_cast<float4*>(smem);
     if (p.parts > 1) {
         for (int e = threadIdx.x; e < VEC; e += kWarps * 32) {
-            float4 x = sv[e];
+            float x = so[e];
 #pragma unroll
-            for (int w = 1; w < kWarps; ++w) {
-                const float4 y = sv[w * VEC + e];
-                x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-            }
-            sv[e] = x;
+            for (int w = 1; w < kWarps; ++w) x += so[w * VEC + e];
+            so[e] = x;
         }
         cg::this_cluster().sync();
     }
@@ -490,33 +506,46 @@ __global__ void __launch_bounds__(kWarps * 32) q8_attention_kernel(const Q8AttnP
                 sum += *cluster.map_shared_rank(&c_l[r], c) * fast_exp2(*cluster.map_shared_rank(&c_m[r], c) - top);
         }
         f_m[r] = top;
-        f_il[r] = sum != 0.0f ? 1.0f / sum : 0.0f;   // a row that saw nothing has sum 0 and o 0
+        // a row that saw nothing has sum 0 and o 0; rows behind the block's last weigh nothing
+        f_il[r] = sum != 0.0f && rb * R + r < rows ? 1.0f / sum : 0.0f;
     }
     __syncthreads();
-    const int ranks = p.parts, share = (VEC + ranks - 1) / ranks;
-    for (int e = part * share + threadIdx.x; e < min(VEC, (part + 1) * share); e += kWarps * 32) {
-        const int r = e / (D / 4), row = rb * R + r;
+    // An item: 8 consecutive channels (4 accumulator tiles) of one row, in one lane's place; shared out over the cluster.
+    constexpr int ITEMS = NT * 2 * (T::MT / 4) * 32;
+    const int share = (ITEMS + p.parts - 1) / p.parts;
+    for (int e = part * share + threadIdx.x; e < min(ITEMS, (part + 1) * share); e += kWarps * 32) {
+        const int el = e & 31, q4 = (e >> 5) % (T::MT / 4), c = (e >> 5) / (T::MT / 4) & 1, nt = (e >> 5) / (T::MT / 4) >> 1;
+        const int r = 8 * nt + 2 * (el & 3) + c, row = rb * R + r;
         if (row >= rows) continue;
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float x[8];
+        const float* src = so + ((nt * T::MT + 4 * q4) * 4 + c) * 32 + el;   // channel 2 i + hf: 4 i + 2 hf accumulators further
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = 0.0f;
         if (p.parts > 1) {
             auto cluster = cg::this_cluster();
-            for (int c = 0; c < p.parts; ++c) {
-                const float a = fast_exp2(*cluster.map_shared_rank(&c_m[r], c) - f_m[r]);
-                const float4 y = *cluster.map_shared_rank(&sv[e], c);
-                x.x += a * y.x; x.y += a * y.y; x.z += a * y.z; x.w += a * y.w;
+            for (int rank = 0; rank < p.parts; ++rank) {
+                const float a = fast_exp2(*cluster.map_shared_rank(&c_m[r], rank) - f_m[r]);
+                const float* peer = cluster.map_shared_rank(src, rank);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] += a * peer[k * 64];
             }
         } else {
 #pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                const float4 y = sv[w * VEC + e];
-                x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
-            }
+            for (int w = 0; w < kWarps; ++w)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] += src[w * VEC + k * 64];
         }
         const float il = f_il[r];
-        x.x *= il; x.y *= il; x.z *= il; x.w *= il;
-        const size_t at = ((size_t)(row0 + row / p.qpk) * nkv * p.qpk + h * p.qpk + row % p.qpk) * D + (e % (D / 4)) * 4;
-        if (p.out_h) *reinterpret_cast<uint2*>(p.out_h + at) = make_uint2(pack_half2(x.x, x.y), pack_half2(x.z, x.w));
-        else *reinterpret_cast<float4*>(p.out + at) = x;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] *= il;
+        const size_t at = ((size_t)(row0 + row / p.qpk) * nkv * p.qpk + h * p.qpk + row % p.qpk) * D + channel_of<D>(el >> 2, 4 * q4, 0);
+        if (p.out_h) {
+            *reinterpret_cast<uint4*>(p.out_h + at) =
+                make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
+        } else {
+            *reinterpret_cast<float4*>(p.out + at) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(p.out + at + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        }
     }
     if constexpr (MASS) {
         // page p's tiles, whichever CTA of the cluster met them (their sums are visible since the cluster's barrier)
@@ -524,7 +553,6 @@ __global__ void __launch_bounds__(kWarps * 32) q8_attention_kernel(const Q8AttnP
         const int pages = (v.len + block - 1) >> p.cache.log2b;
         const float2* ws = p.page_ws + (size_t)(seq * nkv + h) * p.ws_tiles * R;
         float* mass = p.mass + ((size_t)seq * nkv + h) * p.mass_width;
-        const int top_row = min(R, rows - rb * R);
         for (int page = part * kWarps * 32 + threadIdx.x; page < pages; page += p.parts * kWarps * 32) {
             float sum = 0.0f;
             const int t0 = page << sub_log;
@@ -539,10 +567,11 @@ __global__ void __launch_bounds__(kWarps * 32) q8_attention_kernel(const Q8AttnP
                     if (k >= v.tail_tiles) break;
                     item = v.tiles + k;
                 }
-                for (int r = 0; r < top_row; ++r) {
-                    const float2 x = __ldcg(ws + (size_t)item * R + r);
-                    sum += x.x * fast_exp2(x.y - f_m[r]) * f_il[r];
-                }
+                float2 x[R];
+#pragma unroll
+                for (int r = 0; r < R; ++r) x[r] = __ldcg(ws + (size_t)item * R + r);
+#pragma unroll
+                for (int r = 0; r < R; ++r) sum += x[r].x * fast_exp2(x[r].y - f_m[r]) * f_il[r];
             }
             if (sum != 0.0f) mass[page] += sum;
         }
@@ -550,14 +579,12 @@ __global__ void __launch_bounds__(kWarps * 32) q8_attention_kernel(const Q8AttnP
     if (p.parts > 1) cg::this_cluster().sync();   // nobody leaves while a peer may still read its shared memory
 }
 
-constexpr int stages_of(int d) { return d == 64 ? 6 : d == 128 ? 4 : 3; }
-
-template <int D, int FMT, int NT, bool MASS>
+template <int D, int FMT, int NT, bool MASS, int kWarps>
 cudaError_t launch(const Q8AttnParams& p, cudaStream_t stream) {
     constexpr int S = stages_of(D);
     constexpr size_t ring = (size_t)kWarps * S * Tile<D>::STAGE, merge = (size_t)kWarps * 8 * NT * D * 4;
     constexpr size_t smem = ring > merge ? ring : merge;
-    auto kernel = q8_attention_kernel<D, FMT, NT, MASS, S>;
+    auto kernel = q8_attention_kernel<D, FMT, NT, MASS, kWarps, S>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e == cudaSuccess && p.parts > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
@@ -575,17 +602,23 @@ cudaError_t launch(const Q8AttnParams& p, cudaStream_t stream) {
     return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 
+template <int D, int FMT, bool MASS>
+cudaError_t launch_shape(const Q8AttnParams& p, bool wide, int warps, cudaStream_t stream) {
+    if (warps == 4) return wide ? launch<D, FMT, 2, MASS, 4>(p, stream) : launch<D, FMT, 1, MASS, 4>(p, stream);
+    return wide ? launch<D, FMT, 2, MASS, 8>(p, stream) : launch<D, FMT, 1, MASS, 8>(p, stream);
+}
+
 template <int D, int FMT>
-cudaError_t launch_rows(Q8AttnParams p, bool wide, cudaStream_t stream) {
+cudaError_t launch_rows(Q8AttnParams p, bool wide, int warps, cudaStream_t stream) {
     const int r = wide ? 16 : 8, rows = p.max_q * p.qpk, blocks = (rows + r - 1) / r;
     if (!p.mass) {
         p.row_blocks = blocks; p.row_block0 = 0;
-        return wide ? launch<D, FMT, 2, false>(p, stream) : launch<D, FMT, 1, false>(p, stream);
+        return launch_shape<D, FMT, false>(p, wide, warps, stream);
     }
     // page masses of a kv head grow by one block of query heads at a time: its own launch, so nothing races
     p.row_blocks = 1;
     for (p.row_block0 = 0; p.row_block0 < blocks; ++p.row_block0) {
-        const cudaError_t e = wide ? launch<D, FMT, 2, true>(p, stream) : launch<D, FMT, 1, true>(p, stream);
+        const cudaError_t e = launch_shape<D, FMT, true>(p, wide, warps, stream);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -602,10 +635,11 @@ int most_tiles(const Q8Cache& c, int max_q, int max_seq, int window, int sinks) 
 
 // Parts a unit's context is cut into: a power of two up to 16, the CTAs of a cluster. A part should keep two tiles per
 // warp, and cutting stops when the units fill the resident slots (three CTAs per multiprocessor).
-int plan_parts(long long units, int tiles) {
-    int parts = 1;
-    while (parts < 16 && units * parts * 2 <= 3LL * sm_count() && tiles >= parts * 2 * kWarps) parts *= 2;
-    return parts;
+void plan(long long units, int tiles, int& parts, int& warps) {
+    parts = 1; warps = 4;
+    while (parts < 16 && units * parts * 2 <= 3LL * sm_count() && tiles >= parts * 8) parts *= 2;
+    if (const char* e = getenv("KIVI_Q8_PARTS")) parts = atoi(e);
+    if (const char* e = getenv("KIVI_Q8_WARPS")) warps = atoi(e);
 }
 
 }  // namespace
@@ -622,12 +656,13 @@ cudaError_t launch_q8_attention(const Q8AttnParams& args, int d, int fmt, cudaSt
     const bool wide = rows > 8;
     p.ws_tiles = most_tiles(p.cache, p.max_q, p.max_seq, p.window, p.sinks);
     const long long blocks = p.mass ? 1 : (rows + (wide ? 15 : 7)) / (wide ? 16 : 8);
-    p.parts = plan_parts((long long)p.seq.batch * p.cache.nkv * blocks, p.ws_tiles);
+    int warps;
+    plan((long long)p.seq.batch * p.cache.nkv * blocks, p.ws_tiles, p.parts, warps);
     const bool i8 = fmt == KIVI_Q8_INT8;
     switch (d) {
-        case 64: return i8 ? launch_rows<64, KIVI_Q8_INT8>(p, wide, stream) : launch_rows<64, KIVI_Q8_E4M3>(p, wide, stream);
-        case 128: return i8 ? launch_rows<128, KIVI_Q8_INT8>(p, wide, stream) : launch_rows<128, KIVI_Q8_E4M3>(p, wide, stream);
-        default: return i8 ? launch_rows<256, KIVI_Q8_INT8>(p, wide, stream) : launch_rows<256, KIVI_Q8_E4M3>(p, wide, stream);
+        case 64: return i8 ? launch_rows<64, KIVI_Q8_INT8>(p, wide, warps, stream) : launch_rows<64, KIVI_Q8_E4M3>(p, wide, warps, stream);
+        case 128: return i8 ? launch_rows<128, KIVI_Q8_INT8>(p, wide, warps, stream) : launch_rows<128, KIVI_Q8_E4M3>(p, wide, warps, stream);
+        default: return i8 ? launch_rows<256, KIVI_Q8_INT8>(p, wide, warps, stream) : launch_rows<256, KIVI_Q8_E4M3>(p, wide, warps, stream);
     }
 }
 
