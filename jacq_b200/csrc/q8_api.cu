@@ -116,10 +116,8 @@ extern "C" size_t kivi_b200_q8_attention_workspace_bytes(const kivi_q8_geometry*
                                                          int max_seq_len, int window, int sinks, int with_mass) {
     if (check_q8_geometry(geom) != KIVI_OK || batch < 1 || batch > kQ8MaxBatch || max_q_per_seq < 1 || max_seq_len < 0 ||
         max_seq_len > kQ8MaxLen || window < 0 || sinks < 0 || !q8_grid_fits(geom, batch, max_q_per_seq)) return 0;
-    Q8Cache c = {};
-    c.nkv = geom->num_kv_heads; c.log2b = q8_log2(geom->block_size);
-    return q8_attention_workspace(c, geom->num_q_heads / geom->num_kv_heads, batch, max_q_per_seq, max_seq_len,
-                                  window_of(window), sinks, with_mass != 0);
+    return q8_attention_workspace(geom->num_kv_heads, geom->num_q_heads / geom->num_kv_heads, geom->head_dim, geom->block_size, batch, max_q_per_seq,
+                                  max_seq_len, window_of(window), sinks, with_mass != 0);
 }
 
 extern "C" int kivi_b200_q8_attention(const kivi_q8_geometry* geom, const kivi_q8_cache* cache, const kivi_f16* q,
@@ -155,12 +153,14 @@ extern "C" int kivi_b200_q8_attention(const kivi_q8_geometry* geom, const kivi_q
         if (q_offsets) return KIVI_ERR_RANGE;
         if ((int64_t)mass_width * geom->block_size < max_seq_len) return KIVI_ERR_RANGE;
         p.mass = page_mass; p.mass_width = mass_width;
-        const size_t need = q8_attention_workspace(p.cache, p.qpk, batch, 1, max_seq_len, p.window, sinks, true);
+    }
+    const size_t need = q8_attention_workspace(geom->num_kv_heads, p.qpk, geom->head_dim, geom->block_size, batch, max_q_per_seq, max_seq_len, p.window,
+                                               sinks, page_mass != nullptr);
+    if (need) {
         if (!workspace || workspace_bytes < need) return KIVI_ERR_WORKSPACE;
         if (!q8_aligned16(workspace)) return KIVI_ERR_ALIGNMENT;
-        p.page_ws = static_cast<float2*>(workspace);
     }
-    return launch_q8_attention(p, geom->head_dim, geom->format, stream) == cudaSuccess ? KIVI_OK : KIVI_ERR_CUDA;
+    return launch_q8_attention(p, geom->head_dim, geom->format, workspace, stream) == cudaSuccess ? KIVI_OK : KIVI_ERR_CUDA;
 }
 
 extern "C" int kivi_b200_q8_evict(int num_kv_heads, int block_size, const int32_t* block_tables, int max_blocks_per_seq,

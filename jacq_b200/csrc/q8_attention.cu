@@ -89,40 +89,102 @@ __device__ __forceinline__ View make_view(const Q8AttnParams& p, int len, int n,
     return v;
 }
 
-constexpr int stages_of(int d) { return d == 64 ? 4 : 3; }
-constexpr int ctas_of(int d, int nt) { return d == 64 ? (nt == 1 ? 5 : 4) : d == 128 ? (nt == 1 ? 4 : 3) : 2; }
+// One (sequence, kv head, block of R query rows).
+struct Unit {
+    int seq, h, rb, len, n, row0, rows;
+    View v;
+    int items;          // tiles of the page part and of the tail
+};
+__device__ __forceinline__ Unit make_unit(const Q8AttnParams& p, int unit, int r_per_block) {
+    Unit u;
+    u.rb = unit % p.row_blocks + p.row_block0;
+    unit /= p.row_blocks;
+    u.h = unit % p.cache.nkv; u.seq = unit / p.cache.nkv;
+    u.len = min(max(p.seq.lens[u.seq], 0), p.max_seq);
+    u.row0 = u.seq; u.n = 1;
+    if (p.q_offsets) {
+        u.row0 = p.q_offsets[u.seq];
+        u.n = min(p.q_offsets[u.seq + 1] - u.row0, p.max_q);
+        if (u.row0 < 0 || u.n < 0 || u.row0 > p.total_q - u.n) u.n = 0;
+    }
+    u.rows = u.n * p.qpk;
+    const int first = u.rb * r_per_block, last = min(first + r_per_block, u.rows) - 1;
+    u.v = make_view(p, u.len, u.n, first / p.qpk, max(last, 0) / p.qpk);
+    u.items = u.v.tiles + u.v.tail_tiles;
+    return u;
+}
 
-template <int D, int FMT, int NT, bool MASS, int kWarps, int S>
-__global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? ctas_of(D, NT) : 1) q8_attention_kernel(const Q8AttnParams p) {
+// Where row `row` of a unit's output starts, in elements.
+__device__ __forceinline__ size_t out_at(const Q8AttnParams& p, const Unit& u, int row, int d) {
+    return ((size_t)(u.row0 + row / p.qpk) * p.cache.nkv * p.qpk + u.h * p.qpk + row % p.qpk) * d;
+}
+__device__ __forceinline__ void store8(const Q8AttnParams& p, size_t at, const float (&x)[8]) {
+    if (p.out_h) {
+        *reinterpret_cast<uint4*>(p.out_h + at) =
+            make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
+    } else {
+        *reinterpret_cast<float4*>(p.out + at) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(p.out + at + 4) = make_float4(x[4], x[5], x[6], x[7]);
+    }
+}
+
+// Adds to the masses of pages first, first + step, ...: page p's tiles, whichever part met them, relative to the unit's
+// final maximum f_m and 1 / sum f_il of every row.
+template <int R>
+__device__ __forceinline__ void add_masses(const Q8AttnParams& p, const Unit& u, const float* f_m, const float* f_il, int first, int step) {
+    const int sub_log = p.cache.log2b - 4, subs = 1 << sub_log;
+    const int pages = (u.len + (1 << p.cache.log2b) - 1) >> p.cache.log2b;
+    const float2* ws = p.page_ws + (size_t)(u.seq * p.cache.nkv + u.h) * p.ws_tiles * R;
+    float* mass = p.mass + ((size_t)u.seq * p.cache.nkv + u.h) * p.mass_width;
+    for (int page = first; page < pages; page += step) {
+        float sum = 0.0f;
+        const int t0 = page << sub_log;
+        for (int k = 0; k < subs; ++k) {
+            int item;
+            if (t0 * 16 < u.v.paged) {
+                const int tile = t0 + k;
+                if (tile < u.v.ns) item = tile;
+                else if (tile >= u.v.w0 && tile - u.v.w0 + u.v.ns < u.v.tiles) item = tile - u.v.w0 + u.v.ns;
+                else continue;
+            } else {
+                if (k >= u.v.tail_tiles) break;
+                item = u.v.tiles + k;
+            }
+            float2 x[R];
+#pragma unroll
+            for (int r = 0; r < R; ++r) x[r] = __ldcg(ws + (size_t)item * R + r);
+#pragma unroll
+            for (int r = 0; r < R; ++r) sum += x[r].x * fast_exp2(x[r].y - f_m[r]) * f_il[r];
+        }
+        if (sum != 0.0f) mass[page] += sum;
+    }
+}
+
+// Two shapes of the kernel. Four warps and a shallow ring, several CTAs per multiprocessor, where there are units enough
+// to fill it; eight warps and a deep ring, one CTA per multiprocessor, where there are few and each warp's own copies
+// have to cover the latency.
+template <int D, int kWarps>
+constexpr int stages_of() { return kWarps == 4 ? (D == 64 ? 4 : 3) : D == 64 ? 10 : D == 128 ? 6 : 3; }
+template <int D, int kWarps>
+constexpr int ctas_of(int nt) { return kWarps == 8 ? 1 : D == 64 ? (nt == 1 ? 5 : 4) : D == 128 ? (nt == 1 ? 4 : 3) : 2; }
+
+template <int D, int FMT, int NT, bool MASS, int kWarps>
+__global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attention_kernel(const Q8AttnParams p) {
     using T = Tile<D>;
-    constexpr int R = 8 * NT;
+    constexpr int R = 8 * NT, S = stages_of<D, kWarps>();
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float s_m[kWarps][R], s_l[kWarps][R];
     __shared__ float c_m[R], c_l[R];             // this CTA's merged state, read by its cluster
     __shared__ float f_m[R], f_il[R];            // the unit's final maximum and 1 / sum
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int nkv = p.cache.nkv, block = 1 << p.cache.log2b;
-    const int part = blockIdx.x % p.parts;
-    int unit = blockIdx.x / p.parts;
-    const int rb = unit % p.row_blocks + p.row_block0;
-    unit /= p.row_blocks;
-    const int h = unit % nkv, seq = unit / nkv;
-
-    // ---- what this unit is
-    int len = p.seq.lens[seq];
-    len = min(max(len, 0), p.max_seq);
-    int row0 = seq, n = 1;
-    if (p.q_offsets) {
-        row0 = p.q_offsets[seq];
-        n = min(p.q_offsets[seq + 1] - row0, p.max_q);
-        if (row0 < 0 || n < 0 || row0 > p.total_q - n) n = 0;
-    }
-    const int rows = n * p.qpk;
+    const int part = blockIdx.x % p.parts, unit = blockIdx.x / p.parts;
+    const Unit u = make_unit(p, unit, R);
+    const int seq = u.seq, h = u.h, rb = u.rb, len = u.len, n = u.n, row0 = u.row0, rows = u.rows, items = u.items;
+    const View& v = u.v;
     if (rb * R >= rows) return;                  // uniform over the cluster
-    const int tok0 = rb * R / p.qpk, tok1 = min(rb * R + R, rows) - 1;
-    const View v = make_view(p, len, n, tok0, tok1 / p.qpk);
-    const int items = v.tiles + v.tail_tiles;
-    const int i0 = (int)((long long)items * part / p.parts), i1 = (int)((long long)items * (part + 1) / p.parts);
+    const int i0 = min(part * p.chunk, items), i1 = min(i0 + p.chunk, items);
+    if (p.cluster == 0 && i0 == i1 && part > 0) return;   // the merge knows how many parts have something
 
     // ---- query rows as B fragments, in the channel order of the K pieces
     uint32_t qf[NT][T::MT][2];
@@ -486,6 +548,18 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? ctas_of(D, NT) : 1)
         c_m[r] = top; c_l[r] = sum;
     }
     __syncthreads();
+    constexpr int QUADS = T::MT / 4, ITEMS = NT * 2 * QUADS * 32;
+    if (p.parts > 1 && p.cluster == 0) {         // partials for the merge kernel, in the same order
+        const size_t slot = (size_t)unit * p.parts + part;
+        for (int e = threadIdx.x; e < VEC; e += kWarps * 32) {
+            float x = so[e];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) x += so[w * VEC + e];
+            p.part_o[slot * VEC + e] = x;
+        }
+        if (threadIdx.x < R) p.part_ml[slot * R + threadIdx.x] = make_float2(c_m[threadIdx.x], c_l[threadIdx.x]);
+        return;
+    }
     if (p.parts > 1) {
         for (int e = threadIdx.x; e < VEC; e += kWarps * 32) {
             float x = so[e];
@@ -511,10 +585,9 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? ctas_of(D, NT) : 1)
     }
     __syncthreads();
     // An item: 8 consecutive channels (4 accumulator tiles) of one row, in one lane's place; shared out over the cluster.
-    constexpr int ITEMS = NT * 2 * (T::MT / 4) * 32;
     const int share = (ITEMS + p.parts - 1) / p.parts;
     for (int e = part * share + threadIdx.x; e < min(ITEMS, (part + 1) * share); e += kWarps * 32) {
-        const int el = e & 31, q4 = (e >> 5) % (T::MT / 4), c = (e >> 5) / (T::MT / 4) & 1, nt = (e >> 5) / (T::MT / 4) >> 1;
+        const int el = e & 31, q4 = (e >> 5) % QUADS, c = (e >> 5) / QUADS & 1, nt = (e >> 5) / QUADS >> 1;
         const int r = 8 * nt + 2 * (el & 3) + c, row = rb * R + r;
         if (row >= rows) continue;
         float x[8];
@@ -538,58 +611,65 @@ __global__ void __launch_bounds__(kWarps * 32, kWarps == 4 ? ctas_of(D, NT) : 1)
         const float il = f_il[r];
 #pragma unroll
         for (int k = 0; k < 8; ++k) x[k] *= il;
-        const size_t at = ((size_t)(row0 + row / p.qpk) * nkv * p.qpk + h * p.qpk + row % p.qpk) * D + channel_of<D>(el >> 2, 4 * q4, 0);
-        if (p.out_h) {
-            *reinterpret_cast<uint4*>(p.out_h + at) =
-                make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
-        } else {
-            *reinterpret_cast<float4*>(p.out + at) = make_float4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<float4*>(p.out + at + 4) = make_float4(x[4], x[5], x[6], x[7]);
-        }
+        store8(p, out_at(p, u, row, D) + channel_of<D>(el >> 2, 4 * q4, 0), x);
     }
-    if constexpr (MASS) {
-        // page p's tiles, whichever CTA of the cluster met them (their sums are visible since the cluster's barrier)
-        __syncthreads();
-        const int pages = (v.len + block - 1) >> p.cache.log2b;
-        const float2* ws = p.page_ws + (size_t)(seq * nkv + h) * p.ws_tiles * R;
-        float* mass = p.mass + ((size_t)seq * nkv + h) * p.mass_width;
-        for (int page = part * kWarps * 32 + threadIdx.x; page < pages; page += p.parts * kWarps * 32) {
-            float sum = 0.0f;
-            const int t0 = page << sub_log;
-            for (int k = 0; k <= sub_mask; ++k) {
-                int item;
-                if (t0 * 16 < v.paged) {
-                    const int tile = t0 + k;
-                    if (tile < v.ns) item = tile;
-                    else if (tile >= v.w0 && tile - v.w0 + v.ns < v.tiles) item = tile - v.w0 + v.ns;
-                    else continue;
-                } else {
-                    if (k >= v.tail_tiles) break;
-                    item = v.tiles + k;
-                }
-                float2 x[R];
-#pragma unroll
-                for (int r = 0; r < R; ++r) x[r] = __ldcg(ws + (size_t)item * R + r);
-#pragma unroll
-                for (int r = 0; r < R; ++r) sum += x[r].x * fast_exp2(x[r].y - f_m[r]) * f_il[r];
-            }
-            if (sum != 0.0f) mass[page] += sum;
-        }
-    }
+    if constexpr (MASS) add_masses<R>(p, u, f_m, f_il, part * kWarps * 32 + threadIdx.x, p.parts * kWarps * 32);
     if (p.parts > 1) cg::this_cluster().sync();   // nobody leaves while a peer may still read its shared memory
+}
+
+// Joins the parts of a unit that was cut without a cluster. grid (units, slices): slice 0 writes the output, all share
+// the pages' masses out.
+template <int D, int NT, bool MASS>
+__global__ void __launch_bounds__(256) q8_merge_kernel(const Q8AttnParams p) {
+    constexpr int R = 8 * NT, MT = D / 16, VEC = NT * MT * 128, QUADS = MT / 4, ITEMS = NT * 2 * QUADS * 32;
+    __shared__ float f_m[R], f_il[R];
+    const Unit u = make_unit(p, blockIdx.x, R);
+    if (u.rb * R >= u.rows) return;
+    const int live = max(1, (u.items + p.chunk - 1) / p.chunk);
+    const float2* ml = p.part_ml + (size_t)blockIdx.x * p.parts * R;
+    if (threadIdx.x < R) {
+        const int r = threadIdx.x;
+        float top = kUnset, sum = 0.0f;
+        for (int k = 0; k < live; ++k) top = fmaxf(top, ml[k * R + r].x);
+        for (int k = 0; k < live; ++k) sum += ml[k * R + r].y * fast_exp2(ml[k * R + r].x - top);
+        f_m[r] = top;
+        f_il[r] = sum != 0.0f && u.rb * R + r < u.rows ? 1.0f / sum : 0.0f;
+    }
+    __syncthreads();
+    if (blockIdx.y == 0) {
+        for (int e = threadIdx.x; e < ITEMS; e += 256) {
+            const int el = e & 31, q4 = (e >> 5) % QUADS, c = (e >> 5) / QUADS & 1, nt = (e >> 5) / QUADS >> 1;
+            const int r = 8 * nt + 2 * (el & 3) + c, row = u.rb * R + r;
+            if (row >= u.rows) continue;
+            const float* src = p.part_o + (size_t)blockIdx.x * p.parts * VEC + ((nt * MT + 4 * q4) * 4 + c) * 32 + el;
+            float x[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] = 0.0f;
+#pragma unroll 4
+            for (int part = 0; part < live; ++part) {
+                const float a = fast_exp2(ml[part * R + r].x - f_m[r]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] += a * src[(size_t)part * VEC + k * 64];
+            }
+            const float il = f_il[r];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x[k] *= il;
+            store8(p, out_at(p, u, row, D) + channel_of<D>(el >> 2, 4 * q4, 0), x);
+        }
+    }
+    if constexpr (MASS) add_masses<R>(p, u, f_m, f_il, blockIdx.y * 256 + threadIdx.x, gridDim.y * 256);
 }
 
 template <int D, int FMT, int NT, bool MASS, int kWarps>
 cudaError_t launch(const Q8AttnParams& p, cudaStream_t stream) {
-    constexpr int S = stages_of(D);
-    constexpr size_t ring = (size_t)kWarps * S * Tile<D>::STAGE, merge = (size_t)kWarps * 8 * NT * D * 4;
+    constexpr size_t ring = (size_t)kWarps * stages_of<D, kWarps>() * Tile<D>::STAGE, merge = (size_t)kWarps * 8 * NT * D * 4;
     constexpr size_t smem = ring > merge ? ring : merge;
-    auto kernel = q8_attention_kernel<D, FMT, NT, MASS, kWarps, S>;
+    auto kernel = q8_attention_kernel<D, FMT, NT, MASS, kWarps>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess && p.parts > 8) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
     if (e != cudaSuccess) return e;
+    const unsigned units = (unsigned)((size_t)p.seq.batch * p.cache.nkv * p.row_blocks);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)((size_t)p.seq.batch * p.cache.nkv * p.row_blocks * p.parts));
+    cfg.gridDim = dim3(units * p.parts);
     cfg.blockDim = dim3(kWarps * 32);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
@@ -598,8 +678,12 @@ cudaError_t launch(const Q8AttnParams& p, cudaStream_t stream) {
     attr[0].val.clusterDim.x = (unsigned)p.parts;
     attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = p.parts > 1 ? 1 : 0;
-    return cudaLaunchKernelEx(&cfg, kernel, p);
+    cfg.numAttrs = p.cluster ? 1 : 0;
+    e = cudaLaunchKernelEx(&cfg, kernel, p);
+    if (e != cudaSuccess || p.parts == 1 || p.cluster) return e;
+    const unsigned slices = MASS ? (unsigned)((((p.max_seq >> p.cache.log2b) + 1) + 511) / 512) : 1u;
+    q8_merge_kernel<D, NT, MASS><<<dim3(units, slices < 64 ? slices : 64), 256, 0, stream>>>(p);
+    return cudaGetLastError();
 }
 
 template <int D, int FMT, bool MASS>
@@ -624,41 +708,67 @@ cudaError_t launch_rows(Q8AttnParams p, bool wide, int warps, cudaStream_t strea
     return cudaSuccess;
 }
 
-// Tiles of the longest unit the launch allows.
-int most_tiles(const Q8Cache& c, int max_q, int max_seq, int window, int sinks) {
-    const int block = 1 << c.log2b;
-    long long keys = max_seq;
-    if (window != 0x7fffffff && (long long)window + max_q + sinks + 48 < keys) keys = (long long)window + max_q + sinks + 48;
-    (void)block;
-    return (int)((keys + 15) / 16) + 2;
+// Tiles of the longest unit the launch allows: the window of a block of rows, the first tokens, what the two share of
+// tiles at their ends, and the tail, all of whose tiles are visited. Exceeding it would cut units short: View counts the
+// same way.
+int most_tiles(int max_q, int max_seq, int window, int sinks, int block) {
+    const long long whole = max_seq, part = (long long)window + max_q + sinks + block + 48;
+    return (int)(((window != 0x7fffffff && part < whole ? part : whole) + 15) / 16) + 2;
 }
 
-// Parts a unit's context is cut into: a power of two up to 16, the CTAs of a cluster. A part should keep two tiles per
-// warp, and cutting stops when the units fill the resident slots (three CTAs per multiprocessor).
-void plan(long long units, int tiles, int& parts, int& warps) {
-    parts = 1; warps = 4;
-    while (parts < 16 && units * parts * 2 <= 3LL * sm_count() && tiles >= parts * 8) parts *= 2;
+struct Plan {
+    bool wide;                 // 16 query rows per unit, else 8
+    int tiles, units;          // of the longest unit; units of a launch
+    int parts, chunk, cluster, warps;
+    size_t page_ws, part_ml, part_o, total;   // workspace: offsets and size
+};
+
+Plan make_plan(int nkv, int qpk, int d, int block, int batch, int max_q, int max_seq, int window, int sinks, bool mass) {
+    Plan q = {};
+    const int rows = max_q * qpk;
+    q.wide = rows > 8;
+    const int r = q.wide ? 16 : 8;
+    q.tiles = most_tiles(max_q, max_seq, window, sinks, block);
+    const long long units = (long long)batch * nkv * (mass ? 1 : (rows + r - 1) / r);
+    q.units = (int)units;
+    int parts = 1, warps = 4;
+    while (parts < 16 && units * parts * 2 <= 3LL * sm_count() && q.tiles >= parts * 8) parts *= 2;
     if (const char* e = getenv("KIVI_Q8_PARTS")) parts = atoi(e);
     if (const char* e = getenv("KIVI_Q8_WARPS")) warps = atoi(e);
+    q.cluster = parts > 1 && parts <= 8;
+    if (const char* e = getenv("KIVI_Q8_CLUSTER")) q.cluster = parts > 1 && atoi(e);
+    q.parts = parts; q.warps = warps;
+    q.chunk = (q.tiles + parts - 1) / parts;
+    auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+    size_t at = 0;
+    q.page_ws = at;
+    if (mass) at += up((size_t)batch * nkv * q.tiles * r * sizeof(float2));
+    if (parts > 1 && !q.cluster) {
+        q.part_ml = at; at += up((size_t)units * parts * r * sizeof(float2));
+        q.part_o = at; at += up((size_t)units * parts * r * d * sizeof(float));
+    }
+    q.total = at;
+    return q;
 }
 
 }  // namespace
 
-size_t q8_attention_workspace(const Q8Cache& c, int qpk, int batch, int max_q, int max_seq, int window, int sinks, bool mass) {
-    if (!mass) return 0;
-    const int r = qpk > 8 ? 16 : 8;
-    return (size_t)batch * c.nkv * most_tiles(c, max_q, max_seq, window, sinks) * r * sizeof(float2);
+size_t q8_attention_workspace(int nkv, int qpk, int d, int block, int batch, int max_q, int max_seq, int window, int sinks, bool mass) {
+    return make_plan(nkv, qpk, d, block, batch, max_q, max_seq, window, sinks, mass).total;
 }
 
-cudaError_t launch_q8_attention(const Q8AttnParams& args, int d, int fmt, cudaStream_t stream) {
+cudaError_t launch_q8_attention(const Q8AttnParams& args, int d, int fmt, void* workspace, cudaStream_t stream) {
     Q8AttnParams p = args;
-    const int rows = p.max_q * p.qpk;
-    const bool wide = rows > 8;
-    p.ws_tiles = most_tiles(p.cache, p.max_q, p.max_seq, p.window, p.sinks);
-    const long long blocks = p.mass ? 1 : (rows + (wide ? 15 : 7)) / (wide ? 16 : 8);
-    int warps;
-    plan((long long)p.seq.batch * p.cache.nkv * blocks, p.ws_tiles, p.parts, warps);
+    const Plan plan = make_plan(p.cache.nkv, p.qpk, d, 1 << p.cache.log2b, p.seq.batch, p.max_q, p.max_seq, p.window, p.sinks, p.mass != nullptr);
+    p.ws_tiles = plan.tiles;
+    p.parts = plan.parts; p.chunk = plan.chunk; p.cluster = plan.cluster;
+    unsigned char* ws = static_cast<unsigned char*>(workspace);
+    p.page_ws = reinterpret_cast<float2*>(ws + plan.page_ws);
+    p.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
+    p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
     const bool i8 = fmt == KIVI_Q8_INT8;
+    const bool wide = plan.wide;
+    const int warps = plan.warps;
     switch (d) {
         case 64: return i8 ? launch_rows<64, KIVI_Q8_INT8>(p, wide, warps, stream) : launch_rows<64, KIVI_Q8_E4M3>(p, wide, warps, stream);
         case 128: return i8 ? launch_rows<128, KIVI_Q8_INT8>(p, wide, warps, stream) : launch_rows<128, KIVI_Q8_E4M3>(p, wide, warps, stream);

@@ -88,8 +88,10 @@ struct Q8AttnParams {
     float scale_log2;              // scale * log2(e)
     float* mass; int mass_width;
     float2* page_ws; int ws_tiles; // mass: (sum, maximum) of every visited 16-token tile, per row
+    float2* part_ml; float* part_o; // parts without a cluster: state and accumulators of every (unit, part)
     float* out; __half* out_h;
-    int parts, row_blocks, row_block0;
+    int parts, chunk, cluster;     // parts a unit's tiles are cut into, of `chunk` tiles each; whether they form a cluster
+    int row_blocks, row_block0;
 };
 struct Q8EvictParams {
     const int* tables; int width;
@@ -99,8 +101,8 @@ struct Q8EvictParams {
 };
 cudaError_t launch_q8_write(const Q8WriteParams& p, int d, int fmt, cudaStream_t stream);
 cudaError_t launch_q8_read(const Q8ReadParams& p, int d, int fmt, cudaStream_t stream);
-cudaError_t launch_q8_attention(const Q8AttnParams& p, int d, int fmt, cudaStream_t stream);
-size_t q8_attention_workspace(const Q8Cache& c, int qpk, int batch, int max_q, int max_seq, int window, int sinks, bool mass);
+cudaError_t launch_q8_attention(const Q8AttnParams& p, int d, int fmt, void* workspace, cudaStream_t stream);
+size_t q8_attention_workspace(int nkv, int qpk, int d, int block, int batch, int max_q, int max_seq, int window, int sinks, bool mass);
 cudaError_t launch_q8_evict(const Q8EvictParams& p, cudaStream_t stream);
 int q8_evict_max_pages();
 

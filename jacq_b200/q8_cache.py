@@ -264,14 +264,16 @@ class Q8Cache:
         else:
             batch, offsets = q_offsets.numel() - 1, _int32(q_offsets, "q_offsets", self.device)
         tables, lens, slots, keep = self._rows(batch, slot_ids, seq_lens)
-        mass, mass_width, workspace, size = 0, 0, None, 0
+        mass, mass_width, workspace = 0, 0, None
+        if page_mass is not None:
+            if q_offsets is not None:
+                raise RuntimeError("page_mass goes with one token per sequence")
+            _check_mass(page_mass, batch, self.layout.num_kv_heads, self.device)
+            mass, mass_width = page_mass.data_ptr(), page_mass.shape[2]
         with _on(self.device):
-            if page_mass is not None:
-                if q_offsets is not None:
-                    raise RuntimeError("page_mass goes with one token per sequence")
-                _check_mass(page_mass, batch, self.layout.num_kv_heads, self.device)
-                mass, mass_width = page_mass.data_ptr(), page_mass.shape[2]
-                size = self._lib.kivi_b200_q8_attention_workspace_bytes(self._refs[0], batch, 1, max_seq_len, window, sinks, 1)
+            size = self._lib.kivi_b200_q8_attention_workspace_bytes(self._refs[0], batch, max_q_per_seq, max_seq_len, window, sinks,
+                                                                    page_mass is not None)
+            if size:   # of this call alone: the allocator hands it on in stream order, or keeps it for a graph under capture
                 workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
             rc = self._lib.kivi_b200_q8_attention(
                 *self._refs, q.data_ptr(), stride, offsets, q.shape[0], tables.data_ptr(), self.max_blocks_per_seq, lens, slots,
