@@ -57,31 +57,57 @@ __global__ void __launch_bounds__(kThreads) q8_evict_kernel(const Q8EvictParams 
     if (!all) {
         for (int i = lo + tid; i < hi; i += kThreads) {
             double sum = 0.0;
-            for (int h = 0; h < p.nkv; ++h) sum += (double)mass[(size_t)h * p.mass_width + i];
+            for (int h0 = 0; h0 < p.nkv; h0 += 8) {   // eight heads' loads in flight, added in order
+                float x[8];
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x[k] = h0 + k < p.nkv ? mass[(size_t)(h0 + k) * p.mass_width + i] : 0.0f;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) sum += (double)x[k];
+            }
             keys[i] = key_of((float)sum);
         }
         // budget < full and first + recent <= budget, so 0 <= need < hi - lo
         if (tid == 0) { s_prefix = 0; s_need = p.budget - lo - (full - hi); }
         __syncthreads();
+        const int need = p.budget - lo - (full - hi);
         // the need-th largest key, byte by byte (need = 0: nothing but the protected pages stays)
-        for (int shift = 24; shift >= 0; shift -= 8) {
+        for (int shift = 24; need > 0 && shift >= 0; shift -= 8) {
             if (tid < 256) hist[tid] = 0;
             __syncthreads();
             const uint32_t prefix = s_prefix, mask = shift == 24 ? 0u : ~0u << (shift + 8);
-            for (int i = lo + tid; i < hi; i += kThreads)
-                if ((keys[i] & mask) == prefix) atomicAdd(&hist[(keys[i] >> shift) & 255], 1);
+            // masses share their leading bits: one atomic per distinct digit of a warp, not per key
+            for (int base = lo; base < hi; base += kThreads) {
+                const int i = base + tid;
+                const bool in = i < hi && (keys[i] & mask) == prefix;
+                const int digit = in ? (int)(keys[i] >> shift) & 255 : 256;
+                const unsigned same = __match_any_sync(0xffffffffu, digit);
+                if (in && (tid & 31) == __ffs(same) - 1) atomicAdd(&hist[digit], __popc(same));
+            }
             __syncthreads();
-            if (tid == 0) {
-                int left = s_need, b = 255;
-                while (b > 0 && hist[b] < left) left -= hist[b--];
-                s_need = left;
-                s_prefix = prefix | ((uint32_t)b << shift);
+            if (tid < 32) {   // from the highest digit down: lane l counts digits 255 - 8 l .. 248 - 8 l
+                int mine = 0;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) mine += hist[255 - 8 * tid - k];
+                int upto = mine;
+#pragma unroll
+                for (int x = 1; x < 32; x *= 2) {
+                    const int y = __shfl_up_sync(0xffffffffu, upto, x);
+                    if (tid >= x) upto += y;
+                }
+                const int want = s_need;
+                __syncwarp();
+                if (want > upto - mine && want <= upto) {   // exactly one lane, as 1 <= want <= all
+                    int left = want - (upto - mine), b = 255 - 8 * tid;
+                    while (hist[b] < left) left -= hist[b--];
+                    s_need = left;
+                    s_prefix = prefix | ((uint32_t)b << shift);
+                }
             }
             __syncthreads();
         }
         threshold = s_prefix;
         ties = s_need;
-        if (p.budget - lo - (full - hi) == 0) { threshold = 0xffffffffu; ties = 0; }
+        if (need == 0) { threshold = 0xffffffffu; ties = 0; }
     }
     // close up, in order
     int kept = 0, gone = 0, tied = 0;

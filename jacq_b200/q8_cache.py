@@ -78,31 +78,28 @@ class Q8Eviction(NamedTuple):
     freed_counts: torch.Tensor   # int32 [batch]
 
 
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+# The calls of a decode step are a few microseconds long on the device, so the host side is kept short: integers instead
+# of device objects, the raw stream handle, no context manager where the device is the current one already.
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
-def _int32(t: torch.Tensor, name: str, device: torch.device) -> int:
-    if t.dtype != torch.int32 or not t.is_contiguous():
+def _int32(t: torch.Tensor, name: str, index: int) -> int:
+    if t.dtype is not torch.int32 or not t.is_contiguous():
         raise TypeError(f"{name} must be a contiguous torch.int32 tensor")
-    if t.device != device:
-        raise RuntimeError(f"{name} is on {t.device}, the cache on {device}")
+    if t.get_device() != index:
+        raise RuntimeError(f"{name} is on {t.device}, expected cuda:{index}")
     return t.data_ptr()
 
 
-class _on:
-    """The device of the tensors as the current one, for a launch; nothing to do where it is already."""
-
-    def __init__(self, device: torch.device):
-        self._guard = None if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-    def __enter__(self):
-        if self._guard is not None:
-            self._guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
+def _call(index: int, where: str, fn, *args) -> None:
+    """One library call on the current stream of device `index`, with that device current."""
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _native.check(rc, where)
 
 
 def _indexed(device: torch.device | str) -> torch.device:
@@ -146,10 +143,10 @@ class Q8Cache:
             if t.dtype != dtype or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
                 raise TypeError(f"{name} must be a contiguous {dtype} tensor {shape} on {device}")
         for name, t, dim in (("block_tables", block_tables, 2), ("seq_lens", seq_lens, 1)):
-            _int32(t, name, device)
+            _int32(t, name, device.index)
             if t.dim() != dim:
                 raise TypeError(f"{name} must have {dim} dimension(s)")
-        self.layout, self.tensors, self.device = layout, tensors, device
+        self.layout, self.tensors, self.device, self._index = layout, tensors, device, device.index
         self.block_tables, self.seq_lens = block_tables, seq_lens
         self.max_blocks_per_seq = block_tables.shape[1]
         self.num_blocks, self.num_slots = blocks, slots
@@ -157,6 +154,7 @@ class Q8Cache:
         self._struct = _native.KiviQ8CacheStruct(*[t.data_ptr() for t in tensors], blocks, slots)
         self._refs = (ctypes.byref(self._geom), ctypes.byref(self._struct))
         self._lib = _native.lib()
+        self._workspace_bytes: dict[tuple, int] = {}   # by the sizes of a call; the plan behind them is host arithmetic
 
     def set_block_tables(self, tables: torch.Tensor) -> None:
         """Install block tables ``[<= num_slots, <= max_blocks_per_seq]`` (int32; host or device)."""
@@ -165,10 +163,12 @@ class Q8Cache:
         self.block_tables[: tables.shape[0], : tables.shape[1]] = tables
 
     def _rows(self, batch: int, slot_ids, lens):
-        """Block-table rows and lengths of the batch: stored per slot, indexed per batch row by the library."""
+        """Pointers of the batch's block-table rows, lengths and slots, and the tensors to keep alive: tables and lengths
+        are stored per slot, the library indexes them per batch row."""
         tables = self.block_tables
+        slots = 0
         if slot_ids is not None:
-            _int32(slot_ids, "slot_ids", self.device)
+            slots = _int32(slot_ids, "slot_ids", self._index)
             if slot_ids.numel() != batch:
                 raise RuntimeError(f"slot_ids holds {slot_ids.numel()} entries for a batch of {batch}")
             tables = tables.index_select(0, slot_ids)
@@ -178,18 +178,22 @@ class Q8Cache:
             lens = self.seq_lens
         if tables.shape[0] < batch or lens.numel() < batch:
             raise RuntimeError(f"a batch of {batch} exceeds the {tables.shape[0]} block-table rows / {lens.numel()} lengths")
-        return tables, _int32(lens, "sequence lengths", self.device), (0 if slot_ids is None else slot_ids.data_ptr()), lens
+        return tables.data_ptr(), _int32(lens, "sequence lengths", self._index), slots, (tables, lens)
 
-    def _token_rows(self, t: torch.Tensor, name: str, heads: int) -> int:
-        """Checks ``[tokens, heads, head_dim]`` fp16 rows that are contiguous within a token; their stride in elements."""
-        if t.dtype != torch.float16:
+    def _token_rows(self, t: torch.Tensor, name: str, heads: int) -> tuple[int, int]:
+        """Checks ``[tokens, heads, head_dim]`` fp16 rows that are contiguous within a token; tokens, stride in elements."""
+        if t.dtype is not torch.float16:
             raise TypeError(f"{name} must be torch.float16")
         d = self.layout.head_dim
-        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != d or t.device != self.device:
+        if t.dim() != 3 or t.get_device() != self._index:
             raise RuntimeError(f"{name} must be [tokens, {heads}, {d}] on {self.device}")
-        if t.stride(2) != 1 or (heads > 1 and t.stride(1) != d):
+        n, h, width = t.shape
+        if h != heads or width != d:
+            raise RuntimeError(f"{name} must be [tokens, {heads}, {d}] on {self.device}")
+        step, head, one = t.stride()
+        if one != 1 or (head != d and heads > 1):
             raise RuntimeError(f"{name} must be contiguous within a token")
-        return t.stride(0) if t.shape[0] > 1 else heads * d
+        return n, step if n > 1 else heads * d
 
     def write(self, new_k: torch.Tensor, new_v: torch.Tensor, new_offsets: torch.Tensor, *, max_new_per_seq: int,
               max_start_seq_len: int, slot_ids: torch.Tensor | None = None, start_seq_lens: torch.Tensor | None = None,
@@ -198,23 +202,22 @@ class Q8Cache:
         strided, as slices of a fused projection are) to sequence i. Lengths are read from, and with ``advance``
         updated in, ``self.seq_lens``; with ``start_seq_lens`` they are the caller's and nothing is updated."""
         nkv = self.layout.num_kv_heads
-        ks, vs = self._token_rows(new_k, "new_k", nkv), self._token_rows(new_v, "new_v", nkv)
-        if new_k.shape[0] != new_v.shape[0]:
+        total, ks = self._token_rows(new_k, "new_k", nkv)
+        other, vs = self._token_rows(new_v, "new_v", nkv)
+        if total != other:
             raise RuntimeError("new_k and new_v must hold the same tokens")
-        offsets = _int32(new_offsets, "new_offsets", self.device)
+        offsets = _int32(new_offsets, "new_offsets", self._index)
         n = new_offsets.numel() - 1
         tables, starts, slots, keep = self._rows(n, slot_ids, start_seq_lens)
-        with _on(self.device):
-            rc = self._lib.kivi_b200_q8_cache_write(
-                *self._refs, new_k.data_ptr(), new_v.data_ptr(), ks, vs, tables.data_ptr(), self.max_blocks_per_seq, starts,
-                offsets, slots, n, new_k.shape[0], max_new_per_seq, max_start_seq_len, _stream(self.device))
-            _native.check(rc, "kivi_b200_q8_cache_write")
-            if advance and start_seq_lens is None:
-                counts = new_offsets[1:] - new_offsets[:-1]
-                if slot_ids is None:
-                    self.seq_lens[:n] += counts
-                else:
-                    self.seq_lens.index_add_(0, slot_ids, counts)
+        _call(self._index, "kivi_b200_q8_cache_write", self._lib.kivi_b200_q8_cache_write, *self._refs, new_k.data_ptr(),
+              new_v.data_ptr(), ks, vs, tables, self.max_blocks_per_seq, starts, offsets, slots, n, total, max_new_per_seq,
+              max_start_seq_len)
+        if advance and start_seq_lens is None:
+            counts = new_offsets[1:] - new_offsets[:-1]
+            if slot_ids is None:
+                self.seq_lens[:n] += counts
+            else:
+                self.seq_lens.index_add_(0, slot_ids, counts)
 
     def read(self, row_offsets: torch.Tensor, first_rows: torch.Tensor, seq_lens: torch.Tensor | None = None, *, total: int,
              max_rows_per_seq: int, slot_ids: torch.Tensor | None = None, k_out: torch.Tensor | None = None,
@@ -222,21 +225,20 @@ class Q8Cache:
         """What the cache holds, as fp16 ``[total, NKV, D]`` tensors: rows ``row_offsets[i]:row_offsets[i+1]`` receive
         tokens ``first_rows[i]`` onwards of sequence i, zeros behind its last token."""
         shape = (total, self.layout.num_kv_heads, self.layout.head_dim)
-        k_out = torch.empty(shape, dtype=torch.float16, device=self.device) if k_out is None else k_out
-        v_out = torch.empty(shape, dtype=torch.float16, device=self.device) if v_out is None else v_out
+        if k_out is None:
+            k_out = torch.empty(shape, dtype=torch.float16, device=self.device)
+        if v_out is None:
+            v_out = torch.empty(shape, dtype=torch.float16, device=self.device)
         for name, t in (("k_out", k_out), ("v_out", v_out)):
-            if t.dtype != torch.float16 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != self.device:
+            if t.dtype is not torch.float16 or t.shape != shape or not t.is_contiguous() or t.get_device() != self._index:
                 raise TypeError(f"{name} must be a contiguous torch.float16 tensor {shape} on {self.device}")
-        offsets, first = _int32(row_offsets, "row_offsets", self.device), _int32(first_rows, "first_rows", self.device)
+        offsets, first = _int32(row_offsets, "row_offsets", self._index), _int32(first_rows, "first_rows", self._index)
         n = row_offsets.numel() - 1
         if first_rows.numel() < n:
             raise RuntimeError(f"first_rows holds {first_rows.numel()} entries for a batch of {n}")
         tables, lens, slots, keep = self._rows(n, slot_ids, seq_lens)
-        with _on(self.device):
-            rc = self._lib.kivi_b200_q8_cache_read(
-                *self._refs, tables.data_ptr(), self.max_blocks_per_seq, lens, slots, offsets, first, n, total, max_rows_per_seq,
-                k_out.data_ptr(), v_out.data_ptr(), _stream(self.device))
-        _native.check(rc, "kivi_b200_q8_cache_read")
+        _call(self._index, "kivi_b200_q8_cache_read", self._lib.kivi_b200_q8_cache_read, *self._refs, tables, self.max_blocks_per_seq,
+              lens, slots, offsets, first, n, total, max_rows_per_seq, k_out.data_ptr(), v_out.data_ptr())
         return k_out, v_out
 
     def attend(self, q: torch.Tensor, out: torch.Tensor | None = None, *, max_seq_len: int, window: int = 0, sinks: int = 0,
@@ -250,37 +252,39 @@ class Q8Cache:
         j <= i if ``j < sinks`` or ``j > i - window``; ``window=0`` is no window. ``out`` is fp32, or fp16 when an fp16
         tensor is passed. ``page_mass`` (fp32 ``[batch, NKV, width]``, single tokens only) grows by the weight every page
         got. ``scale`` defaults to 1 / sqrt(D)."""
-        nh = self.layout.num_q_heads
-        stride = self._token_rows(q, "q", nh)
+        total, stride = self._token_rows(q, "q", self.layout.num_q_heads)
         if out is None:
-            out = torch.empty((q.shape[0], nh, self.layout.head_dim), dtype=torch.float32, device=self.device)
-        half = out.dtype == torch.float16
-        if (not half and out.dtype != torch.float32) or out.shape != q.shape or not out.is_contiguous() or out.device != self.device:
+            out = torch.empty(q.shape, dtype=torch.float32, device=self.device)
+        half = out.dtype is torch.float16
+        if not (half or out.dtype is torch.float32) or out.shape != q.shape or not out.is_contiguous() or out.get_device() != self._index:
             raise TypeError("out must be a contiguous torch.float32 or float16 tensor shaped like q")
-        if scale is not None and not 0.0 < scale < 1e30:
+        if scale is None:
+            scale = 0.0
+        elif not 0.0 < scale < 1e30:
             raise ValueError("scale must be positive and finite")
         if q_offsets is None:
-            batch, offsets = q.shape[0], 0
+            batch, offsets = total, 0
         else:
-            batch, offsets = q_offsets.numel() - 1, _int32(q_offsets, "q_offsets", self.device)
+            batch, offsets = q_offsets.numel() - 1, _int32(q_offsets, "q_offsets", self._index)
         tables, lens, slots, keep = self._rows(batch, slot_ids, seq_lens)
-        mass, mass_width, workspace = 0, 0, None
+        mass = mass_width = 0
         if page_mass is not None:
             if q_offsets is not None:
                 raise RuntimeError("page_mass goes with one token per sequence")
-            _check_mass(page_mass, batch, self.layout.num_kv_heads, self.device)
+            _check_mass(page_mass, batch, self.layout.num_kv_heads, self._index)
             mass, mass_width = page_mass.data_ptr(), page_mass.shape[2]
-        with _on(self.device):
-            size = self._lib.kivi_b200_q8_attention_workspace_bytes(self._refs[0], batch, max_q_per_seq, max_seq_len, window, sinks,
-                                                                    page_mass is not None)
-            if size:   # of this call alone: the allocator hands it on in stream order, or keeps it for a graph under capture
-                workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
-            rc = self._lib.kivi_b200_q8_attention(
-                *self._refs, q.data_ptr(), stride, offsets, q.shape[0], tables.data_ptr(), self.max_blocks_per_seq, lens, slots,
-                batch, max_q_per_seq, max_seq_len, window, sinks, scale or 0.0, mass, mass_width,
-                0 if half else out.data_ptr(), out.data_ptr() if half else 0,
-                0 if workspace is None else workspace.data_ptr(), size, _stream(self.device))
-        _native.check(rc, "kivi_b200_q8_attention")
+        sizes = (batch, max_q_per_seq, max_seq_len, window, sinks, page_mass is not None)
+        size = self._workspace_bytes.get(sizes)
+        if size is None:
+            size = self._workspace_bytes[sizes] = self._lib.kivi_b200_q8_attention_workspace_bytes(self._refs[0], *sizes)
+        workspace, at = None, 0
+        if size:   # of this call alone: the allocator hands it on in stream order, or keeps it for a graph under capture
+            workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
+            at = workspace.data_ptr()
+        target = out.data_ptr()
+        _call(self._index, "kivi_b200_q8_attention", self._lib.kivi_b200_q8_attention, *self._refs, q.data_ptr(), stride, offsets, total,
+              tables, self.max_blocks_per_seq, lens, slots, batch, max_q_per_seq, max_seq_len, window, sinks, scale, mass, mass_width,
+              0 if half else target, target if half else 0, at, size)
         return out
 
     def evict(self, page_mass: torch.Tensor, *, budget: int, first: int = 0, recent: int = 0, max_seq_len: int,
@@ -296,9 +300,9 @@ class Q8Cache:
         return r
 
 
-def _check_mass(mass: torch.Tensor, batch: int, nkv: int | None, device: torch.device) -> None:
-    if mass.dtype != torch.float32 or mass.dim() != 3 or not mass.is_contiguous() or mass.device != device:
-        raise TypeError(f"page_mass must be a contiguous torch.float32 [batch, kv heads, width] tensor on {device}")
+def _check_mass(mass: torch.Tensor, batch: int, nkv: int | None, index: int) -> None:
+    if mass.dtype is not torch.float32 or mass.dim() != 3 or not mass.is_contiguous() or mass.get_device() != index:
+        raise TypeError(f"page_mass must be a contiguous torch.float32 [batch, kv heads, width] tensor on cuda:{index}")
     if mass.shape[0] != batch or (nkv is not None and mass.shape[1] != nkv):
         raise RuntimeError(f"page_mass must be [{batch}, {'kv heads' if nkv is None else nkv}, width], got {tuple(mass.shape)}")
 
@@ -308,27 +312,25 @@ def evict_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, page_mass: t
     """Keep ``budget`` complete pages of every sequence that has more: its first ``first`` and last ``recent`` ones and, of
     the others, those with the largest ``page_mass [batch, NKV, width]`` over all kv heads (ties: the lowest page). The
     inputs stay as they are. Works on the tables of any paged cache whose pages are self-contained."""
-    device = block_tables.device
-    if device.type != "cuda":
+    index = block_tables.get_device()
+    if index < 0:
         raise RuntimeError("evict_pages needs CUDA tensors; its kernel has no CPU path")
-    tables, lens = _int32(block_tables, "block_tables", device), _int32(seq_lens, "seq_lens", device)
+    tables, lens = _int32(block_tables, "block_tables", index), _int32(seq_lens, "seq_lens", index)
     if block_tables.dim() != 2 or seq_lens.numel() != block_tables.shape[0]:
         raise TypeError("block_tables must be [batch, width] and seq_lens [batch]")
     batch, width = block_tables.shape
-    _check_mass(page_mass, batch, None, device)
-    nkv, mass_width = page_mass.shape[1], page_mass.shape[2]
-    # the five outputs are slices of one allocation, the float one first
-    n_mass, n_table = batch * nkv * mass_width, batch * width
-    flat = torch.empty(n_mass + 2 * n_table + 2 * batch, dtype=torch.int32, device=device)
-    mass = flat[:n_mass].view(torch.float32).view(batch, nkv, mass_width)
-    new_tables, freed = flat[n_mass:n_mass + n_table].view(batch, width), flat[n_mass + n_table:n_mass + 2 * n_table].view(batch, width)
-    new_lens, counts = flat[n_mass + 2 * n_table:n_mass + 2 * n_table + batch], flat[n_mass + 2 * n_table + batch:]
-    with _on(device):
-        rc = _native.lib().kivi_b200_q8_evict(
-            nkv, block_size, tables, width, lens, page_mass.data_ptr(), mass_width, batch, max_seq_len, budget, first, recent,
-            new_tables.data_ptr(), new_lens.data_ptr(), mass.data_ptr(), freed.data_ptr(), counts.data_ptr(), _stream(device))
-    _native.check(rc, "kivi_b200_q8_evict")
-    return Q8Eviction(new_tables, new_lens, mass, freed, counts)
+    _check_mass(page_mass, batch, None, index)
+    _, nkv, mass_width = page_mass.shape
+    mass = torch.empty_like(page_mass)
+    ints = torch.empty((2 * width + 2, batch), dtype=torch.int32, device=block_tables.device)   # both tables and both counts
+    both = ints[:2 * width].view(2, batch, width)
+    out = Q8Eviction(both[0], ints[2 * width], mass, both[1], ints[2 * width + 1])
+    at = ints.data_ptr()
+    table_bytes, row_bytes = 4 * batch * width, 4 * batch
+    _call(index, "kivi_b200_q8_evict", _native.lib().kivi_b200_q8_evict, nkv, block_size, tables, width, lens, page_mass.data_ptr(),
+          mass_width, batch, max_seq_len, budget, first, recent, at, at + 2 * table_bytes, mass.data_ptr(), at + table_bytes,
+          at + 2 * table_bytes + row_bytes)
+    return out
 
 
 def rejected_indices() -> int:
