@@ -17,7 +17,7 @@
 // A sequence's context is cut into `parts`, one CTA each, that form a thread-block cluster: they merge through
 // distributed shared memory, so a call needs no second launch and no workspace.
 #include <cooperative_groups.h>
-#include <cfloat>
+#include <type_traits>
 
 #include "q8_common.cuh"
 
@@ -163,15 +163,20 @@ __device__ __forceinline__ void add_masses(const Q8AttnParams& p, const Unit& u,
 // Two shapes of the kernel. Four warps and a shallow ring, several CTAs per multiprocessor, where there are units enough
 // to fill it; eight warps and a deep ring, one CTA per multiprocessor, where there are few and each warp's own copies
 // have to cover the latency.
+#ifndef Q8S4
+#define Q8S4 2
+#define Q8C4 3
+#endif
+constexpr int tiles_at_once(int d) { return d == 256 ? 1 : 2; }
 template <int D, int kWarps>
-constexpr int stages_of() { return kWarps == 4 ? (D == 64 ? 4 : 3) : D == 64 ? 10 : D == 128 ? 6 : 3; }
+constexpr int stages_of() { return kWarps == 4 ? (D == 64 ? 3 : D == 128 ? Q8S4 : 3) : D == 64 ? 5 : 3; }
 template <int D, int kWarps>
-constexpr int ctas_of(int nt) { return kWarps == 8 ? 1 : D == 64 ? (nt == 1 ? 5 : 4) : D == 128 ? (nt == 1 ? 4 : 3) : 2; }
+constexpr int ctas_of(int nt) { return kWarps == 8 ? 1 : D == 64 ? 4 : D == 128 ? Q8C4 : 2; }
 
 template <int D, int FMT, int NT, bool MASS, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attention_kernel(const Q8AttnParams p) {
     using T = Tile<D>;
-    constexpr int R = 8 * NT, S = stages_of<D, kWarps>();
+    constexpr int R = 8 * NT, S = stages_of<D, kWarps>(), TPI = tiles_at_once(D);
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ float s_m[kWarps][R], s_l[kWarps][R];
     __shared__ float c_m[R], c_l[R];             // this CTA's merged state, read by its cluster
@@ -225,27 +230,48 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
     // V's scales enter the fp16 probabilities relative to vref, a power of two not below any met so far (0: none yet)
     float vref = 0.0f, vmul = 0.0f;
 
-    // Scores of a tile -> probabilities as B fragments pb; also the running state.
-    auto softmax = [&](float (&s)[NT][4], float f, float vs, int key0, int item, uint32_t (&pb)[NT][2]) {
-        const bool whole = key0 + 15 <= v.pos0 && (key0 >= v.low1 || key0 + 16 <= p.sinks);
-        bool raise = false;
+    // Scores of TP tiles -> probabilities as B fragments pb; also the running state. Whether all rows see all of them.
+    auto softmax = [&](auto tp, float (*s)[NT][4], const float* f, const float* vs, const int* key0, int item, int live,
+                       uint32_t (*pb)[NT][2]) {
+        constexpr int TP = decltype(tp)::value;
+        bool whole = true, raise = false;
+        float vtop = vs[0];
+#pragma unroll
+        for (int i = 0; i < TP; ++i) whole = whole && key0[i] + 15 <= v.pos0 && (key0[i] >= v.low1 || key0[i] + 16 <= p.sinks);
+#pragma unroll
+        for (int i = 0; i < TP; ++i)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[i][nt][e] *= f[i];
+        if (!whole) {
+#pragma unroll
+            for (int i = 0; i < TP; ++i)
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int key = key0[i] + g + (e >> 1) * 8, c = e & 1;
+                        if (key > hi[nt][c] || (key < lo[nt][c] && key >= p.sinks)) s[i][nt][e] = -INFINITY;
+                    }
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                s[nt][e] *= f;
-                if (!whole) {
-                    const int key = key0 + g + (e >> 1) * 8, c = e & 1;
-                    if (key > hi[nt][c] || (key < lo[nt][c] && key >= p.sinks)) s[nt][e] = -INFINITY;
-                }
-                raise |= s[nt][e] > m[nt][e & 1] + kLazy;
+            for (int c = 0; c < 2; ++c) {
+                float top = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
+#pragma unroll
+                for (int i = 1; i < TP; ++i) top = fmaxf(top, fmaxf(s[i][nt][c], s[i][nt][c + 2]));
+                raise |= top > m[nt][c] + kLazy;
             }
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    float top = fmaxf(s[nt][c], s[nt][c + 2]);
+                    float top = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
+#pragma unroll
+                    for (int i = 1; i < TP; ++i) top = fmaxf(top, fmaxf(s[i][nt][c], s[i][nt][c + 2]));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
                     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
@@ -256,8 +282,10 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
                     for (int mt = 0; mt < T::MT; ++mt) { o[nt][mt][c] *= a; o[nt][mt][c + 2] *= a; }
                 }
         }
-        if (vs > vref) {   // uniform over the warp; false for a NaN scale, which goes through as it is
-            const float next = __uint_as_float((__float_as_uint(vs) & 0x7f800000u) + 0x00800000u), a = vref / next;
+#pragma unroll
+        for (int i = 1; i < TP; ++i) vtop = fmaxf(vtop, vs[i]);
+        if (vtop > vref) {   // uniform over the warp; NaN scales do not count and go through as they are
+            const float next = __uint_as_float((__float_as_uint(vtop) & 0x7f800000u) + 0x00800000u), a = vref / next;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -267,34 +295,36 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
             vref = next;
             vmul = kHeadroom / next;
         }
-        const float w = vs * vmul;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            float e[4];
+        for (int i = 0; i < TP; ++i) {
+            const float w = vs[i] * vmul;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) e[k] = fast_exp2(s[nt][k] - m[nt][k & 1]);
-            l[nt][0] += e[0] + e[2];
-            l[nt][1] += e[1] + e[3];
-            if constexpr (MASS) {
-                // sums over the 16 tokens: lanes of even g end up with column 2t's, those of odd g with column 2t + 1's
-                const bool odd = g & 1;
-                const float a = e[0] + e[2], b = e[1] + e[3];
-                float x = (odd ? b : a) + __shfl_xor_sync(0xffffffffu, odd ? a : b, 4);
-                x += __shfl_xor_sync(0xffffffffu, x, 8);
-                x += __shfl_xor_sync(0xffffffffu, x, 16);
-                if (g < 2)
-                    p.page_ws[((size_t)(seq * nkv + h) * p.ws_tiles + item) * R + 8 * nt + 2 * t + g] = make_float2(x, g ? m[nt][1] : m[nt][0]);
+            for (int nt = 0; nt < NT; ++nt) {
+                float e[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) e[k] = fast_exp2(s[i][nt][k] - m[nt][k & 1]);
+                l[nt][0] += e[0] + e[2];
+                l[nt][1] += e[1] + e[3];
+                if constexpr (MASS) {
+                    // sums over the 16 tokens: lanes of even g end up with column 2t's, those of odd g with column 2t + 1's
+                    const bool odd = g & 1;
+                    const float a = e[0] + e[2], b = e[1] + e[3];
+                    float x = (odd ? b : a) + __shfl_xor_sync(0xffffffffu, odd ? a : b, 4);
+                    x += __shfl_xor_sync(0xffffffffu, x, 8);
+                    x += __shfl_xor_sync(0xffffffffu, x, 16);
+                    if (g < 2 && i < live)
+                        p.page_ws[((size_t)(seq * nkv + h) * p.ws_tiles + item + i) * R + 8 * nt + 2 * t + g] =
+                            make_float2(x, g ? m[nt][1] : m[nt][0]);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    // a probability of a masked key is 0 whatever the page's scale is
+                    if (!whole && s[i][nt][k] == -INFINITY) e[k] = 0.0f;
+                    else e[k] *= w;
+                }
+                pb[i][nt][0] = movmatrix_trans(pack_half2(e[0], e[1]));
+                pb[i][nt][1] = movmatrix_trans(pack_half2(e[2], e[3]));
             }
-            // a probability of a masked key is 0 whatever the page's scale is
-            if (!whole) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) e[k] = s[nt][k] == -INFINITY ? 0.0f : e[k] * w;
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) e[k] *= w;
-            }
-            pb[nt][0] = movmatrix_trans(pack_half2(e[0], e[1]));
-            pb[nt][1] = movmatrix_trans(pack_half2(e[2], e[3]));
         }
         return whole;
     };
@@ -302,15 +332,21 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
     auto unseen = [&](int key) { return key >= v.end || (key < v.low0 && key >= p.sinks); };
 
     // ---- page tiles: a ring of S stages per warp, filled by the lanes for themselves
-    const uint32_t ring = smem_u32(smem) + (uint32_t)warp * S * T::STAGE;
+    const uint32_t ring = smem_u32(smem) + (uint32_t)(warp * S * TPI) * T::STAGE;
     const int q1 = min(i1, v.tiles);
     const int* table = p.seq.tables + (size_t)seq * p.seq.width;
     const int sub_mask = (block >> 4) - 1, sub_log = p.cache.log2b - 4;
     auto tile_of = [&](int item) { return item < v.ns ? item : item - v.ns + v.w0; };
+    // A warp takes TPI neighbouring tiles at a time. Tile `a` of a warp, and the item a copy that is due reads: the last of
+    // an odd number is copied twice and masked, so that no stage ever holds anything but codes.
+    auto item_of = [&](int a) {
+        const int item = i0 + TPI * (warp + a / TPI * kWarps) + a % TPI;
+        return TPI > 1 && a % TPI && item == q1 ? item - 1 : item;
+    };
     // Page ids of the warp's tiles, 32 at a time, one per lane, a block of 32 ahead of their use: the load's latency and
     // the check against the pool are paid once per 32 tiles.
-    auto load_ids = [&](int k0) {
-        const int item = i0 + warp + (k0 + lane) * kWarps;
+    auto load_ids = [&](int a0) {
+        const int item = item_of(a0 + lane);
         const int page = item < q1 ? tile_of(item) >> sub_log : 0;
         return item < q1 && page < p.seq.width ? table[page] : item < q1 ? -1 : 0;
     };
@@ -327,18 +363,16 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
         const int row = (32 * i + lane) / T::CPR, chunk = lane % T::CPR;
         return (uint32_t)(row * D + ((chunk ^ (is_v ? T::v_swizzle(row) : T::k_swizzle(row))) << 4));
     };
-    auto issue = [&](int item, int id, int stage) {
+    auto issue = [&](int item, int id, uint32_t dst) {
         if (item < q1) {
             const size_t at = (size_t)id * page_bytes + (size_t)(tile_of(item) & sub_mask) * T::BYTES;
             const uint8_t *k = kbase + at, *vv = vbase + at;
-            const uint32_t dst = ring + (uint32_t)stage * T::STAGE;
 #pragma unroll
             for (int i = 0; i < T::BYTES / 512; ++i) cp_async16_32(dst + swizzled(i, false), k + 512 * i);
 #pragma unroll
             for (int i = 0; i < T::BYTES / 512; ++i) cp_async16_32(dst + T::BYTES + swizzled(i, true), vv + 512 * i);
             if (lane == 0) cp_async8(dst + 2 * T::BYTES, p.cache.scales + (size_t)id * nkv + h);
         }
-        cp_async_commit();
     };
     // where this lane's pieces lie in a stage
     const uint32_t k_at = g * D + ((t ^ T::k_swizzle(g)) << 4);
@@ -346,77 +380,94 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
     {
         int ids = checked(load_ids(0)), ids_next = load_ids(32), asked = 0;
         auto issue_next = [&](int stage) {
-            const int id = __shfl_sync(0xffffffffu, ids, asked & 31);
-            issue(i0 + warp + asked * kWarps, id, stage);
-            if ((++asked & 31) == 0) { ids = checked(ids_next); ids_next = load_ids(asked + 32); }
+#pragma unroll
+            for (int i = 0; i < TPI; ++i) {
+                const int id = __shfl_sync(0xffffffffu, ids, (asked + i) & 31);
+                issue(item_of(asked + i), id, ring + (uint32_t)(stage * TPI + i) * T::STAGE);
+            }
+            cp_async_commit();
+            asked += TPI;
+            if ((asked & 31) == 0) { ids = checked(ids_next); ids_next = load_ids(asked + 32); }
         };
 #pragma unroll
         for (int s = 0; s < S - 1; ++s) issue_next(s);
         int stage = 0;
-        for (int item = i0 + warp; item < q1; item += kWarps) {
+        for (int item = i0 + TPI * warp; item < q1; item += TPI * kWarps) {
             issue_next(stage == 0 ? S - 1 : stage - 1);
             cp_async_wait<S - 1>();
             __syncwarp();                          // the other lanes' copies have landed too
-            const uint32_t src = ring + (uint32_t)stage * T::STAGE;
-            const uint2 sc = lds64(src + 2 * T::BYTES);
-            float s[NT][4], s2[NT][4];   // two sums, so that half as many products wait on one another
+            const uint32_t src = ring + (uint32_t)(stage * TPI) * T::STAGE;
+            const int live = TPI > 1 && item + 1 == q1 ? 1 : TPI;
+            float s[TPI][NT][4], f[TPI], vs[TPI];
+            int key0[TPI];
+            uint32_t pb[TPI][NT][2];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int tt = 0; tt < TPI; ++tt) {
+                const uint2 sc = lds64(src + tt * T::STAGE + 2 * T::BYTES);
+                f[tt] = __uint_as_float(sc.x) * p.scale_log2;
+                vs[tt] = __uint_as_float(sc.y);
+                key0[tt] = tt < live ? tile_of(item + tt) * 16 : 0x3fffffff;   // no row sees that far
+                float s2[NT][4];   // two sums, so that half as many products wait on one another
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.0f;
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int j = 0; j < T::KC; ++j) {
-                // piece t + 4 j: the swizzle flips bit 2 of the chunk, that is j's low bit
-                const uint32_t at = src + (k_at ^ (uint32_t)((j & 1) << 6)) + (j >> 1) * 128;
-                const uint4 a = lds128(at), b = lds128(at + 8 * D);
-                const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
+                    for (int e = 0; e < 4; ++e) s[tt][nt][e] = s2[nt][e] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t a0, a1, a2, a3;
-                    q8_unpack<FMT>(aw[i], a0, a2);
-                    q8_unpack<FMT>(bw[i], a1, a3);
+                for (int j = 0; j < T::KC; ++j) {
+                    // piece t + 4 j: the swizzle flips bit 2 of the chunk, that is j's low bit
+                    const uint32_t at = src + tt * T::STAGE + (k_at ^ (uint32_t)((j & 1) << 6)) + (j >> 1) * 128;
+                    const uint4 a = lds128(at), b = lds128(at + 8 * D);
+                    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        mma16816(i & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, qf[nt][4 * j + i][0], qf[nt][4 * j + i][1]);
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t a0, a1, a2, a3;
+                        q8_unpack<FMT>(aw[i], a0, a2);
+                        q8_unpack<FMT>(bw[i], a1, a3);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+                            mma16816(i & 1 ? s2[nt] : s[tt][nt], a0, a1, a2, a3, qf[nt][4 * j + i][0], qf[nt][4 * j + i][1]);
+                    }
                 }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[tt][nt][e] += s2[nt][e];
             }
+            const bool whole = softmax(std::integral_constant<int, TPI>(), s, f, vs, key0, item, live, pb);
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
+            for (int tt = 0; tt < TPI; ++tt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[nt][e] += s2[nt][e];
-            uint32_t pb[NT][2];
-            const int key0 = tile_of(item) * 16;
-            const bool whole = softmax(s, __uint_as_float(sc.x) * p.scale_log2, __uint_as_float(sc.y), key0, item, pb);
+                for (int j = 0; j < T::VP; ++j) {
+                    uint32_t w[4][T::VW];
+                    const uint32_t at = src + tt * T::STAGE + v_at + j * 128;
 #pragma unroll
-            for (int j = 0; j < T::VP; ++j) {
-                uint32_t w[4][T::VW];
+                    for (int k4 = 0; k4 < 4; ++k4) {
+                        const int row = (k4 & 1) + (k4 >> 1) * 8;
+                        if constexpr (T::VB == 8) {
+                            const uint2 x = lds64(at + row * D);
+                            w[k4][0] = x.x; w[k4][1] = x.y;
+                        } else {
+                            const uint4 x = lds128(at + row * D);
+                            w[k4][0] = x.x; w[k4][1] = x.y; w[k4][2] = x.z; w[k4][3] = x.w;
+                        }
+                        if (!whole && unseen(key0[tt] + 2 * t + row)) {
 #pragma unroll
-                for (int k4 = 0; k4 < 4; ++k4) {
-                    if constexpr (T::VB == 8) {
-                        const uint2 x = lds64(src + v_at + ((k4 & 1) + (k4 >> 1) * 8) * D);
-                        w[k4][0] = x.x; w[k4][1] = x.y;
-                    } else {
-                        const uint4 x = lds128(src + v_at + ((k4 & 1) + (k4 >> 1) * 8) * D + j * 128);
-                        w[k4][0] = x.x; w[k4][1] = x.y; w[k4][2] = x.z; w[k4][3] = x.w;
+                            for (int i = 0; i < T::VW; ++i) w[k4][i] = 0u;
+                        }
                     }
-                    if (!whole && unseen(key0 + 2 * t + (k4 & 1) + (k4 >> 1) * 8)) {
 #pragma unroll
-                        for (int i = 0; i < T::VW; ++i) w[k4][i] = 0u;
+                    for (int i = 0; i < T::VW; ++i) {
+                        uint32_t ab[4], cd[4];
+                        q8_unpack_pairs<FMT>(w[0][i], w[1][i], ab);
+                        q8_unpack_pairs<FMT>(w[2][i], w[3][i], cd);
+                        const int mt = 8 * j + 2 * i;
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            mma16816(o[nt][mt], ab[0], ab[1], cd[0], cd[1], pb[tt][nt][0], pb[tt][nt][1]);
+                            mma16816(o[nt][mt + 1], ab[2], ab[3], cd[2], cd[3], pb[tt][nt][0], pb[tt][nt][1]);
+                        }
                     }
                 }
-#pragma unroll
-                for (int i = 0; i < T::VW; ++i) {
-                    uint32_t ab[4], cd[4];
-                    q8_unpack_pairs<FMT>(w[0][i], w[1][i], ab);
-                    q8_unpack_pairs<FMT>(w[2][i], w[3][i], cd);
-                    const int mt = 8 * j + 2 * i;
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) {
-                        mma16816(o[nt][mt], ab[0], ab[1], cd[0], cd[1], pb[nt][0], pb[nt][1]);
-                        mma16816(o[nt][mt + 1], ab[2], ab[3], cd[2], cd[3], pb[nt][0], pb[nt][1]);
-                    }
-                }
-            }
             stage = stage == S - 1 ? 0 : stage + 1;
             __syncwarp();                          // every lane has read the stage that the next copies go to
         }
@@ -431,17 +482,15 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
         }
         const __half* kt = p.cache.k_tail + ((size_t)slot * nkv + h) * block * D;
         const __half* vt = p.cache.v_tail + ((size_t)slot * nkv + h) * block * D;
-        int first = i0 + warp;                    // this warp's items, as in the ring
-        if (first < v.tiles) first += (v.tiles - first + kWarps - 1) / kWarps * kWarps;
-        for (int item = first; item < i1; item += kWarps) {
+        for (int item = max(i0, v.tiles) + warp; item < i1; item += kWarps) {
             const int r0 = (item - v.tiles) * 16, key0 = v.paged + r0;
             auto word4 = [&](const __half* base, int row, int chan) {   // 8 channels of a token, zero unless it is seen
                 if (unseen(v.paged + row)) return make_uint4(0u, 0u, 0u, 0u);
                 return *reinterpret_cast<const uint4*>(base + (size_t)row * D + chan);
             };
-            float s[NT][4];
+            float s[1][NT][4];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) s[nt][0] = s[nt][1] = s[nt][2] = s[nt][3] = 0.0f;
+            for (int nt = 0; nt < NT; ++nt) s[0][nt][0] = s[0][nt][1] = s[0][nt][2] = s[0][nt][3] = 0.0f;
 #pragma unroll
             for (int j = 0; j < T::KC; ++j)
 #pragma unroll
@@ -449,12 +498,13 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
                     const uint4 a = word4(kt, r0 + g, 16 * t + 64 * j + 8 * half), b = word4(kt, r0 + g + 8, 16 * t + 64 * j + 8 * half);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma16816(s[nt], a.x, b.x, a.y, b.y, qf[nt][4 * j + 2 * half][0], qf[nt][4 * j + 2 * half][1]);
-                        mma16816(s[nt], a.z, b.z, a.w, b.w, qf[nt][4 * j + 2 * half + 1][0], qf[nt][4 * j + 2 * half + 1][1]);
+                        mma16816(s[0][nt], a.x, b.x, a.y, b.y, qf[nt][4 * j + 2 * half][0], qf[nt][4 * j + 2 * half][1]);
+                        mma16816(s[0][nt], a.z, b.z, a.w, b.w, qf[nt][4 * j + 2 * half + 1][0], qf[nt][4 * j + 2 * half + 1][1]);
                     }
                 }
-            uint32_t pb[NT][2];
-            softmax(s, p.scale_log2, 1.0f, key0, item, pb);
+            uint32_t pb[1][NT][2];
+            const float one = 1.0f;
+            softmax(std::integral_constant<int, 1>(), s, &p.scale_log2, &one, &key0, item, 1, pb);
 #pragma unroll
             for (int e = 0; e < T::MT / 4; ++e) {   // 8 channels of a token per 16-byte word: output tiles 4 e .. 4 e + 3
                 const int chan = D == 64 ? 8 * g : 16 * g + 8 * (e & 1) + 128 * (e >> 1);
@@ -493,10 +543,10 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma16816(o[nt][4 * e + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[nt][0], pb[nt][1]);
+                        mma16816(o[nt][4 * e + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[0][nt][0], pb[0][nt][1]);
                         if (any_odd) {
                             float hit[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma16816(hit, bad[0], bad[1], bad[2], bad[3], pb[nt][0], pb[nt][1]);
+                            mma16816(hit, bad[0], bad[1], bad[2], bad[3], pb[0][nt][0], pb[0][nt][1]);
 #pragma unroll
                             for (int k = 0; k < 4; ++k) if (hit[k] != 0.0f) o[nt][4 * e + i][k] = __int_as_float(0x7fc00000);
                         }
@@ -662,7 +712,7 @@ __global__ void __launch_bounds__(256) q8_merge_kernel(const Q8AttnParams p) {
 
 template <int D, int FMT, int NT, bool MASS, int kWarps>
 cudaError_t launch(const Q8AttnParams& p, cudaStream_t stream) {
-    constexpr size_t ring = (size_t)kWarps * stages_of<D, kWarps>() * Tile<D>::STAGE, merge = (size_t)kWarps * 8 * NT * D * 4;
+    constexpr size_t ring = (size_t)kWarps * stages_of<D, kWarps>() * tiles_at_once(D) * Tile<D>::STAGE, merge = (size_t)kWarps * 8 * NT * D * 4;
     constexpr size_t smem = ring > merge ? ring : merge;
     auto kernel = q8_attention_kernel<D, FMT, NT, MASS, kWarps>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
@@ -738,7 +788,7 @@ Plan make_plan(int nkv, int qpk, int d, int block, int batch, int max_q, int max
     q.cluster = parts > 1 && parts <= 8;
     if (const char* e = getenv("KIVI_Q8_CLUSTER")) q.cluster = parts > 1 && atoi(e);
     q.parts = parts; q.warps = warps;
-    q.chunk = (q.tiles + parts - 1) / parts;
+    q.chunk = ((q.tiles + parts - 1) / parts + 1) / 2 * 2;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     size_t at = 0;
     q.page_ws = at;
