@@ -26,6 +26,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
+constexpr int kMaxParts = 32;
 constexpr float kUnset = -3.0e38f;     // running maximum before any visible token
 constexpr float kLazy = 8.0f;          // the maximum is raised when a score tops it by 2^8
 constexpr float kHeadroom = 64.0f;     // probabilities in fp16 carry 2^6: p vs <= 2^8 2^6 < 65504, 2^20 below 1 stay normal
@@ -60,6 +61,14 @@ template <int D>
 __device__ __forceinline__ int channel_of(int g, int mt, int hf) {
     if constexpr (D == 256) return (mt < 8 ? 0 : 128) + 16 * g + 2 * (mt & 7) + hf;
     else return (D / 8) * g + 2 * mt + hf;
+}
+
+// Where row r, channel ch (even) lies among the accumulators, [accumulator][lane].
+template <int D>
+__device__ __forceinline__ int accumulator_of(int r, int ch) {
+    const int g = D == 256 ? (ch & 127) >> 4 : ch / (D / 8), in = D == 256 ? ch & 15 : ch % (D / 8);
+    const int mt = (D == 256 ? (ch >> 7) * 8 : 0) + (in >> 1);
+    return (((r >> 3) * (D / 16) + mt) * 4 + 2 * (in & 1) + (r & 1)) * 32 + g * 4 + ((r >> 1) & 3);
 }
 
 // The keys a block of query rows sees: [0, sinks) and [low, end), as 16-token tiles.
@@ -599,13 +608,17 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
     }
     __syncthreads();
     constexpr int QUADS = T::MT / 4, ITEMS = NT * 2 * QUADS * 32;
-    if (p.parts > 1 && p.cluster == 0) {         // partials for the merge kernel, in the same order
+    if (p.parts > 1 && p.cluster == 0) {         // partials for the merge kernel, row by row
+        pdl_trigger();
         const size_t slot = (size_t)unit * p.parts + part;
-        for (int e = threadIdx.x; e < VEC; e += kWarps * 32) {
-            float x = so[e];
+        for (int e = threadIdx.x; e < R * D / 4; e += kWarps * 32) {
+            const int r = e / (D / 4), at = accumulator_of<D>(r, e % (D / 4) * 4);
+            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int w = 1; w < kWarps; ++w) x += so[w * VEC + e];
-            p.part_o[slot * VEC + e] = x;
+            for (int w = 0; w < kWarps; ++w)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] += so[w * VEC + at + k * 64];   // channel + 1: two accumulators further
+            reinterpret_cast<float4*>(p.part_o)[slot * (R * D / 4) + e] = make_float4(x[0], x[1], x[2], x[3]);
         }
         if (threadIdx.x < R) p.part_ml[slot * R + threadIdx.x] = make_float2(c_m[threadIdx.x], c_l[threadIdx.x]);
         return;
@@ -668,43 +681,47 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
 }
 
 // Joins the parts of a unit that was cut without a cluster. grid (units, slices): slice 0 writes the output, all share
-// the pages' masses out.
+// the pages' masses out. Launched early (programmatic dependent launch): what it reads of the caller's is not written by
+// the kernel before it, and of that kernel's results it reads nothing before the wait.
 template <int D, int NT, bool MASS>
 __global__ void __launch_bounds__(256) q8_merge_kernel(const Q8AttnParams p) {
-    constexpr int R = 8 * NT, MT = D / 16, VEC = NT * MT * 128, QUADS = MT / 4, ITEMS = NT * 2 * QUADS * 32;
-    __shared__ float f_m[R], f_il[R];
+    constexpr int R = 8 * NT;
+    __shared__ float f_m[R], f_il[R], weight[kMaxParts][R];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const Unit u = make_unit(p, blockIdx.x, R);
-    if (u.rb * R >= u.rows) return;
     const int live = max(1, (u.items + p.chunk - 1) / p.chunk);
+    pdl_wait();
+    if (u.rb * R >= u.rows) return;
     const float2* ml = p.part_ml + (size_t)blockIdx.x * p.parts * R;
-    if (threadIdx.x < R) {
-        const int r = threadIdx.x;
-        float top = kUnset, sum = 0.0f;
-        for (int k = 0; k < live; ++k) top = fmaxf(top, ml[k * R + r].x);
-        for (int k = 0; k < live; ++k) sum += ml[k * R + r].y * fast_exp2(ml[k * R + r].x - top);
-        f_m[r] = top;
-        f_il[r] = sum != 0.0f && u.rb * R + r < u.rows ? 1.0f / sum : 0.0f;
+    for (int r = warp; r < R; r += 8) {          // a lane per part
+        const float2 x = lane < live ? ml[lane * R + r] : make_float2(kUnset, 0.0f);
+        float top = x.x;
+#pragma unroll
+        for (int k = 16; k > 0; k /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+        const float a = fast_exp2(x.x - top);
+        float sum = x.y * a;
+#pragma unroll
+        for (int k = 16; k > 0; k /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+        const float il = sum != 0.0f && u.rb * R + r < u.rows ? 1.0f / sum : 0.0f;
+        weight[lane][r] = a * il;
+        if (lane == 0) { f_m[r] = top; f_il[r] = il; }
     }
     __syncthreads();
     if (blockIdx.y == 0) {
-        for (int e = threadIdx.x; e < ITEMS; e += 256) {
-            const int el = e & 31, q4 = (e >> 5) % QUADS, c = (e >> 5) / QUADS & 1, nt = (e >> 5) / QUADS >> 1;
-            const int r = 8 * nt + 2 * (el & 3) + c, row = u.rb * R + r;
+        for (int e = threadIdx.x; e < R * D / 4; e += 256) {
+            const int r = e / (D / 4), row = u.rb * R + r;
             if (row >= u.rows) continue;
-            const float* src = p.part_o + (size_t)blockIdx.x * p.parts * VEC + ((nt * MT + 4 * q4) * 4 + c) * 32 + el;
-            float x[8];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] = 0.0f;
-#pragma unroll 4
+            const float4* src = reinterpret_cast<const float4*>(p.part_o) + (size_t)blockIdx.x * p.parts * (R * D / 4) + e;
+            float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
             for (int part = 0; part < live; ++part) {
-                const float a = fast_exp2(ml[part * R + r].x - f_m[r]);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] += a * src[(size_t)part * VEC + k * 64];
+                const float4 y = __ldcg(src + (size_t)part * (R * D / 4));
+                const float a = weight[part][r];
+                x.x += a * y.x; x.y += a * y.y; x.z += a * y.z; x.w += a * y.w;
             }
-            const float il = f_il[r];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) x[k] *= il;
-            store8(p, out_at(p, u, row, D) + channel_of<D>(el >> 2, 4 * q4, 0), x);
+            const size_t at = out_at(p, u, row, D) + e % (D / 4) * 4;
+            if (p.out_h) *reinterpret_cast<uint2*>(p.out_h + at) = make_uint2(pack_half2(x.x, x.y), pack_half2(x.z, x.w));
+            else *reinterpret_cast<float4*>(p.out + at) = x;
         }
     }
     if constexpr (MASS) add_masses<R>(p, u, f_m, f_il, blockIdx.y * 256 + threadIdx.x, gridDim.y * 256);
@@ -732,8 +749,15 @@ cudaError_t launch(const Q8AttnParams& p, cudaStream_t stream) {
     e = cudaLaunchKernelEx(&cfg, kernel, p);
     if (e != cudaSuccess || p.parts == 1 || p.cluster) return e;
     const unsigned slices = MASS ? (unsigned)((((p.max_seq >> p.cache.log2b) + 1) + 511) / 512) : 1u;
-    q8_merge_kernel<D, NT, MASS><<<dim3(units, slices < 64 ? slices : 64), 256, 0, stream>>>(p);
-    return cudaGetLastError();
+    cudaLaunchConfig_t merge_cfg = {};
+    merge_cfg.gridDim = dim3(units, slices < 64 ? slices : 64);
+    merge_cfg.blockDim = dim3(256);
+    merge_cfg.stream = stream;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    merge_cfg.attrs = attr;
+    merge_cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&merge_cfg, q8_merge_kernel<D, NT, MASS>, p);
 }
 
 template <int D, int FMT, bool MASS>
