@@ -27,9 +27,6 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kMaxParts = 32;
-constexpr float kUnset = -3.0e38f;     // running maximum before any visible token
-constexpr float kLazy = 8.0f;          // the maximum is raised when a score tops it by 2^8
-constexpr float kHeadroom = 64.0f;     // probabilities in fp16 carry 2^6: p vs <= 2^8 2^6 < 65504, 2^20 below 1 stay normal
 
 __device__ unsigned int g_q8_attn_rejected;
 
@@ -71,62 +68,6 @@ __device__ __forceinline__ int accumulator_of(int r, int ch) {
     return (((r >> 3) * (D / 16) + mt) * 4 + 2 * (in & 1) + (r & 1)) * 32 + g * 4 + ((r >> 1) & 3);
 }
 
-// The keys a block of query rows sees: [0, sinks) and [low, end), as 16-token tiles.
-struct View {
-    int len, n;          // tokens, query rows' tokens
-    int pos0, pos1;      // positions of the block's first and last query token
-    int low0, low1;      // first windowed key of those two
-    int end;             // keys [0, end) are at most seen
-    int paged;           // tokens held in pages
-    int ns, w0, tiles;   // page tiles: 0 .. ns - 1, then w0 ..; `tiles` in all
-    int tail_tiles;
-};
-__device__ __forceinline__ View make_view(const Q8AttnParams& p, int len, int n, int tok0, int tok1) {
-    View v;
-    v.len = len; v.n = n;
-    v.pos0 = len - n + tok0; v.pos1 = len - n + tok1;
-    v.low0 = max(0, p.window == 0x7fffffff ? 0 : v.pos0 - p.window + 1);
-    v.low1 = max(0, p.window == 0x7fffffff ? 0 : v.pos1 - p.window + 1);
-    v.end = max(0, v.pos1 + 1);
-    v.paged = len >> p.cache.log2b << p.cache.log2b;
-    const int qt = (min(v.end, v.paged) + 15) >> 4;
-    v.ns = min((min(p.sinks, v.low0) + 15) >> 4, qt);
-    v.w0 = min(v.low0 >> 4, qt);
-    if (v.ns >= v.w0) { v.ns = 0; v.w0 = 0; }
-    v.tiles = v.ns + qt - v.w0;
-    v.tail_tiles = v.end > v.paged ? (v.end - v.paged + 15) >> 4 : 0;
-    return v;
-}
-
-// One (sequence, kv head, block of R query rows).
-struct Unit {
-    int seq, h, rb, len, n, row0, rows;
-    View v;
-    int items;          // tiles of the page part and of the tail
-};
-__device__ __forceinline__ Unit make_unit(const Q8AttnParams& p, int unit, int r_per_block) {
-    Unit u;
-    u.rb = unit % p.row_blocks + p.row_block0;
-    unit /= p.row_blocks;
-    u.h = unit % p.cache.nkv; u.seq = unit / p.cache.nkv;
-    u.len = min(max(p.seq.lens[u.seq], 0), p.max_seq);
-    u.row0 = u.seq; u.n = 1;
-    if (p.q_offsets) {
-        u.row0 = p.q_offsets[u.seq];
-        u.n = min(p.q_offsets[u.seq + 1] - u.row0, p.max_q);
-        if (u.row0 < 0 || u.n < 0 || u.row0 > p.total_q - u.n) u.n = 0;
-    }
-    u.rows = u.n * p.qpk;
-    const int first = u.rb * r_per_block, last = min(first + r_per_block, u.rows) - 1;
-    u.v = make_view(p, u.len, u.n, first / p.qpk, max(last, 0) / p.qpk);
-    u.items = u.v.tiles + u.v.tail_tiles;
-    return u;
-}
-
-// Where row `row` of a unit's output starts, in elements.
-__device__ __forceinline__ size_t out_at(const Q8AttnParams& p, const Unit& u, int row, int d) {
-    return ((size_t)(u.row0 + row / p.qpk) * p.cache.nkv * p.qpk + u.h * p.qpk + row % p.qpk) * d;
-}
 __device__ __forceinline__ void store8(const Q8AttnParams& p, size_t at, const float (&x)[8]) {
     if (p.out_h) {
         *reinterpret_cast<uint4*>(p.out_h + at) =
@@ -233,7 +174,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
         for (int mt = 0; mt < T::MT; ++mt) o[nt][mt][0] = o[nt][mt][1] = o[nt][mt][2] = o[nt][mt][3] = 0.0f;
-        m[nt][0] = m[nt][1] = kUnset;
+        m[nt][0] = m[nt][1] = kQ8Unset;
         l[nt][0] = l[nt][1] = 0.0f;
     }
     // V's scales enter the fp16 probabilities relative to vref, a power of two not below any met so far (0: none yet)
@@ -271,7 +212,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
                 float top = fmaxf(s[0][nt][c], s[0][nt][c + 2]);
 #pragma unroll
                 for (int i = 1; i < TP; ++i) top = fmaxf(top, fmaxf(s[i][nt][c], s[i][nt][c + 2]));
-                raise |= top > m[nt][c] + kLazy;
+                raise |= top > m[nt][c] + kQ8Lazy;
             }
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -302,7 +243,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
 #pragma unroll
                     for (int e = 0; e < 4; ++e) o[nt][mt][e] *= a;
             vref = next;
-            vmul = kHeadroom / next;
+            vmul = kQ8Headroom / next;
         }
 #pragma unroll
         for (int i = 0; i < TP; ++i) {
@@ -567,7 +508,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
 
     // ---- merge: the CTA's warps through shared memory (over the ring), then the cluster's CTAs
     cp_async_wait<0>();
-    const float back = vref / kHeadroom;
+    const float back = vref / kQ8Headroom;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -694,7 +635,7 @@ __global__ void __launch_bounds__(256) q8_merge_kernel(const Q8AttnParams p) {
     if (u.rb * R >= u.rows) return;
     const float2* ml = p.part_ml + (size_t)blockIdx.x * p.parts * R;
     for (int r = warp; r < R; r += 8) {          // a lane per part
-        const float2 x = lane < live ? ml[lane * R + r] : make_float2(kUnset, 0.0f);
+        const float2 x = lane < live ? ml[lane * R + r] : make_float2(kQ8Unset, 0.0f);
         float top = x.x;
 #pragma unroll
         for (int k = 16; k > 0; k /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
@@ -833,6 +774,7 @@ size_t q8_attention_workspace(int nkv, int qpk, int d, int block, int batch, int
 
 cudaError_t launch_q8_attention(const Q8AttnParams& args, int d, int fmt, void* workspace, cudaStream_t stream) {
     Q8AttnParams p = args;
+    if (const char* e = getenv("KIVI_Q8_PROMPT")) if (!p.mass && p.max_q * p.qpk >= atoi(e)) return launch_q8_prompt(p, d, fmt, stream);
     const Plan plan = make_plan(p.cache.nkv, p.qpk, d, 1 << p.cache.log2b, p.seq.batch, p.max_q, p.max_seq, p.window, p.sinks, p.mass != nullptr);
     p.ws_tiles = plan.tiles;
     p.parts = plan.parts; p.chunk = plan.chunk; p.cluster = plan.cluster;

@@ -30,6 +30,7 @@ __device__ __forceinline__ int q8_slot(const Q8Seqs& s, int i) { return s.slots 
 // Sequences and ids a launch refused (kivi_b200_q8_rejected_indices adds the files' counters up).
 cudaError_t q8_cache_rejected(unsigned int* count);
 cudaError_t q8_attention_rejected(unsigned int* count);
+cudaError_t q8_prompt_rejected(unsigned int* count);
 
 // Two codes (the low 16 bits of `codes`) as a pair of fp16 values; every e4m3 value is an fp16 value.
 __device__ __forceinline__ uint32_t q8_e4m3_pair(uint16_t codes) {
@@ -93,6 +94,66 @@ struct Q8AttnParams {
     int parts, chunk, cluster;     // parts a unit's tiles are cut into, of `chunk` tiles each; whether they form a cluster
     int row_blocks, row_block0;
 };
+// The keys a block of query rows sees: [0, sinks) and [low, end), as 16-token tiles.
+struct View {
+    int len, n;          // tokens, query rows' tokens
+    int pos0, pos1;      // positions of the block's first and last query token
+    int low0, low1;      // first windowed key of those two
+    int end;             // keys [0, end) are at most seen
+    int paged;           // tokens held in pages
+    int ns, w0, tiles;   // page tiles: 0 .. ns - 1, then w0 ..; `tiles` in all
+    int tail_tiles;
+};
+__device__ __forceinline__ View make_view(const Q8AttnParams& p, int len, int n, int tok0, int tok1) {
+    View v;
+    v.len = len; v.n = n;
+    v.pos0 = len - n + tok0; v.pos1 = len - n + tok1;
+    v.low0 = max(0, p.window == 0x7fffffff ? 0 : v.pos0 - p.window + 1);
+    v.low1 = max(0, p.window == 0x7fffffff ? 0 : v.pos1 - p.window + 1);
+    v.end = max(0, v.pos1 + 1);
+    v.paged = len >> p.cache.log2b << p.cache.log2b;
+    const int qt = (min(v.end, v.paged) + 15) >> 4;
+    v.ns = min((min(p.sinks, v.low0) + 15) >> 4, qt);
+    v.w0 = min(v.low0 >> 4, qt);
+    if (v.ns >= v.w0) { v.ns = 0; v.w0 = 0; }
+    v.tiles = v.ns + qt - v.w0;
+    v.tail_tiles = v.end > v.paged ? (v.end - v.paged + 15) >> 4 : 0;
+    return v;
+}
+
+// One (sequence, kv head, block of R query rows).
+struct Unit {
+    int seq, h, rb, len, n, row0, rows;
+    View v;
+    int items;          // tiles of the page part and of the tail
+};
+__device__ __forceinline__ Unit make_unit(const Q8AttnParams& p, int unit, int r_per_block) {
+    Unit u;
+    u.rb = unit % p.row_blocks + p.row_block0;
+    unit /= p.row_blocks;
+    u.h = unit % p.cache.nkv; u.seq = unit / p.cache.nkv;
+    u.len = min(max(p.seq.lens[u.seq], 0), p.max_seq);
+    u.row0 = u.seq; u.n = 1;
+    if (p.q_offsets) {
+        u.row0 = p.q_offsets[u.seq];
+        u.n = min(p.q_offsets[u.seq + 1] - u.row0, p.max_q);
+        if (u.row0 < 0 || u.n < 0 || u.row0 > p.total_q - u.n) u.n = 0;
+    }
+    u.rows = u.n * p.qpk;
+    const int first = u.rb * r_per_block, last = min(first + r_per_block, u.rows) - 1;
+    u.v = make_view(p, u.len, u.n, first / p.qpk, max(last, 0) / p.qpk);
+    u.items = u.v.tiles + u.v.tail_tiles;
+    return u;
+}
+
+// Where row `row` of a unit's output starts, in elements.
+__device__ __forceinline__ size_t out_at(const Q8AttnParams& p, const Unit& u, int row, int d) {
+    return ((size_t)(u.row0 + row / p.qpk) * p.cache.nkv * p.qpk + u.h * p.qpk + row % p.qpk) * d;
+}
+constexpr float kQ8Unset = -3.0e38f;     // running maximum before any visible token
+constexpr float kQ8Lazy = 8.0f;          // the maximum is raised when a score tops it by 2^8
+constexpr float kQ8Headroom = 64.0f;     // probabilities in fp16 carry 2^6: p vs <= 2^8 2^6 < 65504, 2^20 below 1 stay normal
+
 struct Q8EvictParams {
     const int* tables; int width;
     const int* lens; const float* mass; int mass_width;
@@ -103,6 +164,8 @@ cudaError_t launch_q8_write(const Q8WriteParams& p, int d, int fmt, cudaStream_t
 cudaError_t launch_q8_read(const Q8ReadParams& p, int d, int fmt, cudaStream_t stream);
 cudaError_t launch_q8_attention(const Q8AttnParams& p, int d, int fmt, void* workspace, cudaStream_t stream);
 size_t q8_attention_workspace(int nkv, int qpk, int d, int block, int batch, int max_q, int max_seq, int window, int sinks, bool mass);
+cudaError_t launch_q8_prompt(const Q8AttnParams& p, int d, int fmt, cudaStream_t stream);
+cudaError_t q8_prompt_failures(unsigned int* count);
 cudaError_t launch_q8_evict(const Q8EvictParams& p, cudaStream_t stream);
 int q8_evict_max_pages();
 

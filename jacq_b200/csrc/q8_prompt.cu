@@ -1,0 +1,438 @@
+// Attention over the 8-bit block-scaled cache for many query rows: prompts and long runs of tokens, on tcgen05.
+//
+// Same mathematics as the kernel for few rows: codes are exact in fp16, K's page scale multiplies the scores, V's goes
+// into the probabilities. A unit is 128 query rows (token-major, the query heads of one kv head inside) of one sequence
+// and kv head; keys come 128 at a time, as eight 16-token tiles of whatever pages are seen:
+//
+//   S[128 x 128] = Q Kc^T     operands in shared memory, accumulator in tensor memory
+//   P = 2^(S f - m) vs'       four warps, a thread per row: no shuffles; P goes back to tensor memory, over S
+//   O[128 x D]  += P Vc       P from tensor memory, Vc from shared memory with the channels as its leading dimension
+//
+// Work is split by warps: 0 .. 3 softmax and epilogue, 4 .. 7 load codes and write them as fp16 into the swizzled tiles,
+// one thread of warp 8 issues the products. At 128 rows a byte of codes is worth 256 flops, so the tensor pipe (4 * 128 *
+// 128 * D flops a step) and the exponentials (128 * 128, 16 a cycle) bound it, not HBM. Two CTAs share a multiprocessor
+// (96 KB of shared memory and 256 columns of tensor memory each at D = 128): one's products run under the other's
+// exponentials. Every wait is bounded: a CTA whose wait gave up counts itself, waits for its products and leaves.
+#include "q8_common.cuh"
+
+namespace kivi {
+namespace {
+
+constexpr int kRows = 128, kKeys = 128, kThreads = 288;
+constexpr int kAtom = 128 * 128;   // bytes of 128 rows of 64 fp16 values, 128-byte swizzled
+
+__device__ unsigned int g_q8_prompt_failures, g_q8_prompt_rejected;
+
+__device__ __forceinline__ bool wait_bar(uint64_t* bar, uint32_t parity) {
+    for (int it = 0; it < (1 << 17); ++it)
+        if (mbar_try_wait(bar, parity)) return true;
+    return false;
+}
+__device__ __forceinline__ void arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void commit(uint64_t* bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+
+// 128-byte-swizzled operand tiles: 8-row groups 1024 bytes apart. `lead`: bytes between 64-element column groups, which
+// the layout asks for where the rows are the contraction (V: keys down, channels across).
+__device__ __forceinline__ uint64_t operand(uint32_t smem, uint32_t lead) {
+    return (uint64_t)((smem & 0x3FFFFu) >> 4) | ((uint64_t)(lead >> 4) << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+// kind::f16 with fp32 accumulator (bit 4), fp16 operands; bit 16: B's contraction runs down its rows; N >> 3, M >> 4
+__host__ __device__ constexpr uint32_t shape(int n, bool b_rows) {
+    return (1u << 4) | ((b_rows ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
+}
+__device__ __forceinline__ void product_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                 ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+__device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                 ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
+}
+__device__ __forceinline__ void load32(uint32_t at, float (&v)[32]) {   // 32 columns of the thread's row; whole warps
+    uint32_t r[32];
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void store32(uint32_t at, const float (&v)[32]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
+        ::"f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]),
+          "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]),
+          "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]),
+          "f"(v[31]), "r"(at) : "memory");
+}
+__device__ __forceinline__ void store16(uint32_t at, const uint32_t (&v)[16]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};"
+        ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+          "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(at) : "memory");
+}
+__device__ __forceinline__ void store_wait() { __syncwarp(); asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
+    asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// Byte address of the 16-byte chunk `j` (8 values) of row `row` in a swizzled tile.
+__device__ __forceinline__ uint32_t chunk_at(int row, int j) {
+    return (uint32_t)((j >> 3) * kAtom + row * 128 + (((j & 7) ^ (row & 7)) << 4));
+}
+__device__ __forceinline__ bool odd_half(uint32_t w) { return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u; }
+
+template <int D>
+constexpr int tmem_columns() { return D == 256 ? 512 : 256; }
+template <int D>
+constexpr int smem_bytes() { return 3 * kRows * D * 2 + 1024; }
+
+template <int D, int FMT>
+__global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(const Q8AttnParams p) {
+    constexpr int CPR = D / 16;            // 16-byte chunks of a row of codes
+    constexpr int TILE = kRows * D * 2;    // bytes of an fp16 operand tile
+    extern __shared__ unsigned char raw[];
+    __shared__ uint64_t full_k, full_v, s_ready, p_ready, pv_done, drained;
+    __shared__ uint32_t tmem_slot;
+    __shared__ float meta_ks[2][8], meta_vs[2][8];
+    __shared__ int meta_key0[2][8];
+    __shared__ int odd_v;                  // a tail row held an infinity or NaN in V
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int nkv = p.cache.nkv, block = 1 << p.cache.log2b;
+    // the last rows first: without a window they have the most keys
+    const int at_block = blockIdx.x % p.row_blocks;
+    const Unit u = make_unit(p, blockIdx.x - at_block + (p.row_blocks - 1 - at_block), kRows);
+    if (u.rb * kRows >= u.rows) return;
+    const View& v = u.v;
+    const int steps = (u.items + 7) >> 3;
+    const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u, q_tile = smem, k_tile = smem + TILE, v_tile = smem + 2 * TILE;
+
+    if (tid == 0) {
+        mbar_init(&full_k, 128); mbar_init(&full_v, 128); mbar_init(&p_ready, 128);
+        mbar_init(&s_ready, 1); mbar_init(&pv_done, 1); mbar_init(&drained, 1);
+        fence_barrier_init();
+        odd_v = 0;
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                     ::"r"(smem_u32(&tmem_slot)), "n"(tmem_columns<D>()) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    for (int e = tid; e < kRows * (D / 8); e += kThreads) {   // query rows
+        const int row = e / (D / 8), j = e % (D / 8), r = u.rb * kRows + row;
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (r < u.rows)
+            x = *reinterpret_cast<const uint4*>(p.q + (long long)(u.row0 + r / p.qpk) * p.q_stride + (size_t)(u.h * p.qpk + r % p.qpk) * D + 8 * j);
+        sts128(q_tile + chunk_at(row, j), x);
+    }
+    fence_proxy_async();
+    fence_before();
+    __syncthreads();
+    fence_after();
+    const uint32_t tmem_s = *reinterpret_cast<volatile uint32_t*>(&tmem_slot), tmem_o = tmem_s + kKeys;
+    bool failed = false;
+
+    // row of a softmax thread
+    const int r = u.rb * kRows + (tid & 127);
+    const int hi = r < u.rows ? u.len - u.n + r / p.qpk : -1;
+    const int lo = p.window == 0x7fffffff ? 0 : hi - p.window + 1;
+    auto sees = [&](int key) { return key <= hi && (key >= lo || key < p.sinks); };
+
+    if (warp < 4) {
+        const uint32_t mine = (uint32_t)(warp * 32) << 16;   // this warp's lanes of tensor memory
+        float m = kQ8Unset, l = 0.0f, vref = 0.0f, vmul = 0.0f;
+        for (int i = 0; i < steps; ++i) {
+            const int b = i & 1;
+            if (!wait_bar(&s_ready, b)) { failed = true; break; }
+            fence_after();
+            unsigned inside = 0;
+            float top = -INFINITY, vtop = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int key0 = meta_key0[b][j];
+                if (key0 + 15 <= hi && (key0 >= lo || key0 + 16 <= p.sinks)) inside |= 1u << j;
+                vtop = fmaxf(vtop, meta_vs[b][j]);
+            }
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float s[32];
+                load32(tmem_s + mine + 32 * c, s);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int j = 2 * c + half;
+                    float x = -INFINITY;
+                    if (inside >> j & 1) {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) x = fmaxf(x, s[16 * half + e]);
+                    } else {
+                        const int key0 = meta_key0[b][j];
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) if (sees(key0 + e)) x = fmaxf(x, s[16 * half + e]);
+                    }
+                    // scales are not negative; a tile of which nothing is seen stays at -infinity
+                    if (x != -INFINITY) top = fmaxf(top, x * (meta_ks[b][j] * p.scale_log2));
+                }
+            }
+            const bool raise = top > m + kQ8Lazy;
+            if (__any_sync(0xffffffffu, raise || vtop > vref)) {
+                const float mn = fmaxf(m, top);
+                float a = fast_exp2(m - mn);
+                m = mn;
+                l *= a;
+                if (vtop > vref) {
+                    const float next = __uint_as_float((__float_as_uint(vtop) & 0x7f800000u) + 0x00800000u);
+                    a *= vref / next;
+                    vref = next;
+                    vmul = kQ8Headroom / next;
+                }
+                if (i > 0) {   // S of this step is there, so the products of the one before are done with O
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) {
+                        float o[32];
+                        load32(tmem_o + mine + 32 * c, o);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] *= a;
+                        store32(tmem_o + mine + 32 * c, o);
+                    }
+                }
+            }
+            // P over S: columns of P lie below the columns of S that are still to be read
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float s[32];
+                load32(tmem_s + mine + 32 * c, s);
+                uint32_t out[16];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int j = 2 * c + half;
+                    const float f = meta_ks[b][j] * p.scale_log2, w = meta_vs[b][j] * vmul;
+                    const bool in = inside >> j & 1;
+                    const int key0 = meta_key0[b][j];
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        float x = fast_exp2(fmaf(s[16 * half + e], f, -m)), y = fast_exp2(fmaf(s[16 * half + e + 1], f, -m));
+                        float px = x * w, py = y * w;
+                        if (!in) {   // masked keys weigh 0 whatever the scores and scales are
+                            if (!sees(key0 + e)) x = px = 0.0f;
+                            if (!sees(key0 + e + 1)) y = py = 0.0f;
+                        }
+                        l += x + y;
+                        out[8 * half + e / 2] = pack_half2(px, py);
+                    }
+                }
+                store16(tmem_s + mine + 16 * c, out);
+            }
+            store_wait();
+            fence_before();
+            arrive(&p_ready);
+        }
+        if (!failed && steps > 0 && !wait_bar(&pv_done, (steps - 1) & 1)) failed = true;
+        fence_after();
+        const float scale = l != 0.0f ? vref / kQ8Headroom / l : 0.0f;
+        const size_t at = r < u.rows ? out_at(p, u, r, D) : 0;
+        for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            if (steps > 0) {
+                load32(tmem_o + mine + 32 * c, o);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = l != 0.0f ? o[e] * scale : 0.0f;
+            if (r >= u.rows) {
+                // a row behind the last: nothing to store
+            } else if (p.out_h) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 8)
+                    *reinterpret_cast<uint4*>(p.out_h + at + 32 * c + e) = make_uint4(
+                        pack_half2(o[e], o[e + 1]), pack_half2(o[e + 2], o[e + 3]), pack_half2(o[e + 4], o[e + 5]), pack_half2(o[e + 6], o[e + 7]));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; e += 4)
+                    *reinterpret_cast<float4*>(p.out + at + 32 * c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+            }
+        }
+    } else if (warp < 8) {
+        const int c = tid - 128;
+        const int sub_mask = (block >> 4) - 1, sub_log = p.cache.log2b - 4;
+        const int* table = p.seq.tables + (size_t)u.seq * p.seq.width;
+        int slot = q8_slot(p.seq, u.seq);
+        if (!index_in_pool(slot, p.cache.num_slots)) {
+            if (c == 0 && v.tail_tiles) atomicAdd(&g_q8_prompt_rejected, 1u);
+            slot = 0;
+        }
+        auto tile_of = [&](int item) { return item < v.ns ? item : item - v.ns + v.w0; };
+        auto unseen = [&](int key) { return key >= v.end || (key < v.low0 && key >= p.sinks); };
+        // lanes 0 .. 7 hold the page ids of the step's eight tiles
+        auto load_id = [&](int i) {
+            const int item = 8 * i + (lane & 7);
+            if (item >= v.tiles) return 0;
+            const int page = tile_of(item) >> sub_log;
+            return page < p.seq.width ? table[page] : -1;
+        };
+        int id = load_id(0);
+        for (int i = 0; i < steps && !failed; ++i) {
+            if (!index_in_pool(id, p.cache.num_blocks)) {
+                if (c < 8) atomicAdd(&g_q8_prompt_rejected, 1u);
+                id = 0;
+            }
+            const int id_next = i + 1 < steps ? load_id(i + 1) : 0;
+            const int first = 8 * i, b = i & 1;
+            float2 sc = make_float2(0.0f, 0.0f);
+            int key0 = 0x3fffffff;                       // a tile that is not there: no row sees that far
+            if (c < 8) {
+                const int item = first + c;
+                if (item < v.tiles) { sc = p.cache.scales[(size_t)id * nkv + u.h]; key0 = tile_of(item) * 16; }
+                else if (item < u.items) { sc = make_float2(1.0f, 1.0f); key0 = v.paged + (item - v.tiles) * 16; }
+            }
+#pragma unroll
+            for (int which = 0; which < 2; ++which) {
+                const uint8_t* codes = which ? p.cache.v : p.cache.k;
+                const __half* tail = (which ? p.cache.v_tail : p.cache.k_tail) + ((size_t)slot * nkv + u.h) * block * D;
+                const uint32_t dst = which ? v_tile : k_tile;
+                // codes of this thread's chunks are on their way while the tile is still in use
+                uint4 x[CPR];
+#pragma unroll
+                for (int k = 0; k < CPR; ++k) {
+                    const int e = k * 128 + c, row = e / CPR, sub = row >> 4, item = first + sub;
+                    const int page = __shfl_sync(0xffffffffu, id, sub);
+                    x[k] = make_uint4(0u, 0u, 0u, 0u);
+                    if (item < v.tiles) {
+                        const int tile = tile_of(item);
+                        if (!unseen(tile * 16 + (row & 15)))
+                            x[k] = __ldg(reinterpret_cast<const uint4*>(
+                                codes + (((size_t)page * nkv + u.h) * block + (tile & sub_mask) * 16 + (row & 15)) * D + (e % CPR) * 16));
+                    }
+                }
+                if (i > 0 && !wait_bar(which ? &pv_done : &s_ready, (i - 1) & 1)) { failed = true; break; }
+                if (which == 0 && c < 8) { meta_ks[b][c] = sc.x; meta_vs[b][c] = sc.y; meta_key0[b][c] = key0; }
+#pragma unroll
+                for (int k = 0; k < CPR; ++k) {
+                    const int e = k * 128 + c, row = e / CPR, chunk = e % CPR, item = first + (row >> 4);
+                    uint4 lo4, hi4;
+                    if (item >= v.tiles && item < u.items) {   // fp16 rows of the tail
+                        const int at = (item - v.tiles) * 16 + (row & 15);
+                        lo4 = hi4 = make_uint4(0u, 0u, 0u, 0u);
+                        if (!unseen(v.paged + at)) {
+                            lo4 = *reinterpret_cast<const uint4*>(tail + (size_t)at * D + chunk * 16);
+                            hi4 = *reinterpret_cast<const uint4*>(tail + (size_t)at * D + chunk * 16 + 8);
+                        }
+                        if (which) {   // 0 * infinity would reach rows that do not see the token: out, and seen to at the end
+                            uint32_t w[8] = {lo4.x, lo4.y, lo4.z, lo4.w, hi4.x, hi4.y, hi4.z, hi4.w};
+                            bool odd = false;
+#pragma unroll
+                            for (int z = 0; z < 8; ++z) {
+                                odd |= odd_half(w[z]);
+                                if ((w[z] & 0x7c00u) == 0x7c00u) w[z] &= 0xffff0000u;
+                                if ((w[z] & 0x7c000000u) == 0x7c000000u) w[z] &= 0x0000ffffu;
+                            }
+                            if (odd) {
+                                odd_v = 1;
+                                lo4 = make_uint4(w[0], w[1], w[2], w[3]); hi4 = make_uint4(w[4], w[5], w[6], w[7]);
+                            }
+                        }
+                    } else {
+                        q8_unpack<FMT>(x[k].x, lo4.x, lo4.y); q8_unpack<FMT>(x[k].y, lo4.z, lo4.w);
+                        q8_unpack<FMT>(x[k].z, hi4.x, hi4.y); q8_unpack<FMT>(x[k].w, hi4.z, hi4.w);
+                    }
+                    // the two halves of the row's threads store in opposite order, so that eight threads meet eight bank groups
+                    const bool flip = chunk & 4;
+                    sts128(dst + chunk_at(row, 2 * chunk + (flip ? 1 : 0)), flip ? hi4 : lo4);
+                    sts128(dst + chunk_at(row, 2 * chunk + (flip ? 0 : 1)), flip ? lo4 : hi4);
+                }
+                fence_proxy_async();
+                arrive(which ? &full_v : &full_k);
+            }
+            id = id_next;
+        }
+    } else if (lane == 0) {
+        constexpr uint32_t qk = shape(kKeys, false), pv = shape(D, true);
+        for (int i = 0; i < steps; ++i) {
+            const uint32_t parity = i & 1;
+            // S gives way to P and P to the next S: the products that read P are done first
+            if (!wait_bar(&full_k, parity) || (i > 0 && !wait_bar(&pv_done, parity ^ 1u))) { failed = true; break; }
+            __threadfence_block();   // what the loading warps left beside the tile goes on to those that wait for s_ready
+            fence_after();
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k) {   // 16 channels: 32 bytes on in the swizzled row, the next 64 in the next atom
+                const uint32_t at = (k >> 2) * kAtom + (k & 3) * 32;
+                product_ss(tmem_s, operand(q_tile + at, 16), operand(k_tile + at, 16), qk, k > 0);
+            }
+            commit(&s_ready);
+            if (!wait_bar(&full_v, parity) || !wait_bar(&p_ready, parity)) { failed = true; break; }
+            fence_after();
+#pragma unroll
+            for (int k = 0; k < kKeys / 16; ++k)   // 16 keys: 8 columns of P, 16 rows of V
+                product_ts(tmem_o, tmem_s + 8 * k, operand(v_tile + 2048 * k, kAtom), pv, i > 0 || k > 0);
+            commit(&pv_done);
+        }
+        commit(&drained);
+        if (!wait_bar(&drained, 0)) failed = true;
+    }
+    __syncwarp();
+    fence_before();
+    const bool cta_failed = __syncthreads_or(failed);
+    if (warp == 8)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_s), "n"(tmem_columns<D>()) : "memory");
+    if (cta_failed && tid == 0) atomicAdd(&g_q8_prompt_failures, 1u);
+    if (odd_v && warp < 4 && r < u.rows) {
+        // rare: rows that see a tail token whose V holds an infinity or NaN yield NaN in that channel
+        int slot = q8_slot(p.seq, u.seq);
+        if (!index_in_pool(slot, p.cache.num_slots)) slot = 0;
+        const __half* tail = p.cache.v_tail + ((size_t)slot * nkv + u.h) * block * D;
+        const size_t at = out_at(p, u, r, D);
+        for (int j = 0; v.paged + j < v.end; ++j) {
+            if (!sees(v.paged + j)) continue;
+            for (int ch = 0; ch < D; ++ch) {
+                if ((__half_as_ushort(tail[(size_t)j * D + ch]) & 0x7c00u) != 0x7c00u) continue;
+                if (p.out_h) p.out_h[at + ch] = __ushort_as_half((unsigned short)0x7fff);
+                else p.out[at + ch] = __int_as_float(0x7fc00000);
+            }
+        }
+    }
+}
+
+template <int D, int FMT>
+cudaError_t launch(const Q8AttnParams& p, cudaStream_t stream) {
+    auto kernel = q8_prompt_kernel<D, FMT>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<D>());
+    if (e != cudaSuccess) return e;
+    kernel<<<(unsigned)((size_t)p.seq.batch * p.cache.nkv * p.row_blocks), kThreads, smem_bytes<D>(), stream>>>(p);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_q8_prompt(const Q8AttnParams& args, int d, int fmt, cudaStream_t stream) {
+    Q8AttnParams p = args;
+    p.row_blocks = (p.max_q * p.qpk + kRows - 1) / kRows;
+    p.row_block0 = 0;
+    const bool i8 = fmt == KIVI_Q8_INT8;
+    switch (d) {
+        case 64: return i8 ? launch<64, KIVI_Q8_INT8>(p, stream) : launch<64, KIVI_Q8_E4M3>(p, stream);
+        case 128: return i8 ? launch<128, KIVI_Q8_INT8>(p, stream) : launch<128, KIVI_Q8_E4M3>(p, stream);
+        default: return i8 ? launch<256, KIVI_Q8_INT8>(p, stream) : launch<256, KIVI_Q8_E4M3>(p, stream);
+    }
+}
+
+cudaError_t q8_prompt_rejected(unsigned int* count) { return cudaMemcpyFromSymbol(count, g_q8_prompt_rejected, sizeof(*count)); }
+cudaError_t q8_prompt_failures(unsigned int* count) { return cudaMemcpyFromSymbol(count, g_q8_prompt_failures, sizeof(*count)); }
+
+}  // namespace kivi
