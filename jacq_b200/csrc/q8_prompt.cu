@@ -153,6 +153,13 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
     const int hi = r < u.rows ? u.len - u.n + r / p.qpk : -1;
     const int lo = p.window == 0x7fffffff ? 0 : hi - p.window + 1;
     auto sees = [&](int key) { return key <= hi && (key >= lo || key < p.sinks); };
+    auto mask = [&](float (&s)[32], int key0, int key1) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            if (!sees(key0 + e)) s[e] = -INFINITY;
+            if (!sees(key1 + e)) s[16 + e] = -INFINITY;
+        }
+    };
 
     if (warp < 4) {
         const uint32_t mine = (uint32_t)(warp * 32) << 16;   // this warp's lanes of tensor memory
@@ -161,33 +168,25 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
             const int b = i & 1;
             if (!wait_bar(&s_ready, b)) { failed = true; break; }
             fence_after();
-            unsigned inside = 0;
+            bool all_in = true;
             float top = -INFINITY, vtop = 0.0f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int key0 = meta_key0[b][j];
-                if (key0 + 15 <= hi && (key0 >= lo || key0 + 16 <= p.sinks)) inside |= 1u << j;
+                all_in = all_in && key0 + 15 <= hi && (key0 >= lo || key0 + 16 <= p.sinks);
                 vtop = fmaxf(vtop, meta_vs[b][j]);
             }
-#pragma unroll
+            const bool masked = __any_sync(0xffffffffu, !all_in);
+#pragma unroll 1
             for (int c = 0; c < 4; ++c) {
                 float s[32];
                 load32(tmem_s + mine + 32 * c, s);
+                if (masked) mask(s, meta_key0[b][2 * c], meta_key0[b][2 * c + 1]);
+                float x = s[0], y = s[16];
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int j = 2 * c + half;
-                    float x = -INFINITY;
-                    if (inside >> j & 1) {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) x = fmaxf(x, s[16 * half + e]);
-                    } else {
-                        const int key0 = meta_key0[b][j];
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) if (sees(key0 + e)) x = fmaxf(x, s[16 * half + e]);
-                    }
-                    // scales are not negative; a tile of which nothing is seen stays at -infinity
-                    if (x != -INFINITY) top = fmaxf(top, x * (meta_ks[b][j] * p.scale_log2));
-                }
+                for (int e = 1; e < 16; ++e) { x = fmaxf(x, s[e]); y = fmaxf(y, s[16 + e]); }
+                // scales are not negative; a tile of which nothing is seen stays at -infinity (0 * infinity: fmaxf drops it)
+                top = fmaxf(top, fmaxf(x * (meta_ks[b][2 * c] * p.scale_log2), y * (meta_ks[b][2 * c + 1] * p.scale_log2)));
             }
             const bool raise = top > m + kQ8Lazy;
             if (__any_sync(0xffffffffu, raise || vtop > vref)) {
@@ -213,28 +212,28 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
                 }
             }
             // P over S: columns of P lie below the columns of S that are still to be read
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < 4; ++c) {
                 float s[32];
                 load32(tmem_s + mine + 32 * c, s);
+                if (masked) mask(s, meta_key0[b][2 * c], meta_key0[b][2 * c + 1]);
                 uint32_t out[16];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const int j = 2 * c + half;
-                    const float f = meta_ks[b][j] * p.scale_log2, w = meta_vs[b][j] * vmul;
-                    const bool in = inside >> j & 1;
-                    const int key0 = meta_key0[b][j];
+                    const float f = meta_ks[b][2 * c + half] * p.scale_log2, w = meta_vs[b][2 * c + half] * vmul;
+                    float sum = 0.0f;
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        float x = fast_exp2(fmaf(s[16 * half + e], f, -m)), y = fast_exp2(fmaf(s[16 * half + e + 1], f, -m));
+                    for (int e = 16 * half; e < 16 * half + 16; e += 2) {
+                        float x = fast_exp2(fmaf(s[e], f, -m)), y = fast_exp2(fmaf(s[e + 1], f, -m));
                         float px = x * w, py = y * w;
-                        if (!in) {   // masked keys weigh 0 whatever the scores and scales are
-                            if (!sees(key0 + e)) x = px = 0.0f;
-                            if (!sees(key0 + e + 1)) y = py = 0.0f;
+                        if (masked) {   // masked keys weigh 0 whatever the scales are
+                            if (s[e] == -INFINITY) x = px = 0.0f;
+                            if (s[e + 1] == -INFINITY) y = py = 0.0f;
                         }
-                        l += x + y;
-                        out[8 * half + e / 2] = pack_half2(px, py);
+                        sum += x + y;
+                        out[e / 2] = pack_half2(px, py);
                     }
+                    l += sum;
                 }
                 store16(tmem_s + mine + 16 * c, out);
             }
@@ -280,7 +279,12 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
         }
         auto tile_of = [&](int item) { return item < v.ns ? item : item - v.ns + v.w0; };
         auto unseen = [&](int key) { return key >= v.end || (key < v.low0 && key >= p.sinks); };
-        // lanes 0 .. 7 hold the page ids of the step's eight tiles
+        // This thread's chunks: row16 and chunk of tile sub_of(k), k = 0 .. CPR - 1. Page codes are finite, so masked tokens'
+        // rows may stay what they are; tail rows, which may hold anything, are fetched as zeros where nobody sees them.
+        const int chunk = c % CPR;
+        auto sub_of = [&](int k) { return D == 64 ? 2 * k + (c >> 6) : D == 128 ? k : k >> 1; };
+        auto row_of = [&](int k) { return D == 64 ? (c >> 2) & 15 : D == 128 ? c >> 3 : (k & 1) * 8 + (c >> 4); };
+        // lanes 0 .. 7 hold where the step's eight tiles start
         auto load_id = [&](int i) {
             const int item = 8 * i + (lane & 7);
             if (item >= v.tiles) return 0;
@@ -288,79 +292,72 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
             return page < p.seq.width ? table[page] : -1;
         };
         int id = load_id(0);
+#pragma unroll 1
         for (int i = 0; i < steps && !failed; ++i) {
             if (!index_in_pool(id, p.cache.num_blocks)) {
                 if (c < 8) atomicAdd(&g_q8_prompt_rejected, 1u);
                 id = 0;
             }
-            const int id_next = i + 1 < steps ? load_id(i + 1) : 0;
-            const int first = 8 * i, b = i & 1;
+            const int first = 8 * i, b = i & 1, tile = tile_of(first + (lane & 7));
+            const size_t start = (((size_t)id * nkv + u.h) * block + (size_t)(tile & sub_mask) * 16) * D;
+            const int paged = min(8, max(0, v.tiles - first)), there = min(8, u.items - first);   // tiles of pages; of any kind
             float2 sc = make_float2(0.0f, 0.0f);
             int key0 = 0x3fffffff;                       // a tile that is not there: no row sees that far
-            if (c < 8) {
-                const int item = first + c;
-                if (item < v.tiles) { sc = p.cache.scales[(size_t)id * nkv + u.h]; key0 = tile_of(item) * 16; }
-                else if (item < u.items) { sc = make_float2(1.0f, 1.0f); key0 = v.paged + (item - v.tiles) * 16; }
-            }
-#pragma unroll
+            if (c < paged) { sc = p.cache.scales[(size_t)id * nkv + u.h]; key0 = tile * 16; }
+            else if (c < there) { sc = make_float2(1.0f, 1.0f); key0 = v.paged + (first + c - v.tiles) * 16; }
+            id = i + 1 < steps ? load_id(i + 1) : 0;
+#pragma unroll 1
             for (int which = 0; which < 2; ++which) {
-                const uint8_t* codes = which ? p.cache.v : p.cache.k;
-                const __half* tail = (which ? p.cache.v_tail : p.cache.k_tail) + ((size_t)slot * nkv + u.h) * block * D;
+                const uint8_t* codes = (which ? p.cache.v : p.cache.k) + chunk * 16;
                 const uint32_t dst = which ? v_tile : k_tile;
                 // codes of this thread's chunks are on their way while the tile is still in use
                 uint4 x[CPR];
 #pragma unroll
                 for (int k = 0; k < CPR; ++k) {
-                    const int e = k * 128 + c, row = e / CPR, sub = row >> 4, item = first + sub;
-                    const int page = __shfl_sync(0xffffffffu, id, sub);
+                    const size_t at = __shfl_sync(0xffffffffu, start, sub_of(k));
                     x[k] = make_uint4(0u, 0u, 0u, 0u);
-                    if (item < v.tiles) {
-                        const int tile = tile_of(item);
-                        if (!unseen(tile * 16 + (row & 15)))
-                            x[k] = __ldg(reinterpret_cast<const uint4*>(
-                                codes + (((size_t)page * nkv + u.h) * block + (tile & sub_mask) * 16 + (row & 15)) * D + (e % CPR) * 16));
-                    }
+                    if (sub_of(k) < paged) x[k] = __ldg(reinterpret_cast<const uint4*>(codes + at + row_of(k) * D));
                 }
                 if (i > 0 && !wait_bar(which ? &pv_done : &s_ready, (i - 1) & 1)) { failed = true; break; }
                 if (which == 0 && c < 8) { meta_ks[b][c] = sc.x; meta_vs[b][c] = sc.y; meta_key0[b][c] = key0; }
+                // the two halves of a row's threads store in opposite order, so that eight threads meet eight bank groups
+                const bool flip = chunk & 4;
 #pragma unroll
                 for (int k = 0; k < CPR; ++k) {
-                    const int e = k * 128 + c, row = e / CPR, chunk = e % CPR, item = first + (row >> 4);
+                    const int row = sub_of(k) * 16 + row_of(k);
                     uint4 lo4, hi4;
-                    if (item >= v.tiles && item < u.items) {   // fp16 rows of the tail
-                        const int at = (item - v.tiles) * 16 + (row & 15);
-                        lo4 = hi4 = make_uint4(0u, 0u, 0u, 0u);
+                    q8_unpack<FMT>(x[k].x, lo4.x, lo4.y); q8_unpack<FMT>(x[k].y, lo4.z, lo4.w);
+                    q8_unpack<FMT>(x[k].z, hi4.x, hi4.y); q8_unpack<FMT>(x[k].w, hi4.z, hi4.w);
+                    sts128(dst + chunk_at(row, 2 * chunk + (flip ? 1 : 0)), flip ? hi4 : lo4);
+                    sts128(dst + chunk_at(row, 2 * chunk + (flip ? 0 : 1)), flip ? lo4 : hi4);
+                }
+                if (there > paged) {                     // the step's tail tiles, over what was just written there
+                    const __half* tail = (which ? p.cache.v_tail : p.cache.k_tail) + ((size_t)slot * nkv + u.h) * block * D;
+#pragma unroll 1
+                    for (int k = 0; k < CPR; ++k) {
+                        if (sub_of(k) < paged || sub_of(k) >= there) continue;
+                        const int row = sub_of(k) * 16 + row_of(k), at = (first + sub_of(k) - v.tiles) * 16 + row_of(k);
+                        uint32_t w[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
                         if (!unseen(v.paged + at)) {
-                            lo4 = *reinterpret_cast<const uint4*>(tail + (size_t)at * D + chunk * 16);
-                            hi4 = *reinterpret_cast<const uint4*>(tail + (size_t)at * D + chunk * 16 + 8);
+                            const uint4* src = reinterpret_cast<const uint4*>(tail + (size_t)at * D + chunk * 16);
+                            const uint4 y = src[0], z = src[1];
+                            w[0] = y.x; w[1] = y.y; w[2] = y.z; w[3] = y.w; w[4] = z.x; w[5] = z.y; w[6] = z.z; w[7] = z.w;
                         }
                         if (which) {   // 0 * infinity would reach rows that do not see the token: out, and seen to at the end
-                            uint32_t w[8] = {lo4.x, lo4.y, lo4.z, lo4.w, hi4.x, hi4.y, hi4.z, hi4.w};
-                            bool odd = false;
 #pragma unroll
                             for (int z = 0; z < 8; ++z) {
-                                odd |= odd_half(w[z]);
+                                if (odd_half(w[z])) odd_v = 1;
                                 if ((w[z] & 0x7c00u) == 0x7c00u) w[z] &= 0xffff0000u;
                                 if ((w[z] & 0x7c000000u) == 0x7c000000u) w[z] &= 0x0000ffffu;
                             }
-                            if (odd) {
-                                odd_v = 1;
-                                lo4 = make_uint4(w[0], w[1], w[2], w[3]); hi4 = make_uint4(w[4], w[5], w[6], w[7]);
-                            }
                         }
-                    } else {
-                        q8_unpack<FMT>(x[k].x, lo4.x, lo4.y); q8_unpack<FMT>(x[k].y, lo4.z, lo4.w);
-                        q8_unpack<FMT>(x[k].z, hi4.x, hi4.y); q8_unpack<FMT>(x[k].w, hi4.z, hi4.w);
+                        sts128(dst + chunk_at(row, 2 * chunk), make_uint4(w[0], w[1], w[2], w[3]));
+                        sts128(dst + chunk_at(row, 2 * chunk + 1), make_uint4(w[4], w[5], w[6], w[7]));
                     }
-                    // the two halves of the row's threads store in opposite order, so that eight threads meet eight bank groups
-                    const bool flip = chunk & 4;
-                    sts128(dst + chunk_at(row, 2 * chunk + (flip ? 1 : 0)), flip ? hi4 : lo4);
-                    sts128(dst + chunk_at(row, 2 * chunk + (flip ? 0 : 1)), flip ? lo4 : hi4);
                 }
                 fence_proxy_async();
                 arrive(which ? &full_v : &full_k);
             }
-            id = id_next;
         }
     } else if (lane == 0) {
         constexpr uint32_t qk = shape(kKeys, false), pv = shape(D, true);
