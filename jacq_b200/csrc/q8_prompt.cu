@@ -19,6 +19,7 @@ namespace kivi {
 namespace {
 
 constexpr int kRows = 128, kKeys = 128, kThreads = 288;
+constexpr float kHeadroomLog = 6.0f;   // log2(kQ8Headroom)
 constexpr int kAtom = 128 * 128;   // bytes of 128 rows of 64 fp16 values, 128-byte swizzled
 
 __device__ unsigned int g_q8_prompt_failures, g_q8_prompt_rejected;
@@ -88,6 +89,32 @@ __device__ __forceinline__ void store16(uint32_t at, const uint32_t (&v)[16]) {
         ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
           "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(at) : "memory");
 }
+__device__ __forceinline__ void load16(uint32_t at, uint32_t (&r)[16]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(at) : "memory");
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// two fp32 values in one instruction
+__device__ __forceinline__ uint64_t pack2(float x, float y) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
 __device__ __forceinline__ void store_wait() { __syncwarp(); asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
     asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -110,8 +137,10 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
     extern __shared__ unsigned char raw[];
     __shared__ uint64_t full_k, full_v, s_ready, p_ready, pv_done, drained;
     __shared__ uint32_t tmem_slot;
-    __shared__ float meta_ks[2][8], meta_vs[2][8];
-    __shared__ int meta_key0[2][8];
+    // Of the two steps in flight, per 16-token tile: the factor of its scores, what the bias of int8 codes adds to them per
+    // sum of q, log2 of V's scale, the first key; per step: first and last key, the largest log2 of V's scale.
+    __shared__ float meta_f[2][8], meta_bias[2][8], meta_lv[2][8], step_lv[2];
+    __shared__ int meta_key0[2][8], step_key0[2], step_key1[2];
     __shared__ int odd_v;                  // a tail row held an infinity or NaN in V
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int nkv = p.cache.nkv, block = 1 << p.cache.log2b;
@@ -163,79 +192,107 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
 
     if (warp < 4) {
         const uint32_t mine = (uint32_t)(warp * 32) << 16;   // this warp's lanes of tensor memory
-        float m = kQ8Unset, l = 0.0f, vref = 0.0f, vmul = 0.0f;
+        float qsum = 0.0f;
+        if (FMT == KIVI_Q8_INT8) {
+            for (int j = 0; j < D / 8; ++j) {
+                const uint4 x = lds128(q_tile + chunk_at(tid, j));
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+                    qsum += y.x + y.y;
+                }
+            }
+        }
+        // P = 2^(s f - m) is kept below 2^8 by raising m when a 16-key sum says that it may not be: no pass over S for its
+        // maximum. In fp16 it carries V's scale relative to 2^vref, an exponent not below any scale's met so far, and 2^6.
+        float m = kQ8Unset, l = 0.0f, vref = -1000.0f;
+        auto rescale_o = [&](float a) {
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                float o[32];
+                load32(tmem_o + mine + 32 * c, o);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] *= a;
+                store32(tmem_o + mine + 32 * c, o);
+            }
+        };
+#pragma unroll 1
         for (int i = 0; i < steps; ++i) {
             const int b = i & 1;
             if (!wait_bar(&s_ready, b)) { failed = true; break; }
             fence_after();
-            bool all_in = true;
-            float top = -INFINITY, vtop = 0.0f;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int key0 = meta_key0[b][j];
-                all_in = all_in && key0 + 15 <= hi && (key0 >= lo || key0 + 16 <= p.sinks);
-                vtop = fmaxf(vtop, meta_vs[b][j]);
+            const int key0 = step_key0[b], key1 = step_key1[b];
+            const bool masked = __any_sync(0xffffffffu, key1 > hi || (key0 < lo && key1 >= p.sinks));
+            const float lv = step_lv[b];
+            if (lv > vref) {   // uniform; O of the step before is complete, as S of this one is there
+                const float next = floorf(lv) + 1.0f;
+                if (i > 0) rescale_o(fast_exp2(vref - next));
+                vref = next;
             }
-            const bool masked = __any_sync(0xffffffffu, !all_in);
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-                float s[32];
-                load32(tmem_s + mine + 32 * c, s);
-                if (masked) mask(s, meta_key0[b][2 * c], meta_key0[b][2 * c + 1]);
-                float x = s[0], y = s[16];
-#pragma unroll
-                for (int e = 1; e < 16; ++e) { x = fmaxf(x, s[e]); y = fmaxf(y, s[16 + e]); }
-                // scales are not negative; a tile of which nothing is seen stays at -infinity (0 * infinity: fmaxf drops it)
-                top = fmaxf(top, fmaxf(x * (meta_ks[b][2 * c] * p.scale_log2), y * (meta_ks[b][2 * c + 1] * p.scale_log2)));
-            }
-            const bool raise = top > m + kQ8Lazy;
-            if (__any_sync(0xffffffffu, raise || vtop > vref)) {
-                const float mn = fmaxf(m, top);
-                float a = fast_exp2(m - mn);
-                m = mn;
-                l *= a;
-                if (vtop > vref) {
-                    const float next = __uint_as_float((__float_as_uint(vtop) & 0x7f800000u) + 0x00800000u);
-                    a *= vref / next;
-                    vref = next;
-                    vmul = kQ8Headroom / next;
-                }
-                if (i > 0) {   // S of this step is there, so the products of the one before are done with O
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) {
-                        float o[32];
-                        load32(tmem_o + mine + 32 * c, o);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] *= a;
-                        store32(tmem_o + mine + 32 * c, o);
-                    }
-                }
-            }
-            // P over S: columns of P lie below the columns of S that are still to be read
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
                 float s[32];
                 load32(tmem_s + mine + 32 * c, s);
                 if (masked) mask(s, meta_key0[b][2 * c], meta_key0[b][2 * c + 1]);
                 uint32_t out[16];
+                float sum[2];
+                auto weigh = [&]() {
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const float f = meta_ks[b][2 * c + half] * p.scale_log2, w = meta_vs[b][2 * c + half] * vmul;
-                    float sum = 0.0f;
+                    for (int half = 0; half < 2; ++half) {
+                        const int j = 2 * c + half;
+                        const float f = meta_f[b][j], w = meta_lv[b][j] - vref + kHeadroomLog;
+                        const uint64_t ff = pack2(f, f), add = pack2(fmaf(-qsum, meta_bias[b][j], w - m), fmaf(-qsum, meta_bias[b][j], w - m));
+                        uint64_t acc = pack2(0.0f, 0.0f);
 #pragma unroll
-                    for (int e = 16 * half; e < 16 * half + 16; e += 2) {
-                        float x = fast_exp2(fmaf(s[e], f, -m)), y = fast_exp2(fmaf(s[e + 1], f, -m));
-                        float px = x * w, py = y * w;
-                        if (masked) {   // masked keys weigh 0 whatever the scales are
-                            if (s[e] == -INFINITY) x = px = 0.0f;
-                            if (s[e + 1] == -INFINITY) y = py = 0.0f;
+                        for (int e = 16 * half; e < 16 * half + 16; e += 2) {
+                            float x, y;
+                            unpack2(fma2(pack2(s[e], s[e + 1]), ff, add), x, y);
+                            x = fast_exp2(x);
+                            y = fast_exp2(y);
+                            if (masked) {   // masked keys weigh 0 whatever the scales are
+                                if (s[e] == -INFINITY) x = 0.0f;
+                                if (s[e + 1] == -INFINITY) y = 0.0f;
+                            }
+                            acc = add2(acc, pack2(x, y));
+                            out[e / 2] = pack_half2(x, y);
                         }
-                        sum += x + y;
-                        out[e / 2] = pack_half2(px, py);
+                        float x, y;
+                        unpack2(acc, x, y);
+                        sum[half] = (x + y) * fast_exp2(-w);
                     }
-                    l += sum;
+                };
+                weigh();
+                if (__any_sync(0xffffffffu, !(sum[0] + sum[1] <= 256.0f))) {
+                    // the first keys of a row, or scores far above all before them
+                    float x = -INFINITY, y = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        const float fx = meta_f[b][2 * c], fy = meta_f[b][2 * c + 1];
+                        if (!(masked && s[e] == -INFINITY)) x = fmaxf(x, fmaf(s[e], fx, -qsum * meta_bias[b][2 * c]));
+                        if (!(masked && s[16 + e] == -INFINITY)) y = fmaxf(y, fmaf(s[16 + e], fy, -qsum * meta_bias[b][2 * c + 1]));
+                    }
+                    // whole numbers: the factor is a power of two, and what is there already is not rounded again
+                    const float mn = fmaxf(m, ceilf(fmaxf(x, y))), a = fast_exp2(m - mn);
+                    m = mn;
+                    l *= a;
+                    if (i > 0) rescale_o(a);
+#pragma unroll 1
+                    for (int k = 0; k < c; ++k) {   // the chunks of P that are there already
+                        uint32_t w[16];
+                        load16(tmem_s + mine + 16 * k, w);
+                        const __half2 aa = __float2half2_rn(a);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&w[e]), aa);
+                            w[e] = *reinterpret_cast<const uint32_t*>(&h);
+                        }
+                        store16(tmem_s + mine + 16 * k, w);
+                    }
+                    weigh();
                 }
-                store16(tmem_s + mine + 16 * c, out);
+                l += sum[0] + sum[1];
+                store16(tmem_s + mine + 16 * c, out);   // over columns of S that have been read
             }
             store_wait();
             fence_before();
@@ -243,7 +300,7 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
         }
         if (!failed && steps > 0 && !wait_bar(&pv_done, (steps - 1) & 1)) failed = true;
         fence_after();
-        const float scale = l != 0.0f ? vref / kQ8Headroom / l : 0.0f;
+        const float scale = l != 0.0f ? fast_exp2(vref - kHeadroomLog) / l : 0.0f;
         const size_t at = r < u.rows ? out_at(p, u, r, D) : 0;
         for (int c = 0; c < D / 32; ++c) {
             float o[32];
@@ -299,14 +356,23 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
                 id = 0;
             }
             const int first = 8 * i, b = i & 1, tile = tile_of(first + (lane & 7));
-            const size_t start = (((size_t)id * nkv + u.h) * block + (size_t)(tile & sub_mask) * 16) * D;
+            const uint32_t start = ((uint32_t)id * nkv + u.h) * (uint32_t)(block >> 4) + (uint32_t)(tile & sub_mask);   // in tiles
             const int paged = min(8, max(0, v.tiles - first)), there = min(8, u.items - first);   // tiles of pages; of any kind
-            float2 sc = make_float2(0.0f, 0.0f);
+            float f = 0.0f, bias = 0.0f, lv = -1000.0f;
             int key0 = 0x3fffffff;                       // a tile that is not there: no row sees that far
-            if (c < paged) { sc = p.cache.scales[(size_t)id * nkv + u.h]; key0 = tile * 16; }
-            else if (c < there) { sc = make_float2(1.0f, 1.0f); key0 = v.paged + (first + c - v.tiles) * 16; }
+            if (c < paged) {
+                const float2 sc = p.cache.scales[(size_t)id * nkv + u.h];
+                f = sc.x * p.scale_log2;
+                // a zero scale's codes are zeros too: any other does; NaN stays
+                lv = sc.y == 0.0f ? -1000.0f : log2f(sc.y);
+                key0 = tile * 16;
+                if (FMT == KIVI_Q8_INT8) { bias = 128.0f * f; f *= 16777216.0f; }
+            } else if (c < there) {
+                f = p.scale_log2; lv = 0.0f;
+                key0 = v.paged + (first + c - v.tiles) * 16;
+            }
             id = i + 1 < steps ? load_id(i + 1) : 0;
-#pragma unroll 1
+#pragma unroll
             for (int which = 0; which < 2; ++which) {
                 const uint8_t* codes = (which ? p.cache.v : p.cache.k) + chunk * 16;
                 const uint32_t dst = which ? v_tile : k_tile;
@@ -314,22 +380,46 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
                 uint4 x[CPR];
 #pragma unroll
                 for (int k = 0; k < CPR; ++k) {
-                    const size_t at = __shfl_sync(0xffffffffu, start, sub_of(k));
+                    const uint32_t at = __shfl_sync(0xffffffffu, start, sub_of(k));
                     x[k] = make_uint4(0u, 0u, 0u, 0u);
-                    if (sub_of(k) < paged) x[k] = __ldg(reinterpret_cast<const uint4*>(codes + at + row_of(k) * D));
+                    if (sub_of(k) < paged) x[k] = __ldg(reinterpret_cast<const uint4*>(codes + (size_t)at * (16 * D) + row_of(k) * D));
                 }
                 if (i > 0 && !wait_bar(which ? &pv_done : &s_ready, (i - 1) & 1)) { failed = true; break; }
-                if (which == 0 && c < 8) { meta_ks[b][c] = sc.x; meta_vs[b][c] = sc.y; meta_key0[b][c] = key0; }
+                if (which == 0 && c < 32) {              // one warp: what the softmax has to know of the step
+                    float lv_top = lv;
+                    int k0 = key0, k1 = key0 + 15;
+#pragma unroll
+                    for (int z = 4; z > 0; z /= 2) {
+                        lv_top = fmaxf(lv_top, __shfl_xor_sync(0xffffffffu, lv_top, z));
+                        k0 = min(k0, __shfl_xor_sync(0xffffffffu, k0, z));
+                        k1 = max(k1, __shfl_xor_sync(0xffffffffu, k1, z));
+                    }
+                    if (c < 8) {
+                        meta_f[b][c] = f; meta_bias[b][c] = bias; meta_key0[b][c] = key0;
+                        meta_lv[b][c] = lv == -1000.0f ? fmaxf(lv_top, -100.0f) : lv;
+                    }
+                    if (c == 0) { step_lv[b] = fmaxf(lv_top, -100.0f); step_key0[b] = k0; step_key1[b] = k1; }
+                }
                 // the two halves of a row's threads store in opposite order, so that eight threads meet eight bank groups
                 const bool flip = chunk & 4;
 #pragma unroll
                 for (int k = 0; k < CPR; ++k) {
                     const int row = sub_of(k) * 16 + row_of(k);
-                    uint4 lo4, hi4;
-                    q8_unpack<FMT>(x[k].x, lo4.x, lo4.y); q8_unpack<FMT>(x[k].y, lo4.z, lo4.w);
-                    q8_unpack<FMT>(x[k].z, hi4.x, hi4.y); q8_unpack<FMT>(x[k].w, hi4.z, hi4.w);
-                    sts128(dst + chunk_at(row, 2 * chunk + (flip ? 1 : 0)), flip ? hi4 : lo4);
-                    sts128(dst + chunk_at(row, 2 * chunk + (flip ? 0 : 1)), flip ? lo4 : hi4);
+                    const uint32_t w[4] = {flip ? x[k].z : x[k].x, flip ? x[k].w : x[k].y, flip ? x[k].x : x[k].z, flip ? x[k].y : x[k].w};
+                    uint4 a, z;
+                    if (FMT == KIVI_Q8_INT8 && which == 0) {
+                        // K: a byte alone is a subnormal, (code + 128) 2^-24 exactly; the softmax takes the bias off the score
+                        const uint32_t h = 0x80808080u;
+                        a = make_uint4(__byte_perm(w[0] ^ h, 0u, 0x4140), __byte_perm(w[0] ^ h, 0u, 0x4342), __byte_perm(w[1] ^ h, 0u, 0x4140),
+                                       __byte_perm(w[1] ^ h, 0u, 0x4342));
+                        z = make_uint4(__byte_perm(w[2] ^ h, 0u, 0x4140), __byte_perm(w[2] ^ h, 0u, 0x4342), __byte_perm(w[3] ^ h, 0u, 0x4140),
+                                       __byte_perm(w[3] ^ h, 0u, 0x4342));
+                    } else {
+                        q8_unpack<FMT>(w[0], a.x, a.y); q8_unpack<FMT>(w[1], a.z, a.w);
+                        q8_unpack<FMT>(w[2], z.x, z.y); q8_unpack<FMT>(w[3], z.z, z.w);
+                    }
+                    sts128(dst + chunk_at(row, 2 * chunk + (flip ? 1 : 0)), a);
+                    sts128(dst + chunk_at(row, 2 * chunk + (flip ? 0 : 1)), z);
                 }
                 if (there > paged) {                     // the step's tail tiles, over what was just written there
                     const __half* tail = (which ? p.cache.v_tail : p.cache.k_tail) + ((size_t)slot * nkv + u.h) * block * D;
