@@ -19,6 +19,7 @@ namespace kivi {
 namespace {
 
 constexpr int kRows = 128, kKeys = 128, kThreads = 288;
+constexpr float kMasked = -3.0e38f;    // score of a masked key, before its factor: 2^(factor * this) is 0 for every scale
 constexpr float kHeadroomLog = 6.0f;   // log2(kQ8Headroom)
 constexpr int kAtom = 128 * 128;   // bytes of 128 rows of 64 fp16 values, 128-byte swizzled
 
@@ -138,9 +139,10 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
     __shared__ uint64_t full_k, full_v, s_ready, p_ready, pv_done, drained;
     __shared__ uint32_t tmem_slot;
     // Of the two steps in flight, per 16-token tile: the factor of its scores, what the bias of int8 codes adds to them per
-    // sum of q, log2 of V's scale, the first key; per step: first and last key, the largest log2 of V's scale.
+    // sum of q, log2 of V's scale, the first key; per step: first and last key, the largest
+    // log2 of V's scale, whether a scale is NaN.
     __shared__ float meta_f[2][8], meta_bias[2][8], meta_lv[2][8], step_lv[2];
-    __shared__ int meta_key0[2][8], step_key0[2], step_key1[2];
+    __shared__ int meta_key0[2][8], step_key0[2], step_key1[2], step_poisoned[2];
     __shared__ int odd_v;                  // a tail row held an infinity or NaN in V
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int nkv = p.cache.nkv, block = 1 << p.cache.log2b;
@@ -185,8 +187,8 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
     auto mask = [&](float (&s)[32], int key0, int key1) {
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-            if (!sees(key0 + e)) s[e] = -INFINITY;
-            if (!sees(key1 + e)) s[16 + e] = -INFINITY;
+            if (!sees(key0 + e)) s[e] = kMasked;
+            if (!sees(key1 + e)) s[16 + e] = kMasked;
         }
     };
 
@@ -206,7 +208,7 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
         }
         // P = 2^(s f - m) is kept below 2^8 by raising m when a 16-key sum says that it may not be: no pass over S for its
         // maximum. In fp16 it carries V's scale relative to 2^vref, an exponent not below any scale's met so far, and 2^6.
-        float m = kQ8Unset, l = 0.0f, vref = -1000.0f;
+        float m = hi < 0 ? 0.0f : kQ8Unset, l = 0.0f, vref = -1000.0f;   // kQ8Unset: the row has met no key yet
         auto rescale_o = [&](float a) {
 #pragma unroll 1
             for (int c = 0; c < D / 32; ++c) {
@@ -225,6 +227,7 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
             const int key0 = step_key0[b], key1 = step_key1[b];
             const bool masked = __any_sync(0xffffffffu, key1 > hi || (key0 < lo && key1 >= p.sinks));
             const float lv = step_lv[b];
+            const bool poisoned = step_poisoned[b];
             if (lv > vref) {   // uniform; O of the step before is complete, as S of this one is there
                 const float next = floorf(lv) + 1.0f;
                 if (i > 0) rescale_o(fast_exp2(vref - next));
@@ -242,7 +245,8 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
                     for (int half = 0; half < 2; ++half) {
                         const int j = 2 * c + half;
                         const float f = meta_f[b][j], w = meta_lv[b][j] - vref + kHeadroomLog;
-                        const uint64_t ff = pack2(f, f), add = pack2(fmaf(-qsum, meta_bias[b][j], w - m), fmaf(-qsum, meta_bias[b][j], w - m));
+                        const float at = fmaf(-qsum, meta_bias[b][j], w - (m == kQ8Unset ? 0.0f : m));
+                        const uint64_t ff = pack2(f, f), add = pack2(at, at);
                         uint64_t acc = pack2(0.0f, 0.0f);
 #pragma unroll
                         for (int e = 16 * half; e < 16 * half + 16; e += 2) {
@@ -250,10 +254,6 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
                             unpack2(fma2(pack2(s[e], s[e + 1]), ff, add), x, y);
                             x = fast_exp2(x);
                             y = fast_exp2(y);
-                            if (masked) {   // masked keys weigh 0 whatever the scales are
-                                if (s[e] == -INFINITY) x = 0.0f;
-                                if (s[e + 1] == -INFINITY) y = 0.0f;
-                            }
                             acc = add2(acc, pack2(x, y));
                             out[e / 2] = pack_half2(x, y);
                         }
@@ -261,16 +261,31 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
                         unpack2(acc, x, y);
                         sum[half] = (x + y) * fast_exp2(-w);
                     }
+                    if (poisoned && masked) {   // a masked key weighs 0 whatever its page's scales are
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const int j = 2 * c + half;
+                            const float w = meta_lv[b][j] - vref + kHeadroomLog, add = fmaf(-qsum, meta_bias[b][j], w - (m == kQ8Unset ? 0.0f : m));
+                            sum[half] = 0.0f;
+#pragma unroll
+                            for (int e = 16 * half; e < 16 * half + 16; e += 2) {
+                                const float x = s[e] == kMasked ? 0.0f : fast_exp2(fmaf(s[e], meta_f[b][j], add));
+                                const float y = s[e + 1] == kMasked ? 0.0f : fast_exp2(fmaf(s[e + 1], meta_f[b][j], add));
+                                if (x != 0.0f || y != 0.0f) sum[half] += (x + y) * fast_exp2(-w);   // not 0 * NaN
+                                out[e / 2] = pack_half2(x, y);
+                            }
+                        }
+                    }
                 };
                 weigh();
-                if (__any_sync(0xffffffffu, !(sum[0] + sum[1] <= 256.0f))) {
+                if (__any_sync(0xffffffffu, !(sum[0] + sum[1] <= 256.0f) || m == kQ8Unset)) {
                     // the first keys of a row, or scores far above all before them
                     float x = -INFINITY, y = -INFINITY;
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         const float fx = meta_f[b][2 * c], fy = meta_f[b][2 * c + 1];
-                        if (!(masked && s[e] == -INFINITY)) x = fmaxf(x, fmaf(s[e], fx, -qsum * meta_bias[b][2 * c]));
-                        if (!(masked && s[16 + e] == -INFINITY)) y = fmaxf(y, fmaf(s[16 + e], fy, -qsum * meta_bias[b][2 * c + 1]));
+                        if (s[e] != kMasked) x = fmaxf(x, fmaf(s[e], fx, -qsum * meta_bias[b][2 * c]));
+                        if (s[16 + e] != kMasked) y = fmaxf(y, fmaf(s[16 + e], fy, -qsum * meta_bias[b][2 * c + 1]));
                     }
                     // whole numbers: the factor is a power of two, and what is there already is not rounded again
                     const float mn = fmaxf(m, ceilf(fmaxf(x, y))), a = fast_exp2(m - mn);
@@ -358,12 +373,12 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
             const int first = 8 * i, b = i & 1, tile = tile_of(first + (lane & 7));
             const uint32_t start = ((uint32_t)id * nkv + u.h) * (uint32_t)(block >> 4) + (uint32_t)(tile & sub_mask);   // in tiles
             const int paged = min(8, max(0, v.tiles - first)), there = min(8, u.items - first);   // tiles of pages; of any kind
-            float f = 0.0f, bias = 0.0f, lv = -1000.0f;
+            float f = 1.0f, bias = 0.0f, lv = -1000.0f;
             int key0 = 0x3fffffff;                       // a tile that is not there: no row sees that far
             if (c < paged) {
                 const float2 sc = p.cache.scales[(size_t)id * nkv + u.h];
-                f = sc.x * p.scale_log2;
                 // a zero scale's codes are zeros too: any other does; NaN stays
+                f = (sc.x == 0.0f ? 1.0f : sc.x) * p.scale_log2;
                 lv = sc.y == 0.0f ? -1000.0f : log2f(sc.y);
                 key0 = tile * 16;
                 if (FMT == KIVI_Q8_INT8) { bias = 128.0f * f; f *= 16777216.0f; }
@@ -398,7 +413,8 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
                         meta_f[b][c] = f; meta_bias[b][c] = bias; meta_key0[b][c] = key0;
                         meta_lv[b][c] = lv == -1000.0f ? fmaxf(lv_top, -100.0f) : lv;
                     }
-                    if (c == 0) { step_lv[b] = fmaxf(lv_top, -100.0f); step_key0[b] = k0; step_key1[b] = k1; }
+                    const bool nan = __any_sync(0xffffffffu, c < 8 && !(f + lv == f + lv));
+                    if (c == 0) { step_poisoned[b] = nan; step_lv[b] = fmaxf(lv_top, -100.0f); step_key0[b] = k0; step_key1[b] = k1; }
                 }
                 // the two halves of a row's threads store in opposite order, so that eight threads meet eight bank groups
                 const bool flip = chunk & 4;
