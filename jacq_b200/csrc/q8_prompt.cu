@@ -1,24 +1,25 @@
 // Attention over the 8-bit block-scaled cache for many query rows: prompts and long runs of tokens, on tcgen05.
 //
 // Same mathematics as the kernel for few rows: codes are exact in fp16, K's page scale multiplies the scores, V's goes
-// into the probabilities. A unit is 128 query rows (token-major, the query heads of one kv head inside) of one sequence
-// and kv head; keys come 128 at a time, as eight 16-token tiles of whatever pages are seen:
+// into the probabilities. A unit is 256 query rows (128 at D = 256; token-major, the query heads of one kv head inside)
+// of one sequence and kv head, as two tiles of 128; keys come 128 at a time, as eight 16-token tiles of whatever pages
+// are seen. Per tile of rows:
 //
 //   S[128 x 128] = Q Kc^T     operands in shared memory, accumulator in tensor memory
 //   P = 2^(S f - m) vs'       four warps, a thread per row: no shuffles; P goes back to tensor memory, over S
 //   O[128 x D]  += P Vc       P from tensor memory, Vc from shared memory with the channels as its leading dimension
 //
-// Work is split by warps: 0 .. 3 softmax and epilogue, 4 .. 7 load codes and write them as fp16 into the swizzled tiles,
-// one thread of warp 8 issues the products. At 128 rows a byte of codes is worth 256 flops, so the tensor pipe (4 * 128 *
-// 128 * D flops a step) and the exponentials (128 * 128, 16 a cycle) bound it, not HBM. Two CTAs share a multiprocessor
-// (96 KB of shared memory and 256 columns of tensor memory each at D = 128): one's products run under the other's
-// exponentials. Every wait is bounded: a CTA whose wait gave up counts itself, waits for its products and leaves.
+// Work is split by warps: 0 .. 3 and 4 .. 7 softmax and epilogue of the two tiles, 8 .. 11 load codes and write them as
+// fp16 into the swizzled tiles (once for both), one thread of warp 12 issues the products. At 256 rows a byte of codes is
+// worth 512 flops, so the tensor pipe (2 * 4 * 128 * 128 * D flops a step) and the exponentials (2 * 128 * 128, 16 a
+// cycle) bound it, not HBM; one tile's products run under the other's exponentials. Every wait is bounded: a CTA whose
+// wait gave up counts itself, waits for its products and leaves.
 #include "q8_common.cuh"
 
 namespace kivi {
 namespace {
 
-constexpr int kRows = 128, kKeys = 128, kThreads = 288;
+constexpr int kRows = 128, kKeys = 128, kThreads = 416;
 constexpr float kMasked = -3.0e38f;    // score of a masked key, before its factor: 2^(factor * this) is 0 for every scale
 constexpr float kHeadroomLog = 6.0f;   // log2(kQ8Headroom)
 constexpr int kAtom = 128 * 128;   // bytes of 128 rows of 64 fp16 values, 128-byte swizzled
@@ -58,31 +59,6 @@ __device__ __forceinline__ void product_ts(uint32_t d, uint32_t a, uint64_t b, u
                  "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
                  ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(add) : "memory");
 }
-__device__ __forceinline__ void load32(uint32_t at, float (&v)[32]) {   // 32 columns of the thread's row; whole warps
-    uint32_t r[32];
-    __syncwarp();
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(at) : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-}
-__device__ __forceinline__ void store32(uint32_t at, const float (&v)[32]) {
-    __syncwarp();
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};"
-        ::"f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]),
-          "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]),
-          "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]),
-          "f"(v[31]), "r"(at) : "memory");
-}
 __device__ __forceinline__ void store16(uint32_t at, const uint32_t (&v)[16]) {
     __syncwarp();
     asm volatile(
@@ -98,6 +74,25 @@ __device__ __forceinline__ void load16(uint32_t at, uint32_t (&r)[16]) {
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(at) : "memory");
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// 32 columns of the thread's row, in two halves: the registers are the caller's after await32 alone, which names them.
+__device__ __forceinline__ void request32(uint32_t at, uint32_t (&r)[32]) {
+    __syncwarp();
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at) : "memory");
+}
+__device__ __forceinline__ void await32(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
+                   "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
+                   "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
 }
 // two fp32 values in one instruction
 __device__ __forceinline__ uint64_t pack2(float x, float y) {
@@ -126,78 +121,85 @@ __device__ __forceinline__ uint32_t chunk_at(int row, int j) {
 }
 __device__ __forceinline__ bool odd_half(uint32_t w) { return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u; }
 
+// Tiles of 128 rows per unit and stages of K and V: what shared memory (227 KB) and tensor memory (512 columns) hold.
 template <int D>
-constexpr int tmem_columns() { return D == 256 ? 512 : 256; }
+constexpr int tiles_of() { return D == 256 ? 1 : 2; }
 template <int D>
-constexpr int smem_bytes() { return 3 * kRows * D * 2 + 1024; }
+constexpr int stages_of() { return D == 256 ? 1 : 2; }
+template <int D>
+constexpr int smem_bytes() { return (tiles_of<D>() + 2 * stages_of<D>()) * kRows * D * 2 + 1024; }
 
 template <int D, int FMT>
-__global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(const Q8AttnParams p) {
+__global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnParams p) {
     constexpr int CPR = D / 16;            // 16-byte chunks of a row of codes
     constexpr int TILE = kRows * D * 2;    // bytes of an fp16 operand tile
+    constexpr int TILES = tiles_of<D>(), STAGES = stages_of<D>();
     extern __shared__ unsigned char raw[];
-    __shared__ uint64_t full_k, full_v, s_ready, p_ready, pv_done, drained;
+    __shared__ uint64_t full_k[2], full_v[2], free_k[2], free_v[2], s_ready[2], p_ready[2], pv_done[2], drained;
     __shared__ uint32_t tmem_slot;
-    // Of the two steps in flight, per 16-token tile: the factor of its scores, what the bias of int8 codes adds to them per
-    // sum of q, log2 of V's scale, the first key; per step: first and last key, the largest
-    // log2 of V's scale, whether a scale is NaN.
-    __shared__ float meta_f[2][8], meta_bias[2][8], meta_lv[2][8], step_lv[2];
-    __shared__ int meta_key0[2][8], step_key0[2], step_key1[2], step_poisoned[2];
-    __shared__ int odd_v;                  // a tail row held an infinity or NaN in V
+    // Of the steps in flight, per 16-token tile: the factor of its scores, what the bias of int8 codes adds to them per sum
+    // of q, log2 of V's scale, the first key; per step: first and last key, the largest log2 of V's scale.
+    // Four of them: K of step i is written when the products with K of step i - 2 are done, while the softmax may
+    // still be at step i - 2; it is not at step i - 4, whose probabilities those products' order has waited for.
+    __shared__ float meta_f[4][8], meta_bias[4][8], meta_lv[4][8], step_lv[4];
+    __shared__ int meta_key0[4][8], step_key0[4], step_key1[4];
+    __shared__ int odd_v, odd_page;        // a tail row held an infinity or NaN in V; a page's scale is NaN
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int nkv = p.cache.nkv, block = 1 << p.cache.log2b;
     // the last rows first: without a window they have the most keys
     const int at_block = blockIdx.x % p.row_blocks;
-    const Unit u = make_unit(p, blockIdx.x - at_block + (p.row_blocks - 1 - at_block), kRows);
-    if (u.rb * kRows >= u.rows) return;
+    const Unit u = make_unit(p, blockIdx.x - at_block + (p.row_blocks - 1 - at_block), TILES * kRows);
+    const int row_base = u.rb * TILES * kRows;
+    if (row_base >= u.rows) return;
     const View& v = u.v;
     const int steps = (u.items + 7) >> 3;
-    const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u, q_tile = smem, k_tile = smem + TILE, v_tile = smem + 2 * TILE;
+    const int tiles = row_base + kRows < u.rows ? TILES : 1;       // tiles with rows in them
+    const uint32_t smem = (smem_u32(raw) + 1023u) & ~1023u, k_tile = smem + TILES * TILE, v_tile = k_tile + STAGES * TILE;
 
     if (tid == 0) {
-        mbar_init(&full_k, 128); mbar_init(&full_v, 128); mbar_init(&p_ready, 128);
-        mbar_init(&s_ready, 1); mbar_init(&pv_done, 1); mbar_init(&drained, 1);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            mbar_init(&full_k[k], 128); mbar_init(&full_v[k], 128); mbar_init(&p_ready[k], 128);
+            mbar_init(&free_k[k], 1); mbar_init(&free_v[k], 1); mbar_init(&s_ready[k], 1); mbar_init(&pv_done[k], 1);
+        }
+        mbar_init(&drained, 1);
         fence_barrier_init();
-        odd_v = 0;
+        odd_v = odd_page = 0;
     }
-    if (warp == 8) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
-                     ::"r"(smem_u32(&tmem_slot)), "n"(tmem_columns<D>()) : "memory");
+    if (warp == 12) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_slot)), "n"(512) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    for (int e = tid; e < kRows * (D / 8); e += kThreads) {   // query rows
-        const int row = e / (D / 8), j = e % (D / 8), r = u.rb * kRows + row;
+    for (int e = tid; e < tiles * kRows * (D / 8); e += kThreads) {   // query rows
+        const int row = e / (D / 8), j = e % (D / 8), r = row_base + row;
         uint4 x = make_uint4(0u, 0u, 0u, 0u);
         if (r < u.rows)
             x = *reinterpret_cast<const uint4*>(p.q + (long long)(u.row0 + r / p.qpk) * p.q_stride + (size_t)(u.h * p.qpk + r % p.qpk) * D + 8 * j);
-        sts128(q_tile + chunk_at(row, j), x);
+        sts128(smem + (row >> 7) * TILE + chunk_at(row & 127, j), x);
     }
     fence_proxy_async();
     fence_before();
     __syncthreads();
     fence_after();
-    const uint32_t tmem_s = *reinterpret_cast<volatile uint32_t*>(&tmem_slot), tmem_o = tmem_s + kKeys;
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(&tmem_slot);
+    auto tmem_s = [&](int t) { return tmem + t * kKeys; };
+    auto tmem_o = [&](int t) { return tmem + TILES * kKeys + t * D; };
     bool failed = false;
 
     // row of a softmax thread
-    const int r = u.rb * kRows + (tid & 127);
+    const int t_mine = warp >> 2 & 1, r = row_base + t_mine * kRows + (tid & 127);
     const int hi = r < u.rows ? u.len - u.n + r / p.qpk : -1;
     const int lo = p.window == 0x7fffffff ? 0 : hi - p.window + 1;
     auto sees = [&](int key) { return key <= hi && (key >= lo || key < p.sinks); };
-    auto mask = [&](float (&s)[32], int key0, int key1) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            if (!sees(key0 + e)) s[e] = kMasked;
-            if (!sees(key1 + e)) s[16 + e] = kMasked;
-        }
-    };
 
-    if (warp < 4) {
-        const uint32_t mine = (uint32_t)(warp * 32) << 16;   // this warp's lanes of tensor memory
+    if (warp < 8) {
+        if (t_mine < tiles) {
+        const uint32_t mine = (uint32_t)((warp & 3) * 32) << 16;   // this warp's lanes of tensor memory
+        const uint32_t s_at = tmem_s(t_mine) + mine, o_at = tmem_o(t_mine) + mine;
         float qsum = 0.0f;
         if (FMT == KIVI_Q8_INT8) {
             for (int j = 0; j < D / 8; ++j) {
-                const uint4 x = lds128(q_tile + chunk_at(tid, j));
+                const uint4 x = lds128(smem + t_mine * TILE + chunk_at(tid & 127, j));
                 const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
@@ -206,52 +208,55 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
                 }
             }
         }
-        // P = 2^(s f - m) is kept below 2^8 by raising m when a 16-key sum says that it may not be: no pass over S for its
-        // maximum. In fp16 it carries V's scale relative to 2^vref, an exponent not below any scale's met so far, and 2^6.
-        float m = hi < 0 ? 0.0f : kQ8Unset, l = 0.0f, vref = -1000.0f;   // kQ8Unset: the row has met no key yet
+        // P = 2^(s f - m) is kept below 2^8 by raising m when a sum says that it may not be: no pass over S for its maximum.
+        // In fp16 it carries V's scale relative to 2^vref, an exponent not below any scale's met so far, and 2^6.
+        // kQ8Unset: the row has met no key yet.
+        float m = hi < 0 ? 0.0f : kQ8Unset, l = 0.0f, vref = -1000.0f;
         auto rescale_o = [&](float a) {
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) {
-                float o[32];
-                load32(tmem_o + mine + 32 * c, o);
+            for (int c = 0; c < D; c += 16) {
+                uint32_t o[16];
+                load16(o_at + c, o);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] *= a;
-                store32(tmem_o + mine + 32 * c, o);
+                for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * a);
+                store16(o_at + c, o);
             }
         };
 #pragma unroll 1
         for (int i = 0; i < steps; ++i) {
-            const int b = i & 1;
-            if (!wait_bar(&s_ready, b)) { failed = true; break; }
+            const int b = i & 3;
+            if (!wait_bar(&s_ready[t_mine], i & 1)) { failed = true; break; }
             fence_after();
             const int key0 = step_key0[b], key1 = step_key1[b];
             const bool masked = __any_sync(0xffffffffu, key1 > hi || (key0 < lo && key1 >= p.sinks));
             const float lv = step_lv[b];
-            const bool poisoned = step_poisoned[b];
-            if (lv > vref) {   // uniform; O of the step before is complete, as S of this one is there
+            if (__builtin_expect(lv > vref, 0)) {   // uniform; O of the step before is complete, as S of this one is there
                 const float next = floorf(lv) + 1.0f;
                 if (i > 0) rescale_o(fast_exp2(vref - next));
                 vref = next;
             }
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-                float s[32];
-                load32(tmem_s + mine + 32 * c, s);
-                if (masked) mask(s, meta_key0[b][2 * c], meta_key0[b][2 * c + 1]);
+            // 32 keys: scores to probabilities. What is rare is kept out of the way: this code is run over and over beside
+            // two other roles' and its length counted more than its instructions.
+            auto chunk = [&](uint32_t (&s)[32], int c) {
+                if (__builtin_expect(masked, 0)) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) if (!sees(meta_key0[b][2 * c + (e >> 4)] + (e & 15))) s[e] = __float_as_uint(kMasked);
+                }
                 uint32_t out[16];
-                float sum[2];
-                auto weigh = [&]() {
+                float sum;
+                while (true) {
+                    sum = 0.0f;
+                    const float base = vref - kHeadroomLog + (m == kQ8Unset ? 0.0f : m);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const int j = 2 * c + half;
-                        const float f = meta_f[b][j], w = meta_lv[b][j] - vref + kHeadroomLog;
-                        const float at = fmaf(-qsum, meta_bias[b][j], w - (m == kQ8Unset ? 0.0f : m));
-                        const uint64_t ff = pack2(f, f), add = pack2(at, at);
+                        const float lw = meta_lv[b][2 * c + half], add = fmaf(-qsum, meta_bias[b][2 * c + half], lw - base);
+                        const float f = meta_f[b][2 * c + half];
+                        const uint64_t ff = pack2(f, f), aa = pack2(add, add);
                         uint64_t acc = pack2(0.0f, 0.0f);
 #pragma unroll
                         for (int e = 16 * half; e < 16 * half + 16; e += 2) {
                             float x, y;
-                            unpack2(fma2(pack2(s[e], s[e + 1]), ff, add), x, y);
+                            unpack2(fma2(pack2(__uint_as_float(s[e]), __uint_as_float(s[e + 1])), ff, aa), x, y);
                             x = fast_exp2(x);
                             y = fast_exp2(y);
                             acc = add2(acc, pack2(x, y));
@@ -259,89 +264,80 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
                         }
                         float x, y;
                         unpack2(acc, x, y);
-                        sum[half] = (x + y) * fast_exp2(-w);
+                        sum = fmaf(x + y, fast_exp2(vref - kHeadroomLog - lw), sum);
                     }
-                    if (poisoned && masked) {   // a masked key weighs 0 whatever its page's scales are
-#pragma unroll
-                        for (int half = 0; half < 2; ++half) {
-                            const int j = 2 * c + half;
-                            const float w = meta_lv[b][j] - vref + kHeadroomLog, add = fmaf(-qsum, meta_bias[b][j], w - (m == kQ8Unset ? 0.0f : m));
-                            sum[half] = 0.0f;
-#pragma unroll
-                            for (int e = 16 * half; e < 16 * half + 16; e += 2) {
-                                const float x = s[e] == kMasked ? 0.0f : fast_exp2(fmaf(s[e], meta_f[b][j], add));
-                                const float y = s[e + 1] == kMasked ? 0.0f : fast_exp2(fmaf(s[e + 1], meta_f[b][j], add));
-                                if (x != 0.0f || y != 0.0f) sum[half] += (x + y) * fast_exp2(-w);   // not 0 * NaN
-                                out[e / 2] = pack_half2(x, y);
-                            }
-                        }
-                    }
-                };
-                weigh();
-                if (__any_sync(0xffffffffu, !(sum[0] + sum[1] <= 256.0f) || m == kQ8Unset)) {
+                    if (__builtin_expect(!__any_sync(0xffffffffu, !(sum <= 256.0f) || m == kQ8Unset), 1)) break;
                     // the first keys of a row, or scores far above all before them
-                    float x = -INFINITY, y = -INFINITY;
+                    float top = -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        const float fx = meta_f[b][2 * c], fy = meta_f[b][2 * c + 1];
-                        if (s[e] != kMasked) x = fmaxf(x, fmaf(s[e], fx, -qsum * meta_bias[b][2 * c]));
-                        if (s[16 + e] != kMasked) y = fmaxf(y, fmaf(s[16 + e], fy, -qsum * meta_bias[b][2 * c + 1]));
-                    }
+                    for (int e = 0; e < 32; ++e)
+                        if (__uint_as_float(s[e]) != kMasked)
+                            top = fmaxf(top, fmaf(__uint_as_float(s[e]), meta_f[b][2 * c + (e >> 4)], -qsum * meta_bias[b][2 * c + (e >> 4)]));
                     // whole numbers: the factor is a power of two, and what is there already is not rounded again
-                    const float mn = fmaxf(m, ceilf(fmaxf(x, y))), a = fast_exp2(m - mn);
+                    const bool none = !__any_sync(0xffffffffu, top > m);
+                    const float mn = fmaxf(m, ceilf(top)), a = fast_exp2(m - mn);
+                    if (none) break;                    // nothing new to go by: NaN, or keys that nobody sees
                     m = mn;
                     l *= a;
                     if (i > 0) rescale_o(a);
 #pragma unroll 1
-                    for (int k = 0; k < c; ++k) {   // the chunks of P that are there already
+                    for (int k = 0; k < c; ++k) {       // the chunks of P that are there already
                         uint32_t w[16];
-                        load16(tmem_s + mine + 16 * k, w);
+                        load16(s_at + 16 * k, w);
                         const __half2 aa = __float2half2_rn(a);
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
                             const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&w[e]), aa);
                             w[e] = *reinterpret_cast<const uint32_t*>(&h);
                         }
-                        store16(tmem_s + mine + 16 * k, w);
+                        store16(s_at + 16 * k, w);
                     }
-                    weigh();
                 }
-                l += sum[0] + sum[1];
-                store16(tmem_s + mine + 16 * c, out);   // over columns of S that have been read
+                l += sum;
+                store16(s_at + 16 * c, out);            // P over columns of S that have been read
+            };
+            uint32_t s0[32], s1[32];
+            request32(s_at, s0);
+#pragma unroll 1
+            for (int c = 0; c < 4; c += 2) {
+                await32(s0);
+                request32(s_at + 32 * (c + 1), s1);
+                chunk(s0, c);
+                await32(s1);
+                if (c == 0) request32(s_at + 64, s0);
+                chunk(s1, c + 1);
             }
             store_wait();
             fence_before();
-            arrive(&p_ready);
+            arrive(&p_ready[t_mine]);
         }
-        if (!failed && steps > 0 && !wait_bar(&pv_done, (steps - 1) & 1)) failed = true;
+        if (!failed && steps > 0 && !wait_bar(&pv_done[t_mine], (steps - 1) & 1)) failed = true;
         fence_after();
         const float scale = l != 0.0f ? fast_exp2(vref - kHeadroomLog) / l : 0.0f;
         const size_t at = r < u.rows ? out_at(p, u, r, D) : 0;
-        for (int c = 0; c < D / 32; ++c) {
-            float o[32];
-            if (steps > 0) {
-                load32(tmem_o + mine + 32 * c, o);
-            } else {
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+            uint32_t w[16];
+            float o[16];
+            if (steps > 0) load16(o_at + c, w);
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = 0.0f;
-            }
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = l != 0.0f ? o[e] * scale : 0.0f;
+            for (int e = 0; e < 16; ++e) o[e] = steps > 0 && l != 0.0f ? __uint_as_float(w[e]) * scale : 0.0f;
             if (r >= u.rows) {
                 // a row behind the last: nothing to store
             } else if (p.out_h) {
 #pragma unroll
-                for (int e = 0; e < 32; e += 8)
-                    *reinterpret_cast<uint4*>(p.out_h + at + 32 * c + e) = make_uint4(
+                for (int e = 0; e < 16; e += 8)
+                    *reinterpret_cast<uint4*>(p.out_h + at + c + e) = make_uint4(
                         pack_half2(o[e], o[e + 1]), pack_half2(o[e + 2], o[e + 3]), pack_half2(o[e + 4], o[e + 5]), pack_half2(o[e + 6], o[e + 7]));
             } else {
 #pragma unroll
-                for (int e = 0; e < 32; e += 4)
-                    *reinterpret_cast<float4*>(p.out + at + 32 * c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                for (int e = 0; e < 16; e += 4)
+                    *reinterpret_cast<float4*>(p.out + at + c + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
             }
         }
-    } else if (warp < 8) {
-        const int c = tid - 128;
+        }
+    } else if (warp < 12) {
+        const int c = tid - 256;
         const int sub_mask = (block >> 4) - 1, sub_log = p.cache.log2b - 4;
         const int* table = p.seq.tables + (size_t)u.seq * p.seq.width;
         int slot = q8_slot(p.seq, u.seq);
@@ -363,43 +359,55 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
             const int page = tile_of(item) >> sub_log;
             return page < p.seq.width ? table[page] : -1;
         };
-        int id = load_id(0);
-#pragma unroll 1
-        for (int i = 0; i < steps && !failed; ++i) {
+        // Codes travel ahead: a thread asks for its chunks of step i + 1 as soon as those of step i are stored.
+        uint4 x[2][CPR];
+        auto fetch = [&](int which, int step, uint32_t start) {
+            const uint8_t* codes = (which ? p.cache.v : p.cache.k) + chunk * 16;
+            const int paged = v.tiles - 8 * step;
+#pragma unroll
+            for (int k = 0; k < CPR; ++k) {
+                const uint32_t at = __shfl_sync(0xffffffffu, start, sub_of(k));
+                x[which][k] = make_uint4(0u, 0u, 0u, 0u);
+                if (sub_of(k) < paged) x[which][k] = __ldg(reinterpret_cast<const uint4*>(codes + (size_t)at * (16 * D) + row_of(k) * D));
+            }
+        };
+        // id: of the step to come; where its tiles start, counted in tiles
+        auto start_of = [&](int& id, int step) {
             if (!index_in_pool(id, p.cache.num_blocks)) {
                 if (c < 8) atomicAdd(&g_q8_prompt_rejected, 1u);
                 id = 0;
             }
-            const int first = 8 * i, b = i & 1, tile = tile_of(first + (lane & 7));
-            const uint32_t start = ((uint32_t)id * nkv + u.h) * (uint32_t)(block >> 4) + (uint32_t)(tile & sub_mask);   // in tiles
+            return ((uint32_t)id * nkv + u.h) * (uint32_t)(block >> 4) + (uint32_t)(tile_of(8 * step + (lane & 7)) & sub_mask);
+        };
+        int id = load_id(0), id_next = load_id(1);
+        uint32_t start = start_of(id, 0);
+        fetch(0, 0, start);
+        fetch(1, 0, start);
+#pragma unroll 1
+        for (int i = 0; i < steps && !failed; ++i) {
+            const int first = 8 * i, b = i & 3, stage = i % STAGES;
             const int paged = min(8, max(0, v.tiles - first)), there = min(8, u.items - first);   // tiles of pages; of any kind
             float f = 1.0f, bias = 0.0f, lv = -1000.0f;
             int key0 = 0x3fffffff;                       // a tile that is not there: no row sees that far
             if (c < paged) {
-                const float2 sc = p.cache.scales[(size_t)id * nkv + u.h];
-                // a zero scale's codes are zeros too: any other does; NaN stays
+                float2 sc = p.cache.scales[(size_t)id * nkv + u.h];
+                if (!(sc.x + sc.y == sc.x + sc.y)) { odd_page = 1; sc = make_float2(1.0f, 1.0f); }   // seen to at the end
+                // a zero scale's codes are zeros too: any other does
                 f = (sc.x == 0.0f ? 1.0f : sc.x) * p.scale_log2;
                 lv = sc.y == 0.0f ? -1000.0f : log2f(sc.y);
-                key0 = tile * 16;
+                key0 = tile_of(first + lane) * 16;
                 if (FMT == KIVI_Q8_INT8) { bias = 128.0f * f; f *= 16777216.0f; }
             } else if (c < there) {
                 f = p.scale_log2; lv = 0.0f;
                 key0 = v.paged + (first + c - v.tiles) * 16;
             }
-            id = i + 1 < steps ? load_id(i + 1) : 0;
+            id = id_next;
+            id_next = load_id(i + 2);
+            start = start_of(id, i + 1);
 #pragma unroll
             for (int which = 0; which < 2; ++which) {
-                const uint8_t* codes = (which ? p.cache.v : p.cache.k) + chunk * 16;
-                const uint32_t dst = which ? v_tile : k_tile;
-                // codes of this thread's chunks are on their way while the tile is still in use
-                uint4 x[CPR];
-#pragma unroll
-                for (int k = 0; k < CPR; ++k) {
-                    const uint32_t at = __shfl_sync(0xffffffffu, start, sub_of(k));
-                    x[k] = make_uint4(0u, 0u, 0u, 0u);
-                    if (sub_of(k) < paged) x[k] = __ldg(reinterpret_cast<const uint4*>(codes + (size_t)at * (16 * D) + row_of(k) * D));
-                }
-                if (i > 0 && !wait_bar(which ? &pv_done : &s_ready, (i - 1) & 1)) { failed = true; break; }
+                const uint32_t dst = (which ? v_tile : k_tile) + stage * TILE;
+                if (i >= STAGES && !wait_bar(which ? &free_v[stage] : &free_k[stage], (i / STAGES - 1) & 1)) { failed = true; break; }
                 if (which == 0 && c < 32) {              // one warp: what the softmax has to know of the step
                     float lv_top = lv;
                     int k0 = key0, k1 = key0 + 15;
@@ -413,15 +421,15 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
                         meta_f[b][c] = f; meta_bias[b][c] = bias; meta_key0[b][c] = key0;
                         meta_lv[b][c] = lv == -1000.0f ? fmaxf(lv_top, -100.0f) : lv;
                     }
-                    const bool nan = __any_sync(0xffffffffu, c < 8 && !(f + lv == f + lv));
-                    if (c == 0) { step_poisoned[b] = nan; step_lv[b] = fmaxf(lv_top, -100.0f); step_key0[b] = k0; step_key1[b] = k1; }
+                    if (c == 0) { step_lv[b] = fmaxf(lv_top, -100.0f); step_key0[b] = k0; step_key1[b] = k1; }
                 }
                 // the two halves of a row's threads store in opposite order, so that eight threads meet eight bank groups
                 const bool flip = chunk & 4;
 #pragma unroll
                 for (int k = 0; k < CPR; ++k) {
                     const int row = sub_of(k) * 16 + row_of(k);
-                    const uint32_t w[4] = {flip ? x[k].z : x[k].x, flip ? x[k].w : x[k].y, flip ? x[k].x : x[k].z, flip ? x[k].y : x[k].w};
+                    const uint4 y = x[which][k];
+                    const uint32_t w[4] = {flip ? y.z : y.x, flip ? y.w : y.y, flip ? y.x : y.z, flip ? y.y : y.w};
                     uint4 a, z;
                     if (FMT == KIVI_Q8_INT8 && which == 0) {
                         // K: a byte alone is a subnormal, (code + 128) 2^-24 exactly; the softmax takes the bias off the score
@@ -462,29 +470,47 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
                     }
                 }
                 fence_proxy_async();
-                arrive(which ? &full_v : &full_k);
+                arrive(which ? &full_v[stage] : &full_k[stage]);
+                fetch(which, i + 1, start);
             }
         }
     } else if (lane == 0) {
         constexpr uint32_t qk = shape(kKeys, false), pv = shape(D, true);
-        for (int i = 0; i < steps; ++i) {
-            const uint32_t parity = i & 1;
-            // S gives way to P and P to the next S: the products that read P are done first
-            if (!wait_bar(&full_k, parity) || (i > 0 && !wait_bar(&pv_done, parity ^ 1u))) { failed = true; break; }
-            __threadfence_block();   // what the loading warps left beside the tile goes on to those that wait for s_ready
-            fence_after();
+        auto scores = [&](int t, int i) {
+            const uint32_t q_at = smem + t * TILE, k_at = k_tile + (i % STAGES) * TILE;
 #pragma unroll
             for (int k = 0; k < D / 16; ++k) {   // 16 channels: 32 bytes on in the swizzled row, the next 64 in the next atom
                 const uint32_t at = (k >> 2) * kAtom + (k & 3) * 32;
-                product_ss(tmem_s, operand(q_tile + at, 16), operand(k_tile + at, 16), qk, k > 0);
+                product_ss(tmem_s(t), operand(q_at + at, 16), operand(k_at + at, 16), qk, k > 0);
             }
-            commit(&s_ready);
-            if (!wait_bar(&full_v, parity) || !wait_bar(&p_ready, parity)) { failed = true; break; }
+            commit(&s_ready[t]);
+            if (t == tiles - 1) commit(&free_k[i % STAGES]);
+        };
+        auto keys_there = [&](int i) {
+            const bool ok = wait_bar(&full_k[i % STAGES], (i / STAGES) & 1);
+            __threadfence_block();   // what the loading warps left beside the tile goes on to those that wait for s_ready
             fence_after();
+            return ok;
+        };
+        failed = steps > 0 && !keys_there(0);
+        for (int t = 0; t < tiles && steps > 0 && !failed; ++t) scores(t, 0);
+        for (int i = 0; i < steps && !failed; ++i) {
+            if (!wait_bar(&full_v[i % STAGES], (i / STAGES) & 1)) { failed = true; break; }
+            for (int t = 0; t < tiles; ++t) {
+                if (!wait_bar(&p_ready[t], i & 1)) { failed = true; break; }
+                fence_after();
+                const uint32_t v_at = v_tile + (i % STAGES) * TILE;
 #pragma unroll
-            for (int k = 0; k < kKeys / 16; ++k)   // 16 keys: 8 columns of P, 16 rows of V
-                product_ts(tmem_o, tmem_s + 8 * k, operand(v_tile + 2048 * k, kAtom), pv, i > 0 || k > 0);
-            commit(&pv_done);
+                for (int k = 0; k < kKeys / 16; ++k)   // 16 keys: 8 columns of P, 16 rows of V
+                    product_ts(tmem_o(t), tmem_s(t) + 8 * k, operand(v_at + 2048 * k, kAtom), pv, i > 0 || k > 0);
+                commit(&pv_done[t]);
+                if (t == tiles - 1) commit(&free_v[i % STAGES]);
+                if (i + 1 == steps) continue;
+                // P gives way to the next S: the products that read it are done first
+                if ((t == 0 && !keys_there(i + 1)) || !wait_bar(&pv_done[t], i & 1)) { failed = true; break; }
+                fence_after();
+                scores(t, i + 1);
+            }
         }
         commit(&drained);
         if (!wait_bar(&drained, 0)) failed = true;
@@ -492,10 +518,27 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 1 : 2) q8_prompt_kernel(c
     __syncwarp();
     fence_before();
     const bool cta_failed = __syncthreads_or(failed);
-    if (warp == 8)
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_s), "n"(tmem_columns<D>()) : "memory");
+    if (warp == 12)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
     if (cta_failed && tid == 0) atomicAdd(&g_q8_prompt_failures, 1u);
-    if (odd_v && warp < 4 && r < u.rows) {
+    if (odd_page && warp < 8 && t_mine < tiles && r < u.rows) {
+        // rare: a row that sees a token of a page with a NaN scale yields NaN throughout
+        const int* table = p.seq.tables + (size_t)u.seq * p.seq.width;
+        const size_t at = out_at(p, u, r, D);
+        for (int item = 0; item < v.tiles; ++item) {
+            const int tile = item < v.ns ? item : item - v.ns + v.w0, page = tile >> (p.cache.log2b - 4);
+            const int id = page < p.seq.width ? table[page] : 0;
+            const float2 sc = p.cache.scales[(size_t)(index_in_pool(id, p.cache.num_blocks) ? id : 0) * nkv + u.h];
+            if (sc.x + sc.y == sc.x + sc.y) continue;
+            bool seen = false;
+            for (int e = 0; e < 16; ++e) seen |= sees(tile * 16 + e);
+            for (int ch = 0; seen && ch < D; ++ch) {
+                if (p.out_h) p.out_h[at + ch] = __ushort_as_half((unsigned short)0x7fff);
+                else p.out[at + ch] = __int_as_float(0x7fc00000);
+            }
+        }
+    }
+    if (odd_v && warp < 8 && t_mine < tiles && r < u.rows) {   // (one of a row's two threads)
         // rare: rows that see a tail token whose V holds an infinity or NaN yield NaN in that channel
         int slot = q8_slot(p.seq, u.seq);
         if (!index_in_pool(slot, p.cache.num_slots)) slot = 0;
@@ -525,7 +568,8 @@ cudaError_t launch(const Q8AttnParams& p, cudaStream_t stream) {
 
 cudaError_t launch_q8_prompt(const Q8AttnParams& args, int d, int fmt, cudaStream_t stream) {
     Q8AttnParams p = args;
-    p.row_blocks = (p.max_q * p.qpk + kRows - 1) / kRows;
+    const int rows = kRows * (d == 256 ? 1 : 2);
+    p.row_blocks = (p.max_q * p.qpk + rows - 1) / rows;
     p.row_block0 = 0;
     const bool i8 = fmt == KIVI_Q8_INT8;
     switch (d) {
