@@ -359,7 +359,9 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
             const int page = tile_of(item) >> sub_log;
             return page < p.seq.width ? table[page] : -1;
         };
-        // Codes travel ahead: a thread asks for its chunks of step i + 1 as soon as those of step i are stored.
+        // Codes travel ahead: a thread asks for its chunks of step i + 1 as soon as those of step i are stored (at D = 256,
+        // where K's and V's together would not fit its registers, just before it waits for room in the tile).
+        constexpr bool AHEAD = D < 256;
         uint4 x[2][CPR];
         auto fetch = [&](int which, int step, uint32_t start) {
             const uint8_t* codes = (which ? p.cache.v : p.cache.k) + chunk * 16;
@@ -381,8 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
         };
         int id = load_id(0), id_next = load_id(1);
         uint32_t start = start_of(id, 0);
-        fetch(0, 0, start);
-        fetch(1, 0, start);
+        if (AHEAD) { fetch(0, 0, start); fetch(1, 0, start); }
 #pragma unroll 1
         for (int i = 0; i < steps && !failed; ++i) {
             const int first = 8 * i, b = i & 3, stage = i % STAGES;
@@ -401,12 +402,14 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
                 f = p.scale_log2; lv = 0.0f;
                 key0 = v.paged + (first + c - v.tiles) * 16;
             }
+            const uint32_t start_now = start;
             id = id_next;
             id_next = load_id(i + 2);
             start = start_of(id, i + 1);
 #pragma unroll
             for (int which = 0; which < 2; ++which) {
                 const uint32_t dst = (which ? v_tile : k_tile) + stage * TILE;
+                if (!AHEAD) fetch(which, i, start_now);
                 if (i >= STAGES && !wait_bar(which ? &free_v[stage] : &free_k[stage], (i / STAGES - 1) & 1)) { failed = true; break; }
                 if (which == 0 && c < 32) {              // one warp: what the softmax has to know of the step
                     float lv_top = lv;
@@ -471,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
                 }
                 fence_proxy_async();
                 arrive(which ? &full_v[stage] : &full_k[stage]);
-                fetch(which, i + 1, start);
+                if (AHEAD) fetch(which, i + 1, start);
             }
         }
     } else if (lane == 0) {
