@@ -30,6 +30,12 @@ constexpr int kMaxParts = 32;
 
 __device__ unsigned int g_q8_attn_rejected;
 
+// mma16816 without "volatile": the products may be moved among the unpacking
+__device__ __forceinline__ void product(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
 __device__ __forceinline__ void cp_async8(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -182,7 +188,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
 
     // Scores of TP tiles -> probabilities as B fragments pb; also the running state. Whether all rows see all of them.
     auto softmax = [&](auto tp, float (*s)[NT][4], const float* f, const float* vs, const int* key0, int item, int live,
-                       uint32_t (*pb)[NT][2]) {
+                       uint32_t (*pb)[NT][4]) {
         constexpr int TP = decltype(tp)::value;
         bool whole = true, raise = false;
         float vtop = vs[0];
@@ -272,8 +278,14 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
                     if (!whole && s[i][nt][k] == -INFINITY) e[k] = 0.0f;
                     else e[k] *= w;
                 }
-                pb[i][nt][0] = movmatrix_trans(pack_half2(e[0], e[1]));
-                pb[i][nt][1] = movmatrix_trans(pack_half2(e[2], e[3]));
+                // fp16 takes a probability to 11 bits; what that leaves goes into a second product, so that the output's
+                // own rounding is the only one of its size (one product alone: 1.4 times the error, 3 % less time)
+                const uint32_t h0 = pack_half2(e[0], e[1]), h1 = pack_half2(e[2], e[3]);
+                const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+                pb[i][nt][0] = movmatrix_trans(h0);
+                pb[i][nt][1] = movmatrix_trans(h1);
+                pb[i][nt][2] = movmatrix_trans(pack_half2(e[0] - f0.x, e[1] - f0.y));
+                pb[i][nt][3] = movmatrix_trans(pack_half2(e[2] - f1.x, e[3] - f1.y));
             }
         }
         return whole;
@@ -350,7 +362,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
             const int live = TPI > 1 && item + 1 == q1 ? 1 : TPI;
             float s[TPI][NT][4], f[TPI], vs[TPI];
             int key0[TPI];
-            uint32_t pb[TPI][NT][2];
+            uint32_t pb[TPI][NT][4];
 #pragma unroll
             for (int tt = 0; tt < TPI; ++tt) {
                 const uint2 sc = lds64(src + tt * T::STAGE + 2 * T::BYTES);
@@ -375,7 +387,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
                         q8_unpack<FMT>(bw[i], a1, a3);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt)
-                            mma16816(i & 1 ? s2[nt] : s[tt][nt], a0, a1, a2, a3, qf[nt][4 * j + i][0], qf[nt][4 * j + i][1]);
+                            product(i & 1 ? s2[nt] : s[tt][nt], a0, a1, a2, a3, qf[nt][4 * j + i][0], qf[nt][4 * j + i][1]);
                     }
                 }
 #pragma unroll
@@ -413,8 +425,10 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
                         const int mt = 8 * j + 2 * i;
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            mma16816(o[nt][mt], ab[0], ab[1], cd[0], cd[1], pb[tt][nt][0], pb[tt][nt][1]);
-                            mma16816(o[nt][mt + 1], ab[2], ab[3], cd[2], cd[3], pb[tt][nt][0], pb[tt][nt][1]);
+                            product(o[nt][mt], ab[0], ab[1], cd[0], cd[1], pb[tt][nt][0], pb[tt][nt][1]);
+                            product(o[nt][mt + 1], ab[2], ab[3], cd[2], cd[3], pb[tt][nt][0], pb[tt][nt][1]);
+                            product(o[nt][mt], ab[0], ab[1], cd[0], cd[1], pb[tt][nt][2], pb[tt][nt][3]);
+                            product(o[nt][mt + 1], ab[2], ab[3], cd[2], cd[3], pb[tt][nt][2], pb[tt][nt][3]);
                         }
                     }
                 }
@@ -448,11 +462,11 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
                     const uint4 a = word4(kt, r0 + g, 16 * t + 64 * j + 8 * half), b = word4(kt, r0 + g + 8, 16 * t + 64 * j + 8 * half);
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma16816(s[0][nt], a.x, b.x, a.y, b.y, qf[nt][4 * j + 2 * half][0], qf[nt][4 * j + 2 * half][1]);
-                        mma16816(s[0][nt], a.z, b.z, a.w, b.w, qf[nt][4 * j + 2 * half + 1][0], qf[nt][4 * j + 2 * half + 1][1]);
+                        product(s[0][nt], a.x, b.x, a.y, b.y, qf[nt][4 * j + 2 * half][0], qf[nt][4 * j + 2 * half][1]);
+                        product(s[0][nt], a.z, b.z, a.w, b.w, qf[nt][4 * j + 2 * half + 1][0], qf[nt][4 * j + 2 * half + 1][1]);
                     }
                 }
-            uint32_t pb[1][NT][2];
+            uint32_t pb[1][NT][4];
             const float one = 1.0f;
             softmax(std::integral_constant<int, 1>(), s, &p.scale_log2, &one, &key0, item, 1, pb);
 #pragma unroll
@@ -493,10 +507,11 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        mma16816(o[nt][4 * e + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[0][nt][0], pb[0][nt][1]);
+                        product(o[nt][4 * e + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[0][nt][0], pb[0][nt][1]);
+                        product(o[nt][4 * e + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[0][nt][2], pb[0][nt][3]);
                         if (any_odd) {
                             float hit[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma16816(hit, bad[0], bad[1], bad[2], bad[3], pb[0][nt][0], pb[0][nt][1]);
+                            product(hit, bad[0], bad[1], bad[2], bad[3], pb[0][nt][0], pb[0][nt][1]);
 #pragma unroll
                             for (int k = 0; k < 4; ++k) if (hit[k] != 0.0f) o[nt][4 * e + i][k] = __int_as_float(0x7fc00000);
                         }
@@ -733,34 +748,89 @@ int most_tiles(int max_q, int max_seq, int window, int sinks, int block) {
 
 struct Plan {
     bool wide;                 // 16 query rows per unit, else 8
+    bool prompt;               // the kernel for many rows
     int tiles, units;          // of the longest unit; units of a launch
     int parts, chunk, cluster, warps;
     size_t page_ws, part_ml, part_o, total;   // workspace: offsets and size
 };
 
+// How many parts a unit's context is cut into, and whether the parts form a cluster. The model, in us, fitted to
+// measurements at 8192 and 32768 tokens: a CTA costs kStart before and after its tiles; a warp's two tiles (one at
+// D = 256) take pair_us[c - 1] with c CTAs on a multiprocessor (the copy rate bounds it from c = 2 on at D = 128); a
+// multiprocessor runs its queue in rounds of as many CTAs as fit. Parts are joined in a cluster (about 1 us, parts 2, 4
+// or 8) while all clusters are resident at once -- 16 units of 512 tokens, head_dim 64: 6.8 us against 8.2 with the
+// merge kernel -- and by the merge kernel beyond that (256 units of ragged lengths in 2 parts: 63 us against 56, as
+// clusters wait for all of their CTAs' slots). With one unit per multiprocessor or fewer, eight-warp CTAs with deeper
+// rings (8 units of 32768 tokens: 24.7 us against 26.6).
+constexpr double kStart = 4.0, kClusterUs = 1.0, kMergeUs = 3.0;
+
+void plan_parts(Plan& q, int d) {
+    static const double pair64[4] = {0.95, 1.16, 1.42, 1.73}, pair128[3] = {1.08, 1.57, 2.45}, pair256[2] = {1.3, 2.4};
+    const double* pair_us = d == 64 ? pair64 : d == 128 ? pair128 : pair256;
+    const int resident = d == 64 ? 4 : d == 128 ? 3 : 2, sms = sm_count(), at_once = tiles_at_once(d);
+    const double slow = q.wide ? 1.25 : 1.0;
+    double best = 1e30;
+    auto chunk_of = [&](int parts) { return ((q.tiles + parts - 1) / parts + 1) / 2 * 2; };
+    auto offer = [&](int parts, int cluster, int warps) {
+        const long long queue = ((long long)q.units * parts + sms - 1) / sms;
+        const int pairs = (chunk_of(parts) + warps * at_once - 1) / (warps * at_once);
+        double t = parts == 1 ? 0.0 : cluster ? kClusterUs : kMergeUs;
+        if (warps == 8) {
+            t += (double)queue * (kStart + pairs * slow * pair_us[1]);
+        } else {
+            const int rest = (int)(queue % resident);
+            t += (double)(queue / resident) * (kStart + pairs * slow * pair_us[resident - 1]);
+            if (rest) t += kStart + pairs * slow * pair_us[rest - 1];
+        }
+        // lengths of a batch differ, and a launch of whole units is as long as its longest: 256 units of 500 .. 6000 tokens
+        // take 69 us whole and 56 in two parts, 1024 equal ones of 8192 tokens 356 and 349
+        t *= parts > 1 ? 1.03 : q.tiles >= 192 && q.units > 1 ? 1.15 : 1.0;
+        if (t < best) { best = t; q.parts = parts; q.cluster = cluster; q.warps = warps; }
+    };
+    offer(1, 0, 4);
+    for (int parts = 2; parts <= kMaxParts && q.tiles >= parts * 4; ++parts) {
+        const bool fits = (long long)q.units * parts <= (long long)resident * sms;
+        if (fits && (parts == 2 || parts == 4 || parts == 8)) offer(parts, 1, 4);
+        else offer(parts, 0, 4);
+        if ((long long)q.units * parts <= sms && q.tiles >= parts * 32) offer(parts, 0, 8);
+    }
+    if (const char* e = getenv("KIVI_Q8_PARTS")) { q.parts = atoi(e); q.cluster = q.parts > 1 && q.parts <= 8; }
+    if (const char* e = getenv("KIVI_Q8_WARPS")) q.warps = atoi(e);
+    if (const char* e = getenv("KIVI_Q8_CLUSTER")) q.cluster = q.parts > 1 && atoi(e);
+    q.chunk = chunk_of(q.parts);
+}
+
+// Whether the kernel for many rows is the faster one. It takes 3.1, 3.8 and 4.6 us (head_dim 64, 128, 256) for 128 keys of
+// its 256 (128) rows on every multiprocessor; the other one 0.40, 0.60 and 1.3 ns for 16 keys of 16 rows. At head_dim
+// 128, 8 sequences of 8192 tokens, 8 kv heads: 128 rows each 276 us against 181, 256 rows 287 against 409, 512 rows
+// 282 against 766.
+bool many_rows(int d, int batch, int nkv, long long rows, int tiles) {
+    const int per = d == 256 ? 128 : 256;
+    const double step_us = d == 64 ? 3.1 : d == 128 ? 3.8 : 4.6, tile_us = (d == 64 ? 0.40 : d == 128 ? 0.60 : 1.3) * 1e-3;
+    const long long units = (long long)batch * nkv * ((rows + per - 1) / per), rounds = (units + sm_count() - 1) / sm_count();
+    const double many = 15.0 + (double)rounds * ((tiles + 7) / 8) * step_us;
+    const double few = 20.0 + (double)batch * nkv * ((rows + 15) / 16) * tiles * tile_us;
+    return rows > 16 && 1.25 * many < few;
+}
+
 Plan make_plan(int nkv, int qpk, int d, int block, int batch, int max_q, int max_seq, int window, int sinks, bool mass) {
     Plan q = {};
-    const int rows = max_q * qpk;
+    const long long rows = (long long)max_q * qpk;
     q.wide = rows > 8;
     const int r = q.wide ? 16 : 8;
     q.tiles = most_tiles(max_q, max_seq, window, sinks, block);
-    const long long units = (long long)batch * nkv * (mass ? 1 : (rows + r - 1) / r);
-    q.units = (int)units;
-    int parts = 1, warps = 4;
-    while (parts < 16 && units * parts * 2 <= 3LL * sm_count() && q.tiles >= parts * 8) parts *= 2;
-    if (const char* e = getenv("KIVI_Q8_PARTS")) parts = atoi(e);
-    if (const char* e = getenv("KIVI_Q8_WARPS")) warps = atoi(e);
-    q.cluster = parts > 1 && parts <= 8;
-    if (const char* e = getenv("KIVI_Q8_CLUSTER")) q.cluster = parts > 1 && atoi(e);
-    q.parts = parts; q.warps = warps;
-    q.chunk = ((q.tiles + parts - 1) / parts + 1) / 2 * 2;
+    q.prompt = !mass && many_rows(d, batch, nkv, rows, q.tiles);
+    if (const char* e = getenv("KIVI_Q8_PROMPT")) q.prompt = !mass && rows >= atoi(e);
+    if (q.prompt) return q;
+    q.units = (int)((long long)batch * nkv * (mass ? 1 : (rows + r - 1) / r));
+    plan_parts(q, d);
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     size_t at = 0;
     q.page_ws = at;
     if (mass) at += up((size_t)batch * nkv * q.tiles * r * sizeof(float2));
-    if (parts > 1 && !q.cluster) {
-        q.part_ml = at; at += up((size_t)units * parts * r * sizeof(float2));
-        q.part_o = at; at += up((size_t)units * parts * r * d * sizeof(float));
+    if (q.parts > 1 && !q.cluster) {
+        q.part_ml = at; at += up((size_t)q.units * q.parts * r * sizeof(float2));
+        q.part_o = at; at += up((size_t)q.units * q.parts * r * d * sizeof(float));
     }
     q.total = at;
     return q;
@@ -774,8 +844,8 @@ size_t q8_attention_workspace(int nkv, int qpk, int d, int block, int batch, int
 
 cudaError_t launch_q8_attention(const Q8AttnParams& args, int d, int fmt, void* workspace, cudaStream_t stream) {
     Q8AttnParams p = args;
-    if (const char* e = getenv("KIVI_Q8_PROMPT")) if (!p.mass && p.max_q * p.qpk >= atoi(e)) return launch_q8_prompt(p, d, fmt, stream);
     const Plan plan = make_plan(p.cache.nkv, p.qpk, d, 1 << p.cache.log2b, p.seq.batch, p.max_q, p.max_seq, p.window, p.sinks, p.mass != nullptr);
+    if (plan.prompt) return launch_q8_prompt(p, d, fmt, stream);
     p.ws_tiles = plan.tiles;
     p.parts = plan.parts; p.chunk = plan.chunk; p.cluster = plan.cluster;
     unsigned char* ws = static_cast<unsigned char*>(workspace);
