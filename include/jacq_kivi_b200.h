@@ -327,6 +327,11 @@ int kivi_b200_q8_evict(int num_kv_heads, int block_size, const int32_t* block_ta
  * healthy run. Synchronises the device. */
 int kivi_b200_q8_rejected_indices(uint32_t* count_out);
 
+/* CTAs of the attention kernel for many query rows whose waits on shared-memory barriers, all of them bounded, gave up
+ * since the library was loaded on the current device (their output is undefined); 0 in any healthy run. Synchronises
+ * the device. */
+int kivi_b200_q8_wait_failures(uint32_t* count_out);
+
 /* ------------------------------------------------------------------ ABI v1 (reference lane) -- */
 
 /* ---------------------------------------------------------------------------------------------

@@ -138,6 +138,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
                                        _P, _P, c_size_t, _P]),
     "kivi_b200_q8_evict": (c_int, [c_int, c_int, _P, c_int, _P, _P] + [c_int] * 6 + [_P] * 6),
     "kivi_b200_q8_rejected_indices": (c_int, [ctypes.POINTER(c_uint32)]),
+    "kivi_b200_q8_wait_failures": (c_int, [ctypes.POINTER(c_uint32)]),
     "jac_launch": (None, [_P, _P] + _V1_CACHE + [c_int, _P, _P]),
     "jac_launch_tp2_local": (None, [_P, _P] + _V1_CACHE + [c_int, _P, _P]),
     "jac_launch_batched": (None, [_P, _P, _P] + _V1_CACHE + [c_int, _P, _P]),

@@ -47,7 +47,7 @@ V2_SYMBOLS = (
     "kivi_b200_p2p_region_close", "kivi_b200_p2p_region_destroy", "kivi_b200_p2p_status",
     "kivi_b200_q8_validate_geometry", "kivi_b200_q8_cache_write", "kivi_b200_q8_cache_read",
     "kivi_b200_q8_attention_workspace_bytes", "kivi_b200_q8_attention", "kivi_b200_q8_evict",
-    "kivi_b200_q8_rejected_indices",
+    "kivi_b200_q8_rejected_indices", "kivi_b200_q8_wait_failures",
 )
 
 

@@ -688,7 +688,8 @@ cudaError_t launch(const Q8AttnParams& p, cudaStream_t stream) {
     constexpr size_t ring = (size_t)kWarps * stages_of<D, kWarps>() * tiles_at_once(D) * Tile<D>::STAGE, merge = (size_t)kWarps * 8 * NT * D * 4;
     constexpr size_t smem = ring > merge ? ring : merge;
     auto kernel = q8_attention_kernel<D, FMT, NT, MASS, kWarps>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    static Q8SmemLimit limit;
+    cudaError_t e = limit.raise(kernel, (int)smem);
     if (e != cudaSuccess) return e;
     const unsigned units = (unsigned)((size_t)p.seq.batch * p.cache.nkv * p.row_blocks);
     cudaLaunchConfig_t cfg = {};
@@ -794,9 +795,6 @@ void plan_parts(Plan& q, int d) {
         else offer(parts, 0, 4);
         if ((long long)q.units * parts <= sms && q.tiles >= parts * 32) offer(parts, 0, 8);
     }
-    if (const char* e = getenv("KIVI_Q8_PARTS")) { q.parts = atoi(e); q.cluster = q.parts > 1 && q.parts <= 8; }
-    if (const char* e = getenv("KIVI_Q8_WARPS")) q.warps = atoi(e);
-    if (const char* e = getenv("KIVI_Q8_CLUSTER")) q.cluster = q.parts > 1 && atoi(e);
     q.chunk = chunk_of(q.parts);
 }
 
@@ -820,7 +818,6 @@ Plan make_plan(int nkv, int qpk, int d, int block, int batch, int max_q, int max
     const int r = q.wide ? 16 : 8;
     q.tiles = most_tiles(max_q, max_seq, window, sinks, block);
     q.prompt = !mass && many_rows(d, batch, nkv, rows, q.tiles);
-    if (const char* e = getenv("KIVI_Q8_PROMPT")) q.prompt = !mass && rows >= atoi(e);
     if (q.prompt) return q;
     q.units = (int)((long long)batch * nkv * (mass ? 1 : (rows + r - 1) / r));
     plan_parts(q, d);

@@ -1,7 +1,7 @@
 // Shared by the kernels of the 8-bit block-scaled cache: its pointers, how a launch finds a sequence, conversions.
 #pragma once
 
-#include <cuda_fp8.h>
+#include <atomic>
 
 #include "kivi_common.cuh"
 
@@ -65,6 +65,21 @@ __device__ __forceinline__ void q8_unpack_pairs(uint32_t a, uint32_t b, uint32_t
     q8_unpack<FMT>(x, p[0], p[1]);
     q8_unpack<FMT>(y, p[2], p[3]);
 }
+
+// A kernel's dynamic shared memory limit, raised once per device (a microsecond of every launch otherwise).
+struct Q8SmemLimit {
+    std::atomic<bool> done[64] = {};
+    template <class Kernel>
+    cudaError_t raise(Kernel kernel, int bytes) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e != cudaSuccess) return e;
+        if (dev >= 0 && dev < 64 && done[dev].load(std::memory_order_acquire)) return cudaSuccess;
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+        if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev].store(true, std::memory_order_release);
+        return e;
+    }
+};
 
 // Host launchers.
 struct Q8WriteParams {

@@ -149,7 +149,8 @@ int q8_evict_max_pages() { return kMaxKeys; }
 
 cudaError_t launch_q8_evict(const Q8EvictParams& p, cudaStream_t stream) {
     const size_t smem = sizeof(uint32_t) * (size_t)(p.width < 1 ? 1 : p.width);
-    const cudaError_t e = cudaFuncSetAttribute(q8_evict_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(kMaxKeys * sizeof(uint32_t)));
+    static Q8SmemLimit limit;
+    const cudaError_t e = limit.raise(q8_evict_kernel, (int)(kMaxKeys * sizeof(uint32_t)));
     if (e != cudaSuccess) return e;
     q8_evict_kernel<<<p.batch, kThreads, smem, stream>>>(p);
     return cudaGetLastError();

@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
             int key0 = 0x3fffffff;                       // a tile that is not there: no row sees that far
             if (c < paged) {
                 float2 sc = p.cache.scales[(size_t)id * nkv + u.h];
-                if (!(sc.x + sc.y == sc.x + sc.y)) { odd_page = 1; sc = make_float2(1.0f, 1.0f); }   // seen to at the end
+                if (!(sc.x + sc.y == sc.x + sc.y)) { odd_page = 1; sc = make_float2(1.0f, 0.0f); }   // seen to at the end
                 // a zero scale's codes are zeros too: any other does
                 f = (sc.x == 0.0f ? 1.0f : sc.x) * p.scale_log2;
                 lv = sc.y == 0.0f ? -1000.0f : log2f(sc.y);
@@ -561,7 +561,8 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
 template <int D, int FMT>
 cudaError_t launch(const Q8AttnParams& p, cudaStream_t stream) {
     auto kernel = q8_prompt_kernel<D, FMT>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes<D>());
+    static Q8SmemLimit limit;
+    const cudaError_t e = limit.raise(kernel, smem_bytes<D>());
     if (e != cudaSuccess) return e;
     kernel<<<(unsigned)((size_t)p.seq.batch * p.cache.nkv * p.row_blocks), kThreads, smem_bytes<D>(), stream>>>(p);
     return cudaGetLastError();

@@ -84,6 +84,34 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int = 0, s
     return out, weights, bound
 
 
+def attend_block(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, window: int = 0, sinks: int = 0, products: int = 2,
+                 bias: float = 0.0):
+    """``attend`` for many tokens at once, on the device of its inputs: out and the bound. ``products`` 1: the kernel
+    rounds the probabilities to fp16 (2^-11 each); 2: it keeps what that leaves in a second product, whose own rounding
+    is 2^-22. ``bias``: largest magnitude that a score's codes are shifted by in the product and back in fp32, as a
+    multiple of sum|q| (128 K scales for int8): it is part of the sum whose fp32 accumulation counts."""
+    n, nh, d = q.shape
+    t, nkv, _ = k.shape
+    qpk = nh // nkv
+    scale = 1.0 / math.sqrt(d)
+    out, bound = torch.zeros((2, n, nh, d), dtype=torch.float64, device=q.device)
+    pos, me = torch.arange(t, device=q.device), torch.arange(t - n, t, device=q.device)[:, None]
+    seen = pos <= me
+    if window:
+        seen &= (pos < sinks) | (pos > me - window)
+    for h in range(nh):
+        kk, vv, qq = k[:, h // qpk], v[:, h // qpk], q[:, h].double()
+        s = (qq @ kk.T * scale).masked_fill(~seen, float("-inf"))
+        w = torch.softmax(s, 1).masked_fill(~seen, 0.0)
+        out[:, h] = w @ vv
+        worst = (qq.abs() @ kk.abs().T * scale).masked_fill(~seen, 0.0).amax(1) + qq.abs().sum(1) * scale * bias
+        rel = (2 * (d + 4) * 2.0 ** -24 * worst + 2.0 ** -18)[:, None]
+        half = 2.0 ** -11 if products == 1 else 2.0 ** -22
+        top = torch.where(seen[:, :, None], vv.abs(), 0.0).amax(1) if n * t * d < 1 << 27 else vv.abs().amax(0).expand(n, d)
+        bound[:, h] = (half + rel) * (w @ vv.abs()) + rel * out[:, h].abs() + seen.sum(1)[:, None] * 2.0 ** -30 * top.amax(1, keepdim=True)
+    return out, bound
+
+
 def masses(weights: torch.Tensor, nkv: int, block: int) -> torch.Tensor:
     """[1, NH, T] weights of one token -> [NKV, pages]."""
     _, nh, t = weights.shape

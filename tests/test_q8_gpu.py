@@ -364,6 +364,135 @@ def test_pages_beyond_four_gigabytes(native_lib):
     assert ((k[:100].cpu().double() - w.held()[0][0]).abs() <= HALF * 1.001 * w.held()[0][0].abs() + 2.0 ** -25).all()
 
 
+class Large:
+    """A batch too large for the oracle's loops: codes quantised by the library's own writer (whose bits the tests above
+    pin) and read back, attention against the oracle in 64 bits on the device."""
+
+    def __init__(self, layout, lens, seed):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        self.layout, self.lens, self.g = layout, lens, g
+        nkv, b, d = layout.num_kv_heads, layout.block_size, layout.head_dim
+        width = max(1, -(-max(lens) // b))
+        self.cache = Q8Cache(layout, len(lens) * width + 1, len(lens), width, DEV)
+        ids = torch.randperm(len(lens) * width, generator=torch.Generator().manual_seed(seed)).to(torch.int32)
+        self.cache.set_block_tables(ids.view(len(lens), width))
+        total = sum(lens)
+        self.k, self.v = (torch.randn((total, nkv, d), generator=g, device=DEV).half() for _ in range(2))
+        self.k[..., 1::29] *= 10.0
+        self.at = offsets_of(lens)
+        self.cache.write(self.k, self.v, i32(self.at), max_new_per_seq=max(lens), max_start_seq_len=0)
+        self.scales = [float(x) for x in self.cache.tensors.SCALES.nan_to_num().amax((0, 1))]
+
+    def held(self, i):
+        """K and V of sequence i in 64 bits: the pages' codes times their scales, the tail as it is."""
+        t, c = self.lens[i], self.cache
+        b, nkv, d = self.layout.block_size, self.layout.num_kv_heads, self.layout.head_dim
+        ids, got = c.block_tables[i, :t // b].long(), []
+        for j, (pages, rows) in enumerate(((c.tensors.K_PAGES, self.k), (c.tensors.V_PAGES, self.v))):
+            codes = pages.view(torch.int8)[ids].view(pages.dtype).float().double()
+            x = (codes * c.tensors.SCALES[ids, :, j].double()[..., None, None]).transpose(1, 2).reshape(-1, nkv, d)
+            got.append(torch.cat([x, rows[self.at[i] + t // b * b:self.at[i + 1]].double()]))
+        return got
+
+    def check(self, counts, window=0, sinks=0, half=True, products=2):
+        lay = self.layout
+        q = torch.randn((sum(counts), lay.num_q_heads, lay.head_dim), generator=self.g, device=DEV).half()
+        got = torch.full(q.shape, 9.0, dtype=torch.float16 if half else torch.float32, device=DEV)
+        kw = {} if max(counts) == 1 and min(counts) == 1 else dict(q_offsets=i32(offsets_of(counts)), max_q_per_seq=max(counts))
+        self.cache.attend(q, got, max_seq_len=max(self.lens), window=window, sinks=sinks, **kw)
+        at = offsets_of(counts)
+        for i, n in enumerate(counts):
+            if not n:
+                continue
+            bias = 128.0 * self.scales[0] if products == 1 and lay.fmt == "int8" else 0.0
+            want, bound = qo.attend_block(q[at[i]:at[i + 1]], *self.held(i), window, sinks, products, bias)
+            if half:
+                bound = bound + HALF * want.abs() + 2.0 ** -25
+            err = (got[at[i]:at[i + 1]].double() - want).abs()
+            assert (err <= bound).all(), (i, float((err - bound).max()), float(err.max()), (err > bound).nonzero()[:3].tolist())
+
+
+# many rows: the batch is large enough for the kernel of 256-row units (128 at head_dim 256) to be chosen
+MANY = [(Q8Layout(8, 2, 128, 16, "int8"), 48, 300), (Q8Layout(32, 4, 64, 32, "e4m3"), 16, 400), (Q8Layout(14, 2, 64, 16, "int8"), 30, 300),
+        (Q8Layout(12, 4, 128, 128, "e4m3"), 24, 500), (Q8Layout(6, 2, 256, 16, "int8"), 24, 300), (Q8Layout(16, 1, 256, 64, "e4m3"), 16, 300)]
+
+
+@pytest.mark.parametrize("layout,batch,longest", MANY, ids=[f"{x.num_q_heads}/{x.num_kv_heads}x{x.head_dim}b{x.block_size}{x.fmt}" for x, _, _ in MANY])
+def test_attention_of_prompts(layout, batch, longest, native_lib):
+    rng = random.Random(batch)
+    lens = [longest] + [rng.randint(1, longest) for _ in range(batch - 1)]
+    lens[1], lens[2], lens[3] = 1, layout.block_size, longest - 1
+    w = Large(layout, lens, 31)
+    counts = [t if i % 3 else rng.randint(0, t) for i, t in enumerate(lens)]
+    counts[0] = longest
+    for window, sinks, half in ((0, 0, True), (0, 0, False), (33, 5, True), (longest // 2, 200, True), (1, 0, False)):
+        w.check(counts, window, sinks, half, products=1)
+    fewer = [min(t, 130) for t in lens]              # one tile of rows with a few in the second
+    w.check(fewer, 0, 0, True, products=1)
+
+
+def test_prompt_chunk_behind_a_long_cache(native_lib):
+    w = Large(Q8Layout(32, 8, 128, 16, "int8"), [3000, 2100], 32)
+    w.check([513, 700], window=1024, sinks=4, products=1)
+    w.check([513, 700], products=1)
+
+
+def test_prompts_with_masked_and_visible_poison(native_lib):
+    """In the kernel for many rows: a page with a NaN scale, an infinity in a tail row of V."""
+    layout, n = Q8Layout(8, 2, 128, 32, "int8"), 48
+    w = Large(layout, [300] * n, 33)
+    clean = w.cache
+    k, v = w.k.clone(), w.v.clone()
+    k[100, 1, 7] = float("nan")                      # sequence 0, page 3 (tokens 96 .. 127), kv head 1
+    v[295, 0, 9] = float("inf")                      # sequence 0, tail (tokens 288 ..), kv head 0
+    bad = Q8Cache(layout, clean.num_blocks, n, clean.max_blocks_per_seq, DEV)
+    bad.set_block_tables(clean.block_tables)
+    bad.write(k, v, i32(w.at), max_new_per_seq=300, max_start_seq_len=0)
+    q = torch.randn((300 * n, 8, 128), generator=w.g, device=DEV).half()
+    kw = dict(max_seq_len=300, q_offsets=i32([300 * i for i in range(n + 1)]), max_q_per_seq=300)
+    outs = []
+    for window in (0, 40):
+        for cache in (clean, bad):
+            out = torch.empty_like(q)
+            cache.attend(q, out, window=window, **kw)
+            outs.append(out)
+    tok = torch.arange(300, device=DEV)
+    for window, good, got in ((0, *outs[:2]), (40, *outs[2:])):
+        assert torch.equal(got[300:], good[300:])    # the other sequences
+        hit = torch.zeros((300, 8, 128), dtype=torch.bool, device=DEV)
+        seen = (tok >= 96) if window == 0 else (tok >= 96) & (tok < 127 + window)
+        hit[:, 4:] = seen[:, None, None]
+        hit[295:, :4, 9] = True
+        assert got[:300][hit].isnan().all() and torch.equal(got[:300][~hit], good[:300][~hit])
+
+
+@pytest.mark.parametrize("layout,lens", [
+    (Q8Layout(8, 2, 128, 16, "int8"), [20000]), (Q8Layout(10, 1, 64, 16, "e4m3"), [30000]), (Q8Layout(4, 2, 256, 32, "int8"), [9000]),
+    (Q8Layout(32, 8, 128, 16, "e4m3"), [5000, 1, 4000, 300, 16, 2500]), (Q8Layout(14, 2, 64, 32, "int8"), [700] * 20 + [3, 1500]),
+    (Q8Layout(32, 8, 128, 16, "int8"), [2000] * 40), (Q8Layout(16, 1, 128, 64, "int8"), [6000, 100, 3333])])
+def test_contexts_cut_into_parts(layout, lens, native_lib):
+    """Long contexts of few units (many parts, the merge kernel, eight-warp CTAs), of some (clusters) and of many."""
+    w = Large(layout, lens, 34)
+    w.check([1] * len(lens))
+    w.check([1] * len(lens), half=False)
+    w.check([1] * len(lens), window=1000, sinks=3)
+    w.check([min(t, 3) for t in lens])
+
+
+def test_masses_of_a_long_context(native_lib):
+    w = Large(Q8Layout(10, 2, 128, 16, "int8"), [20000, 777], 35)
+    q = torch.randn((2, 10, 128), generator=w.g, device=DEV).half()
+    mass = torch.zeros((2, 2, 1250), device=DEV)
+    w.cache.attend(q, max_seq_len=20000, page_mass=mass)
+    for i, t in enumerate(w.lens):
+        k, _ = w.held(i)
+        s = torch.stack([q[i, h].double() @ k[:, h // 5].T / 128 ** 0.5 for h in range(10)])
+        p = torch.nn.functional.pad(torch.softmax(s, 1), (0, 20000 - t)).view(2, 5, 1250, 16).sum((1, 3))
+        # a weight is off by the fp32 errors of its score, at most 2 (D + 4) 2^-24 sum|q k| / sqrt(D), here under 200, and 2^-18
+        assert ((mass[i].double() - p).abs() <= (2 * 132 * 2.0 ** -24 * 200 + 2.0 ** -18) * p + 2.0 ** -40).all()
+        assert abs(float(mass[i].double().sum()) - 10) < 1e-3
+
+
 # ------------------------------------------------------------------------------------------------ page masses, eviction
 
 @pytest.mark.parametrize("layout", LAYOUTS, ids=IDS)
@@ -629,3 +758,9 @@ def test_python_refusals(native_lib):
         Q8Cache.over(layout, Q8CacheTensors(*w.cache.tensors)._replace(SCALES=w.cache.tensors.SCALES.half()), w.cache.block_tables, w.cache.seq_lens)
     assert w.cache.attend(q[:0], max_seq_len=64).shape == (0, 4, 64)
     w.cache.write(k[:0], k[:0], i32([0, 0, 0]), **kw)
+
+
+def test_no_bounded_wait_gave_up(native_lib):
+    import ctypes
+    out = ctypes.c_uint32(123)
+    assert native_lib.kivi_b200_q8_wait_failures(ctypes.byref(out)) == 0 and out.value == 0

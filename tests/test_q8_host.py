@@ -154,7 +154,7 @@ def test_bytes_of_a_decode_step():
 def test_workspace_bytes_follow_the_visible_context(native_lib):
     g = geometry()
     ask = lambda *a: native_lib.kivi_b200_q8_attention_workspace_bytes(ctypes.byref(g), *a)  # noqa: E731
-    assert ask(400, 1, 4096, 0, 0, 0) == 0          # units enough to fill the GPU uncut: nothing to join
+    assert ask(400, 1, 512, 0, 0, 0) == 0           # units enough to fill the GPU uncut: nothing to join
     full, windowed = ask(4, 1, 4096, 0, 0, 1), ask(4, 1, 4096, 256, 4, 1)
     assert full >= 4 * 2 * 256 * 8 * 8 and 0 < windowed < full // 8
     for bad in ((0, 1, 10, 0, 0, 1), (1, 0, 10, 0, 0, 1), (1, 1, -1, 0, 0, 1), (1, 1, 10, -1, 0, 1), (1, 1, 10, 0, -1, 1)):
