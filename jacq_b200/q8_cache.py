@@ -91,13 +91,13 @@ def _int32(t: torch.Tensor, name: str, index: int) -> int:
     return t.data_ptr()
 
 
-def _call(index: int, where: str, fn, *args) -> None:
-    """One library call on the current stream of device `index`, with that device current."""
-    if torch.cuda.current_device() == index:
+_current_device = torch._C._cuda_getDevice
+
+
+def _elsewhere(index: int, where: str, fn, *args) -> None:
+    """A library call on the current stream of device `index` where another device is the current one."""
+    with torch.cuda.device(index):
         rc = fn(*args, _raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(*args, _raw_stream(index))
     if rc:
         _native.check(rc, where)
 
@@ -152,8 +152,10 @@ class Q8Cache:
         self.num_blocks, self.num_slots = blocks, slots
         self._geom = _native.KiviQ8Geometry(layout.num_q_heads, nkv, d, b, _FORMATS[layout.fmt][0])
         self._struct = _native.KiviQ8CacheStruct(*[t.data_ptr() for t in tensors], blocks, slots)
-        self._refs = (ctypes.byref(self._geom), ctypes.byref(self._struct))
-        self._lib = _native.lib()
+        self._geom_ref, self._cache_ref = ctypes.byref(self._geom), ctypes.byref(self._struct)
+        lib = _native.lib()
+        self._write, self._read, self._attention = lib.kivi_b200_q8_cache_write, lib.kivi_b200_q8_cache_read, lib.kivi_b200_q8_attention
+        self._workspace_of = lib.kivi_b200_q8_attention_workspace_bytes
         self._workspace_bytes: dict[tuple, int] = {}   # by the sizes of a call; the plan behind them is host arithmetic
 
     def set_block_tables(self, tables: torch.Tensor) -> None:
@@ -209,9 +211,15 @@ class Q8Cache:
         offsets = _int32(new_offsets, "new_offsets", self._index)
         n = new_offsets.numel() - 1
         tables, starts, slots, keep = self._rows(n, slot_ids, start_seq_lens)
-        _call(self._index, "kivi_b200_q8_cache_write", self._lib.kivi_b200_q8_cache_write, *self._refs, new_k.data_ptr(),
-              new_v.data_ptr(), ks, vs, tables, self.max_blocks_per_seq, starts, offsets, slots, n, total, max_new_per_seq,
-              max_start_seq_len)
+        index, geom, cache = self._index, self._geom_ref, self._cache_ref
+        if index == _current_device():
+            rc = self._write(geom, cache, new_k.data_ptr(), new_v.data_ptr(), ks, vs, tables, self.max_blocks_per_seq, starts, offsets,
+                             slots, n, total, max_new_per_seq, max_start_seq_len, _raw_stream(index))
+            if rc:
+                _native.check(rc, "kivi_b200_q8_cache_write")
+        else:
+            _elsewhere(index, "kivi_b200_q8_cache_write", self._write, geom, cache, new_k.data_ptr(), new_v.data_ptr(), ks, vs, tables,
+                       self.max_blocks_per_seq, starts, offsets, slots, n, total, max_new_per_seq, max_start_seq_len)
         if advance and start_seq_lens is None:
             counts = new_offsets[1:] - new_offsets[:-1]
             if slot_ids is None:
@@ -226,19 +234,27 @@ class Q8Cache:
         tokens ``first_rows[i]`` onwards of sequence i, zeros behind its last token."""
         shape = (total, self.layout.num_kv_heads, self.layout.head_dim)
         if k_out is None:
-            k_out = torch.empty(shape, dtype=torch.float16, device=self.device)
+            k_out = self.tensors.K_TAIL.new_empty(shape)
+        elif k_out.dtype is not torch.float16 or k_out.shape != shape or not k_out.is_contiguous() or k_out.get_device() != self._index:
+            raise TypeError(f"k_out must be a contiguous torch.float16 tensor {shape} on {self.device}")
         if v_out is None:
-            v_out = torch.empty(shape, dtype=torch.float16, device=self.device)
-        for name, t in (("k_out", k_out), ("v_out", v_out)):
-            if t.dtype is not torch.float16 or t.shape != shape or not t.is_contiguous() or t.get_device() != self._index:
-                raise TypeError(f"{name} must be a contiguous torch.float16 tensor {shape} on {self.device}")
+            v_out = self.tensors.K_TAIL.new_empty(shape)
+        elif v_out.dtype is not torch.float16 or v_out.shape != shape or not v_out.is_contiguous() or v_out.get_device() != self._index:
+            raise TypeError(f"v_out must be a contiguous torch.float16 tensor {shape} on {self.device}")
         offsets, first = _int32(row_offsets, "row_offsets", self._index), _int32(first_rows, "first_rows", self._index)
         n = row_offsets.numel() - 1
         if first_rows.numel() < n:
             raise RuntimeError(f"first_rows holds {first_rows.numel()} entries for a batch of {n}")
         tables, lens, slots, keep = self._rows(n, slot_ids, seq_lens)
-        _call(self._index, "kivi_b200_q8_cache_read", self._lib.kivi_b200_q8_cache_read, *self._refs, tables, self.max_blocks_per_seq,
-              lens, slots, offsets, first, n, total, max_rows_per_seq, k_out.data_ptr(), v_out.data_ptr())
+        index, geom, cache = self._index, self._geom_ref, self._cache_ref
+        if index == _current_device():
+            rc = self._read(geom, cache, tables, self.max_blocks_per_seq, lens, slots, offsets, first, n, total, max_rows_per_seq,
+                            k_out.data_ptr(), v_out.data_ptr(), _raw_stream(index))
+            if rc:
+                _native.check(rc, "kivi_b200_q8_cache_read")
+        else:
+            _elsewhere(index, "kivi_b200_q8_cache_read", self._read, geom, cache, tables, self.max_blocks_per_seq, lens, slots, offsets,
+                       first, n, total, max_rows_per_seq, k_out.data_ptr(), v_out.data_ptr())
         return k_out, v_out
 
     def attend(self, q: torch.Tensor, out: torch.Tensor | None = None, *, max_seq_len: int, window: int = 0, sinks: int = 0,
@@ -276,15 +292,26 @@ class Q8Cache:
         sizes = (batch, max_q_per_seq, max_seq_len, window, sinks, page_mass is not None)
         size = self._workspace_bytes.get(sizes)
         if size is None:
-            size = self._workspace_bytes[sizes] = self._lib.kivi_b200_q8_attention_workspace_bytes(self._refs[0], *sizes)
+            size = self._workspace_bytes[sizes] = self._workspace_of(self._geom_ref, *sizes)
         workspace, at = None, 0
         if size:   # of this call alone: the allocator hands it on in stream order, or keeps it for a graph under capture
             workspace = torch.empty(size, dtype=torch.uint8, device=self.device)
             at = workspace.data_ptr()
-        target = out.data_ptr()
-        _call(self._index, "kivi_b200_q8_attention", self._lib.kivi_b200_q8_attention, *self._refs, q.data_ptr(), stride, offsets, total,
-              tables, self.max_blocks_per_seq, lens, slots, batch, max_q_per_seq, max_seq_len, window, sinks, scale, mass, mass_width,
-              0 if half else target, target if half else 0, at, size)
+        if half:
+            out32, out16 = 0, out.data_ptr()
+        else:
+            out32, out16 = out.data_ptr(), 0
+        index, geom, cache = self._index, self._geom_ref, self._cache_ref
+        if index == _current_device():
+            rc = self._attention(geom, cache, q.data_ptr(), stride, offsets, total, tables, self.max_blocks_per_seq, lens, slots, batch,
+                                 max_q_per_seq, max_seq_len, window, sinks, scale, mass, mass_width, out32, out16, at, size,
+                                 _raw_stream(index))
+            if rc:
+                _native.check(rc, "kivi_b200_q8_attention")
+        else:
+            _elsewhere(index, "kivi_b200_q8_attention", self._attention, geom, cache, q.data_ptr(), stride, offsets, total, tables,
+                       self.max_blocks_per_seq, lens, slots, batch, max_q_per_seq, max_seq_len, window, sinks, scale, mass, mass_width,
+                       out32, out16, at, size)
         return out
 
     def evict(self, page_mass: torch.Tensor, *, budget: int, first: int = 0, recent: int = 0, max_seq_len: int,
@@ -322,15 +349,18 @@ def evict_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, page_mass: t
     _check_mass(page_mass, batch, None, index)
     _, nkv, mass_width = page_mass.shape
     mass = torch.empty_like(page_mass)
-    ints = torch.empty((2 * width + 2, batch), dtype=torch.int32, device=block_tables.device)   # both tables and both counts
-    both = ints[:2 * width].view(2, batch, width)
-    out = Q8Eviction(both[0], ints[2 * width], mass, both[1], ints[2 * width + 1])
-    at = ints.data_ptr()
-    table_bytes, row_bytes = 4 * batch * width, 4 * batch
-    _call(index, "kivi_b200_q8_evict", _native.lib().kivi_b200_q8_evict, nkv, block_size, tables, width, lens, page_mass.data_ptr(),
-          mass_width, batch, max_seq_len, budget, first, recent, at, at + 2 * table_bytes, mass.data_ptr(), at + table_bytes,
-          at + 2 * table_bytes + row_bytes)
-    return out
+    new_tables, freed = torch.empty_like(block_tables), torch.empty_like(block_tables)
+    new_lens, counts = torch.empty_like(seq_lens), torch.empty_like(seq_lens)
+    args = (nkv, block_size, tables, width, lens, page_mass.data_ptr(), mass_width, batch, max_seq_len, budget, first, recent,
+            new_tables.data_ptr(), new_lens.data_ptr(), mass.data_ptr(), freed.data_ptr(), counts.data_ptr())
+    fn = _native.lib().kivi_b200_q8_evict
+    if index == _current_device():
+        rc = fn(*args, _raw_stream(index))
+        if rc:
+            _native.check(rc, "kivi_b200_q8_evict")
+    else:
+        _elsewhere(index, "kivi_b200_q8_evict", fn, *args)
+    return Q8Eviction(new_tables, new_lens, mass, freed, counts)
 
 
 def rejected_indices() -> int:
