@@ -119,18 +119,22 @@ __device__ __forceinline__ void add_masses(const Q8AttnParams& p, const Unit& u,
 // Two shapes of the kernel. Four warps and a shallow ring, several CTAs per multiprocessor, where there are units enough
 // to fill it; eight warps and a deep ring, one CTA per multiprocessor, where there are few and each warp's own copies
 // have to cover the latency.
-#ifndef Q8S4
-#define Q8S4 2
-#define Q8C4 3
-#endif
 constexpr int tiles_at_once(int d) { return d == 256 ? 1 : 2; }
 template <int D, int kWarps>
-constexpr int stages_of() { return kWarps == 4 ? (D == 64 ? 3 : D == 128 ? Q8S4 : 3) : D == 64 ? 5 : 3; }
+constexpr int stages_of() { return kWarps == 4 ? (D == 64 ? 3 : D == 128 ? 2 : 3) : D == 64 ? 5 : 3; }
 template <int D, int kWarps>
-constexpr int ctas_of(int nt) { return kWarps == 8 ? 1 : D == 64 ? 4 : D == 128 ? Q8C4 : 2; }
+constexpr int ctas_of() { return kWarps == 8 ? 1 : D == 64 ? 4 : D == 128 ? 3 : 2; }
 
-template <int D, int FMT, int NT, bool MASS, int kWarps>
-__global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attention_kernel(const Q8AttnParams p) {
+// Query rows of a unit: at most 4, at most 8, at most 16. Probabilities are kept to 22 bits as two fp16 numbers (the
+// output's own rounding is then the only one of its size; one number alone gave 1.4 times the plain form's error). With
+// at most 4 rows the second numbers are columns 4 .. 7 of the same product, whose queries repeat columns 0 .. 3; beyond
+// that they take a second product. 128 x 8192 tokens, 4 rows, back to back at the power limit: 408 us with one number,
+// 404 with both in one product, 419 with two products.
+constexpr int kRows4 = 4, kRows8 = 8, kRows16 = 16;
+
+template <int D, int FMT, int ROWS, bool MASS, int kWarps, int NT>   // NT: groups of 8 columns, ROWS / 8 or 1
+__global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>()) q8_attention_kernel(const Q8AttnParams p) {
+    constexpr bool FOLD = ROWS == kRows4;
     using T = Tile<D>;
     constexpr int R = 8 * NT, S = stages_of<D, kWarps>(), TPI = tiles_at_once(D);
     extern __shared__ __align__(16) unsigned char smem[];
@@ -151,7 +155,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
     uint32_t qf[NT][T::MT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int r = rb * R + 8 * nt + g;
+        const int r = rb * R + 8 * nt + (FOLD ? g & 3 : g);
         const __half* row = p.q + (long long)(row0 + r / p.qpk) * p.q_stride + (size_t)(h * p.qpk + r % p.qpk) * D + 16 * t;
 #pragma unroll
         for (int j = 0; j < T::KC; ++j) {
@@ -170,7 +174,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-            const int r = rb * R + 8 * nt + 2 * t + c;
+            const int r = rb * R + 8 * nt + (FOLD ? 2 * (t & 1) : 2 * t) + c;
             hi[nt][c] = r < rows ? len - n + r / p.qpk : -1;
             lo[nt][c] = p.window == 0x7fffffff ? 0 : hi[nt][c] - p.window + 1;
         }
@@ -185,6 +189,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
     }
     // V's scales enter the fp16 probabilities relative to vref, a power of two not below any met so far (0: none yet)
     float vref = 0.0f, vmul = 0.0f;
+    const float second = FOLD && t >= 2 ? 1.0f : 0.0f;
 
     // Scores of TP tiles -> probabilities as B fragments pb; also the running state. Whether all rows see all of them.
     auto softmax = [&](auto tp, float (*s)[NT][4], const float* f, const float* vs, const int* key0, int item, int live,
@@ -278,14 +283,17 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
                     if (!whole && s[i][nt][k] == -INFINITY) e[k] = 0.0f;
                     else e[k] *= w;
                 }
-                // fp16 takes a probability to 11 bits; what that leaves goes into a second product, so that the output's
-                // own rounding is the only one of its size (one product alone: 1.4 times the error, 3 % less time)
                 const uint32_t h0 = pack_half2(e[0], e[1]), h1 = pack_half2(e[2], e[3]);
                 const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-                pb[i][nt][0] = movmatrix_trans(h0);
-                pb[i][nt][1] = movmatrix_trans(h1);
-                pb[i][nt][2] = movmatrix_trans(pack_half2(e[0] - f0.x, e[1] - f0.y));
-                pb[i][nt][3] = movmatrix_trans(pack_half2(e[2] - f1.x, e[3] - f1.y));
+                if (FOLD) {   // columns 4 .. 7 have the probabilities of 0 .. 3 and take what fp16 leaves of them
+                    pb[i][nt][0] = movmatrix_trans(pack_half2(fmaf(-second, f0.x, e[0]), fmaf(-second, f0.y, e[1])));
+                    pb[i][nt][1] = movmatrix_trans(pack_half2(fmaf(-second, f1.x, e[2]), fmaf(-second, f1.y, e[3])));
+                } else {
+                    pb[i][nt][0] = movmatrix_trans(h0);
+                    pb[i][nt][1] = movmatrix_trans(h1);
+                    pb[i][nt][2] = movmatrix_trans(pack_half2(e[0] - f0.x, e[1] - f0.y));
+                    pb[i][nt][3] = movmatrix_trans(pack_half2(e[2] - f1.x, e[3] - f1.y));
+                }
             }
         }
         return whole;
@@ -427,8 +435,10 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
                         for (int nt = 0; nt < NT; ++nt) {
                             product(o[nt][mt], ab[0], ab[1], cd[0], cd[1], pb[tt][nt][0], pb[tt][nt][1]);
                             product(o[nt][mt + 1], ab[2], ab[3], cd[2], cd[3], pb[tt][nt][0], pb[tt][nt][1]);
-                            product(o[nt][mt], ab[0], ab[1], cd[0], cd[1], pb[tt][nt][2], pb[tt][nt][3]);
-                            product(o[nt][mt + 1], ab[2], ab[3], cd[2], cd[3], pb[tt][nt][2], pb[tt][nt][3]);
+                            if (!FOLD) {
+                                product(o[nt][mt], ab[0], ab[1], cd[0], cd[1], pb[tt][nt][2], pb[tt][nt][3]);
+                                product(o[nt][mt + 1], ab[2], ab[3], cd[2], cd[3], pb[tt][nt][2], pb[tt][nt][3]);
+                            }
                         }
                     }
                 }
@@ -508,7 +518,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         product(o[nt][4 * e + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[0][nt][0], pb[0][nt][1]);
-                        product(o[nt][4 * e + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[0][nt][2], pb[0][nt][3]);
+                        if (!FOLD) product(o[nt][4 * e + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[0][nt][2], pb[0][nt][3]);
                         if (any_odd) {
                             float hit[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                             product(hit, bad[0], bad[1], bad[2], bad[3], pb[0][nt][0], pb[0][nt][1]);
@@ -573,7 +583,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
 #pragma unroll
             for (int w = 0; w < kWarps; ++w)
 #pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] += so[w * VEC + at + k * 64];   // channel + 1: two accumulators further
+                for (int k = 0; k < 4; ++k)   // channel + 1: two accumulators further; column + 4: two lanes
+                    x[k] += so[w * VEC + at + k * 64] + (FOLD && r < 4 ? so[w * VEC + at + k * 64 + 2] : 0.0f);
             reinterpret_cast<float4*>(p.part_o)[slot * (R * D / 4) + e] = make_float4(x[0], x[1], x[2], x[3]);
         }
         if (threadIdx.x < R) p.part_ml[slot * R + threadIdx.x] = make_float2(c_m[threadIdx.x], c_l[threadIdx.x]);
@@ -619,13 +630,13 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>(NT)) q8_attent
                 const float a = fast_exp2(*cluster.map_shared_rank(&c_m[r], rank) - f_m[r]);
                 const float* peer = cluster.map_shared_rank(src, rank);
 #pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] += a * peer[k * 64];
+                for (int k = 0; k < 8; ++k) x[k] += a * (peer[k * 64] + (FOLD ? peer[k * 64 + 2] : 0.0f));
             }
         } else {
 #pragma unroll
             for (int w = 0; w < kWarps; ++w)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) x[k] += src[w * VEC + k * 64];
+                for (int k = 0; k < 8; ++k) x[k] += src[w * VEC + k * 64] + (FOLD ? src[w * VEC + k * 64 + 2] : 0.0f);
         }
         const float il = f_il[r];
 #pragma unroll
@@ -683,11 +694,12 @@ __global__ void __launch_bounds__(256) q8_merge_kernel(const Q8AttnParams p) {
     if constexpr (MASS) add_masses<R>(p, u, f_m, f_il, blockIdx.y * 256 + threadIdx.x, gridDim.y * 256);
 }
 
-template <int D, int FMT, int NT, bool MASS, int kWarps>
+template <int D, int FMT, int ROWS, bool MASS, int kWarps>
 cudaError_t launch(const Q8AttnParams& p, cudaStream_t stream) {
+    constexpr int NT = ROWS == kRows16 ? 2 : 1;
     constexpr size_t ring = (size_t)kWarps * stages_of<D, kWarps>() * tiles_at_once(D) * Tile<D>::STAGE, merge = (size_t)kWarps * 8 * NT * D * 4;
     constexpr size_t smem = ring > merge ? ring : merge;
-    auto kernel = q8_attention_kernel<D, FMT, NT, MASS, kWarps>;
+    auto kernel = q8_attention_kernel<D, FMT, ROWS, MASS, kWarps, NT>;
     static Q8SmemLimit limit;
     cudaError_t e = limit.raise(kernel, (int)smem);
     if (e != cudaSuccess) return e;
@@ -717,23 +729,24 @@ cudaError_t launch(const Q8AttnParams& p, cudaStream_t stream) {
     return cudaLaunchKernelEx(&merge_cfg, q8_merge_kernel<D, NT, MASS>, p);
 }
 
-template <int D, int FMT, bool MASS>
-cudaError_t launch_shape(const Q8AttnParams& p, bool wide, int warps, cudaStream_t stream) {
-    if (warps == 4) return wide ? launch<D, FMT, 2, MASS, 4>(p, stream) : launch<D, FMT, 1, MASS, 4>(p, stream);
-    return wide ? launch<D, FMT, 2, MASS, 8>(p, stream) : launch<D, FMT, 1, MASS, 8>(p, stream);
+template <int D, int FMT, bool MASS, int kWarps>
+cudaError_t launch_shape(const Q8AttnParams& p, int rows, cudaStream_t stream) {
+    return rows == kRows4 ? launch<D, FMT, kRows4, MASS, kWarps>(p, stream)
+         : rows == kRows8 ? launch<D, FMT, kRows8, MASS, kWarps>(p, stream) : launch<D, FMT, kRows16, MASS, kWarps>(p, stream);
 }
 
 template <int D, int FMT>
-cudaError_t launch_rows(Q8AttnParams p, bool wide, int warps, cudaStream_t stream) {
-    const int r = wide ? 16 : 8, rows = p.max_q * p.qpk, blocks = (rows + r - 1) / r;
+cudaError_t launch_rows(Q8AttnParams p, int warps, cudaStream_t stream) {
+    const int n = p.max_q * p.qpk, r = n > 8 ? 16 : 8, blocks = (n + r - 1) / r;
+    const int rows = n <= 4 ? kRows4 : n <= 8 ? kRows8 : kRows16;
     if (!p.mass) {
         p.row_blocks = blocks; p.row_block0 = 0;
-        return launch_shape<D, FMT, false>(p, wide, warps, stream);
+        return warps == 4 ? launch_shape<D, FMT, false, 4>(p, rows, stream) : launch_shape<D, FMT, false, 8>(p, rows, stream);
     }
     // page masses of a kv head grow by one block of query heads at a time: its own launch, so nothing races
     p.row_blocks = 1;
     for (p.row_block0 = 0; p.row_block0 < blocks; ++p.row_block0) {
-        const cudaError_t e = launch_shape<D, FMT, true>(p, wide, warps, stream);
+        const cudaError_t e = warps == 4 ? launch_shape<D, FMT, true, 4>(p, rows, stream) : launch_shape<D, FMT, true, 8>(p, rows, stream);
         if (e != cudaSuccess) return e;
     }
     return cudaSuccess;
@@ -850,12 +863,11 @@ cudaError_t launch_q8_attention(const Q8AttnParams& args, int d, int fmt, void* 
     p.part_ml = reinterpret_cast<float2*>(ws + plan.part_ml);
     p.part_o = reinterpret_cast<float*>(ws + plan.part_o);
     const bool i8 = fmt == KIVI_Q8_INT8;
-    const bool wide = plan.wide;
     const int warps = plan.warps;
     switch (d) {
-        case 64: return i8 ? launch_rows<64, KIVI_Q8_INT8>(p, wide, warps, stream) : launch_rows<64, KIVI_Q8_E4M3>(p, wide, warps, stream);
-        case 128: return i8 ? launch_rows<128, KIVI_Q8_INT8>(p, wide, warps, stream) : launch_rows<128, KIVI_Q8_E4M3>(p, wide, warps, stream);
-        default: return i8 ? launch_rows<256, KIVI_Q8_INT8>(p, wide, warps, stream) : launch_rows<256, KIVI_Q8_E4M3>(p, wide, warps, stream);
+        case 64: return i8 ? launch_rows<64, KIVI_Q8_INT8>(p, warps, stream) : launch_rows<64, KIVI_Q8_E4M3>(p, warps, stream);
+        case 128: return i8 ? launch_rows<128, KIVI_Q8_INT8>(p, warps, stream) : launch_rows<128, KIVI_Q8_E4M3>(p, warps, stream);
+        default: return i8 ? launch_rows<256, KIVI_Q8_INT8>(p, warps, stream) : launch_rows<256, KIVI_Q8_E4M3>(p, warps, stream);
     }
 }
 

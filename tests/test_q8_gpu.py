@@ -479,6 +479,34 @@ def test_contexts_cut_into_parts(layout, lens, native_lib):
     w.check([min(t, 3) for t in lens])
 
 
+def test_a_captured_call_with_parts_and_a_captured_prompt(native_lib):
+    """Two graphs, one with the merge kernel and one with the kernel for many rows, replayed in turn and on two streams."""
+    w = Large(Q8Layout(10, 2, 128, 16, "int8"), [9000, 700], 36)
+    many = Large(Q8Layout(8, 2, 128, 16, "int8"), [300] * 48, 37)
+    q, q2 = (torch.randn((n, h, 128), generator=w.g, device=DEV).half() for n, h in ((2, 10), (300 * 48, 8)))
+    mass, ends = torch.zeros((2, 2, 600), device=DEV), i32([300 * i for i in range(49)])
+    calls = (lambda: w.cache.attend(q, max_seq_len=9000, page_mass=mass),
+             lambda: many.cache.attend(q2, max_seq_len=300, q_offsets=ends, max_q_per_seq=300))
+    eager = [c() for c in calls]
+    one = mass.clone()
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for c in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(c())
+        graphs.append(g)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for k in range(6):
+        for g, s in zip(graphs, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(eager, outs))
+    assert ((mass - 7 * one).abs() <= 7 * 2.0 ** -22 * 7 * one + 1e-30).all()     # seven passes, six fp32 additions
+
+
 def test_masses_of_a_long_context(native_lib):
     w = Large(Q8Layout(10, 2, 128, 16, "int8"), [20000, 777], 35)
     q = torch.randn((2, 10, 128), generator=w.g, device=DEV).half()
@@ -707,6 +735,7 @@ def test_ids_and_offsets_outside_the_pools_are_refused(native_lib):
     w.cache.block_tables.copy_(tables)
     got = w.cache.attend(q, max_seq_len=64, seq_lens=i32([40, -3, 40]))
     assert torch.equal(got[0], good[0]) and int(got[1].abs().max()) == 0
+    good = w.cache.attend(q, max_seq_len=64, seq_lens=lens, q_offsets=i32([0, 1, 2, 3]), max_q_per_seq=8)
     out = torch.full((3, 4, 64), 5.0, device=DEV)
     w.cache.attend(q, out, max_seq_len=64, seq_lens=lens, q_offsets=i32([0, 1, 9, 3]), max_q_per_seq=8)   # rows 1..8 of 3
     assert torch.equal(out[0], good[0]) and (out[1:] == 5.0).all()
