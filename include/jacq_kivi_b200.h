@@ -289,7 +289,7 @@ int kivi_b200_q8_cache_read(const kivi_q8_geometry* geom, const kivi_q8_cache* c
                             int batch, int total_rows, int max_rows_per_seq, kivi_f16* k_out, kivi_f16* v_out,
                             cudaStream_t stream);
 
-/* Bytes of workspace kivi_b200_q8_attention needs (0: none; also 0 for arguments it would refuse). */
+/* Bytes of workspace kivi_b200_q8_attention needs on the current device (0: none; also 0 for arguments it would refuse). */
 size_t kivi_b200_q8_attention_workspace_bytes(const kivi_q8_geometry* geom, int batch, int max_q_per_seq,
                                               int max_seq_len, int window, int sinks, int with_mass);
 
@@ -302,7 +302,10 @@ size_t kivi_b200_q8_attention_workspace_bytes(const kivi_q8_geometry* geom, int 
  * page_mass (or NULL) f32 [batch, NKV, mass_width], single-token calls only (q_offsets NULL): entry [i, h, p] grows by the
  * softmax weight that the query heads of kv head h gave the tokens of logical page p; mass_width * B >= max_seq_len.
  * Lengths are on the device: a longer one than max_seq_len counts as max_seq_len, a negative one as 0; page and slot
- * ids outside the pools are read as 0 and counted; a sequence whose q rows lie outside 0 .. total_q is skipped. */
+ * ids outside the pools are read as 0 and counted; a sequence whose q rows lie outside 0 .. total_q, or are more than
+ * max_q_per_seq, is skipped (its output rows are left) and counted.
+ * The workspace belongs to the call until it is done: calls that may run at the same time need one each. Results do not
+ * depend on what it holds, and for given sizes repeat bit for bit. */
 int kivi_b200_q8_attention(const kivi_q8_geometry* geom, const kivi_q8_cache* cache, const kivi_f16* q,
                            int64_t q_stride, const int32_t* q_offsets, int total_q, const int32_t* block_tables,
                            int max_blocks_per_seq, const int32_t* seq_lens, const int32_t* slot_ids, int batch,

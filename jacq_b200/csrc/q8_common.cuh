@@ -141,6 +141,7 @@ struct Unit {
     int seq, h, rb, len, n, row0, rows;
     View v;
     int items;          // tiles of the page part and of the tail
+    bool refused;       // its query rows do not lie inside the launch's
 };
 __device__ __forceinline__ Unit make_unit(const Q8AttnParams& p, int unit, int r_per_block) {
     Unit u;
@@ -149,10 +150,11 @@ __device__ __forceinline__ Unit make_unit(const Q8AttnParams& p, int unit, int r
     u.h = unit % p.cache.nkv; u.seq = unit / p.cache.nkv;
     u.len = min(max(p.seq.lens[u.seq], 0), p.max_seq);
     u.row0 = u.seq; u.n = 1;
+    u.refused = false;
     if (p.q_offsets) {
         u.row0 = p.q_offsets[u.seq];
-        u.n = min(p.q_offsets[u.seq + 1] - u.row0, p.max_q);
-        if (u.row0 < 0 || u.n < 0 || u.row0 > p.total_q - u.n) u.n = 0;
+        u.n = p.q_offsets[u.seq + 1] - u.row0;
+        if (u.row0 < 0 || u.n < 0 || u.n > p.max_q || u.row0 > p.total_q - u.n) { u.n = 0; u.refused = true; }
     }
     u.rows = u.n * p.qpk;
     const int first = u.rb * r_per_block, last = min(first + r_per_block, u.rows) - 1;

@@ -239,6 +239,20 @@ def test_attention_of_empty_and_unequal_sequences(fmt, native_lib):
     w.check_attention(max_seq_len=2015)    # a looser bound changes nothing but the launch
 
 
+def test_a_cache_without_a_page(native_lib):
+    """Nothing written yet, or fewer tokens than a page: tables may have no entry at all."""
+    layout = Q8Layout(4, 2, 64, 128, "int8")
+    w = World(layout, [0, 0], seed=23)
+    w.cache = Q8Cache(layout, 1, 2, 0, DEV)
+    assert int(w.attend(w.randn(2, 4, 64), max_seq_len=0).abs().max()) == 0
+    mass = torch.zeros((2, 2, 1), device=DEV)
+    w.attend(w.randn(2, 4, 64), max_seq_len=0, page_mass=mass)
+    assert int(mass.abs().max()) == 0
+    w.feed([5, 100])
+    w.check_attention()
+    w.check_attention([5, 40], window=3)
+
+
 @pytest.mark.parametrize("layout", LAYOUTS, ids=IDS)
 def test_attention_of_runs_of_tokens(layout, native_lib):
     b = layout.block_size
@@ -739,6 +753,11 @@ def test_ids_and_offsets_outside_the_pools_are_refused(native_lib):
     out = torch.full((3, 4, 64), 5.0, device=DEV)
     w.cache.attend(q, out, max_seq_len=64, seq_lens=lens, q_offsets=i32([0, 1, 9, 3]), max_q_per_seq=8)   # rows 1..8 of 3
     assert torch.equal(out[0], good[0]) and (out[1:] == 5.0).all()
+    torch.cuda.synchronize()
+    now = rejected_indices()
+    out.fill_(5.0)
+    w.cache.attend(q, out, max_seq_len=64, seq_lens=lens, q_offsets=i32([0, 3, 3, 3]), max_q_per_seq=2)   # three rows, two stated
+    assert (out == 5.0).all() and rejected_indices() == now + 1
 
 
 def test_python_refusals(native_lib):
