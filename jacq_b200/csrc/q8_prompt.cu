@@ -16,8 +16,8 @@
 // wait gave up counts itself, waits for its products and leaves.
 //
 // Measured: 8 x 1024 query tokens behind 8192, 32/8 heads, no window: 1.64 ms, 627 TFLOP/s (e4m3 647), 0.37 of a large
-// library product's rate; 2 x 1024 behind 6144, window 4096: 268 us, where 256 units on 148 multiprocessors leave a
-// quarter idle. A step takes 6300 cycles of which the products fill 2300: a tile's own chain (products, then 4100 cycles
+// library product's rate; 2 x 1024 behind 6144, window 4096: 268 us, where the second round of 256 units leaves
+// 40 of 148 multiprocessors idle. A step takes 6300 cycles of which the products fill 2300: a tile's own chain (products, then 4100 cycles
 // of softmax at a third of the exponential unit's rate, then products) is what bounds it. Steps of the softmax: two
 // passes with the maximum 312 us -> none, packed arithmetic, K's bias taken off the score 288 -> masks as values 278 ->
 // two tiles under one load of the keys 268. Two threads per row (274 us) and two CTAs of one tile (278) were no faster:
