@@ -827,10 +827,12 @@ void plan_parts(Plan& q, int d) {
 // Whether the kernel for many rows is the faster one. It takes 3.1, 3.8 and 4.6 us (head_dim 64, 128, 256) for 128 keys of
 // its 256 (128) rows on every multiprocessor; the other one 0.40, 0.60 and 1.3 ns for 16 keys of 16 rows. At head_dim
 // 128, 8 sequences of 8192 tokens, 8 kv heads: 128 rows each 276 us against 181, 256 rows 287 against 409, 512 rows
-// 282 against 766. Of 36 other calls between both kernels' ranges a margin of 1.1 on the model chooses two better than 1.25
-// (64: 5 x 99 tokens behind 29173, 3/36 heads, 603 us -> 527; 256: 28 x 46, 4/32 heads, 49 -> 42) and one worse (256:
-// 5 x 62 tokens, 2/16 heads, 18.7 -> 22.6). Two stay with the slower kernel: 64, 3 x 150 tokens behind 5163, 3/36 heads,
-// 182 us against 128; 256, 2 x 68 behind 6104, 8/40 heads, 256 against 210.
+// 282 against 766. Of 36 calls between both kernels' ranges a margin
+// of 1.1 on the model chose two better than 1.25 and one worse; over 36 others, drawn afterwards, it takes 1.5 % more
+// than the faster kernel of each call, 1.25 takes 3.1 %, always the one for few rows 15 %, always the other 27 %
+// (geometric means). It gains on long contexts (256, 2 x 123 tokens, window 1654, 8/32 heads: 117 us -> 80) and loses 1
+// to 6 us on small calls (128, 4 x 104 tokens, 2/14 heads: 18.5 -> 24.0). Known misses: 64, 3 x 150 tokens behind 5163,
+// 3/36 heads, 182 us against 128; 256, 2 x 68 behind 6104, 8/40 heads, 256 against 210.
 bool many_rows(int d, int batch, int nkv, long long rows, int tiles) {
     const int per = d == 256 ? 128 : 256;
     const double step_us = d == 64 ? 3.1 : d == 128 ? 3.8 : 4.6, tile_us = (d == 64 ? 0.40 : d == 128 ? 0.60 : 1.3) * 1e-3;
