@@ -75,14 +75,15 @@ __device__ __forceinline__ void store16(uint32_t at, const uint32_t (&v)[16]) {
         ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
           "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(at) : "memory");
 }
+// Load and wait in one statement: arithmetic on the registers cannot be moved between the two.
 __device__ __forceinline__ void load16(uint32_t at, uint32_t (&r)[16]) {
     __syncwarp();
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(at) : "memory");
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
 // 32 columns of the thread's row, in two halves: the registers are the caller's after await32 alone, which names them.
 __device__ __forceinline__ void request32(uint32_t at, uint32_t (&r)[32]) {
@@ -289,6 +290,9 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
                     const bool none = !__any_sync(0xffffffffu, top > m);
                     const float mn = fmaxf(m, ceilf(top)), a = fast_exp2(m - mn);
                     if (none) break;                    // nothing new to go by: NaN, or keys that nobody sees
+                    // P of this step's earlier chunks, and O if it was rescaled in this step, are on their way to tensor
+                    // memory: a load does not wait for an earlier store of the same columns by itself
+                    store_wait();
                     m = mn;
                     l *= a;
                     if (i > 0) rescale_o(a);

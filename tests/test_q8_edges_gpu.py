@@ -1,0 +1,59 @@
+"""The 8-bit cache's calls at their edges: masks, magnitudes, lengths and ids that the main tests do not combine."""
+import pytest
+import torch
+
+from jacq_b200.q8_cache import Q8Layout
+from tests import q8_oracle as qo
+from tests.test_q8_gpu import DEV, HALF, MANY, Large, i32, offsets_of
+
+pytestmark = pytest.mark.gpu
+
+MANY_IDS = [f"{x.num_q_heads}/{x.num_kv_heads}x{x.head_dim}b{x.block_size}{x.fmt}" for x, _, _ in MANY]
+
+
+class Prompts(Large):
+    """A batch large enough for the kernel for many rows, with chosen K and V instead of normal ones."""
+
+    def fill(self, k=None, v=None):
+        self.k, self.v = self.k if k is None else k.half(), self.v if v is None else v.half()
+        self.cache.seq_lens.zero_()
+        self.cache.write(self.k, self.v, i32(self.at), max_new_per_seq=max(self.lens), max_start_seq_len=0)
+        self.scales = [float(x) for x in self.cache.tensors.SCALES.nan_to_num().amax((0, 1))]
+
+    def positions(self):
+        return torch.cat([torch.arange(t, device=DEV) for t in self.lens])
+
+    def run(self, q, counts, half=True, **kw):
+        out = torch.full(q.shape, 9.0, dtype=torch.float16 if half else torch.float32, device=DEV)
+        self.cache.attend(q, out, max_seq_len=max(self.lens), q_offsets=i32(offsets_of(counts)), max_q_per_seq=max(counts), **kw)
+        return out
+
+    def compare(self, q, counts, window=0, sinks=0, half=True, products=1, some=None):
+        lay, at = self.layout, offsets_of(counts)
+        got = self.run(q, counts, half, window=window, sinks=sinks)
+        bias = 128.0 * self.scales[0] if products == 1 and lay.fmt == "int8" else 0.0
+        for i in range(len(counts)) if some is None else some:
+            want, bound = qo.attend_block(q[at[i]:at[i + 1]], *self.held(i), window, sinks, products, bias)
+            if half:
+                bound = bound + HALF * want.abs() + 2.0 ** -25
+            err = (got[at[i]:at[i + 1]].double() - want).abs()
+            assert (err <= bound).all(), (i, float((err - bound).max()), float(err.max()), (err > bound).nonzero()[:3].tolist())
+
+
+@pytest.mark.parametrize("layout,batch,longest", MANY, ids=MANY_IDS)
+def test_prompts_whose_scores_and_v_scales_rise_all_the_time(layout, batch, longest, native_lib):
+    """Every 32 keys the scores rise by 2.5 and every 16 the magnitude of V doubles (17 times, then again): the running
+    maximum and V's reference are raised several times within a step and from step to step."""
+    w = Prompts(layout, [longest - 3 * (i % 7) for i in range(batch)], 41)
+    d, pos = layout.head_dim, w.positions()
+    level = (pos // 32).float() * 2.5 / d ** 0.5
+    k = level[:, None, None] + 0.05 * torch.randn(w.k.shape, generator=w.g, device=DEV)
+    v = torch.randn(w.v.shape, generator=w.g, device=DEV) * torch.exp2((pos // 16 % 18).float() - 9.0)[:, None, None]
+    w.fill(k, v)
+    q = (1.0 + 0.05 * torch.randn((sum(w.lens), layout.num_q_heads, d), generator=w.g, device=DEV)).half()
+    some = [0, 1, 5, batch - 1]
+    for window, sinks, half in ((0, 0, True), (0, 0, False), (70, 3, True), (longest // 2, 40, False)):
+        w.compare(q, w.lens, window, sinks, half, some=some)
+    # and falling: the maximum is the first key's, V's reference the first page's
+    w.fill(k.flip(0), v.flip(0))
+    w.compare(q, w.lens, 0, 0, True, some=some)
