@@ -300,11 +300,10 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
                     for (int k = 0; k < c; ++k) {       // the chunks of P that are there already
                         uint32_t w[16];
                         load16(s_at + 16 * k, w);
-                        const __half2 aa = __float2half2_rn(a);
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&w[e]), aa);
-                            w[e] = *reinterpret_cast<const uint32_t*>(&h);
+                        for (int e = 0; e < 16; ++e) {   // in fp32: the factor alone may lie below fp16's range
+                            const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
+                            w[e] = pack_half2(h.x * a, h.y * a);
                         }
                         store16(s_at + 16 * k, w);
                     }

@@ -28,10 +28,9 @@ class Prompts(Large):
         self.cache.attend(q, out, max_seq_len=max(self.lens), q_offsets=i32(offsets_of(counts)), max_q_per_seq=max(counts), **kw)
         return out
 
-    def compare(self, q, counts, window=0, sinks=0, half=True, products=1, some=None):
-        lay, at = self.layout, offsets_of(counts)
+    def compare(self, q, counts, window=0, sinks=0, half=True, products=1, some=None, bias=0.0):
+        at = offsets_of(counts)
         got = self.run(q, counts, half, window=window, sinks=sinks)
-        bias = 128.0 * self.scales[0] if products == 1 and lay.fmt == "int8" else 0.0
         for i in range(len(counts)) if some is None else some:
             want, bound = qo.attend_block(q[at[i]:at[i + 1]], *self.held(i), window, sinks, products, bias)
             if half:
@@ -52,8 +51,25 @@ def test_prompts_whose_scores_and_v_scales_rise_all_the_time(layout, batch, long
     w.fill(k, v)
     q = (1.0 + 0.05 * torch.randn((sum(w.lens), layout.num_q_heads, d), generator=w.g, device=DEV)).half()
     some = [0, 1, 5, batch - 1]
+    bias = 128.0 * w.scales[0] if layout.fmt == "int8" else 0.0
     for window, sinks, half in ((0, 0, True), (0, 0, False), (70, 3, True), (longest // 2, 40, False)):
-        w.compare(q, w.lens, window, sinks, half, some=some)
+        w.compare(q, w.lens, window, sinks, half, some=some, bias=bias)
     # and falling: the maximum is the first key's, V's reference the first page's
     w.fill(k.flip(0), v.flip(0))
-    w.compare(q, w.lens, 0, 0, True, some=some)
+    w.compare(q, w.lens, 0, 0, True, some=some, bias=bias)
+
+
+@pytest.mark.parametrize("layout,batch,longest", MANY, ids=MANY_IDS)
+def test_probabilities_kept_over_a_large_rise_within_a_step(layout, batch, longest, native_lib):
+    """Keys 32 and 64 score 2^8 and 2^25 times the keys before them: what key 32 has left, 2^-17, is far above fp16's
+    range although the factor between the two maxima, 2^-25, is not. Key 64's V is 0 in every other channel."""
+    w = Prompts(layout, [longest] * batch, 43)
+    pos, d = w.positions(), layout.head_dim
+    level = torch.where(pos < 32, 0.5, -10.0)
+    level[pos == 32], level[pos == 64] = 8.5, 25.5
+    v = torch.randn(w.v.shape, generator=w.g, device=DEV)
+    v[pos == 64, :, ::2] = 0.0
+    w.fill((level / (d ** 0.5 * 1.4427))[:, None, None].expand_as(w.k).contiguous(), v)
+    q = torch.ones((sum(w.lens), layout.num_q_heads, d), dtype=torch.float16, device=DEV)
+    bias = 128.0 * w.scales[0] if layout.fmt == "int8" else 0.0
+    w.compare(q, w.lens, half=False, some=[0, batch - 1], bias=bias)
