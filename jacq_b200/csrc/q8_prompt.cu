@@ -19,7 +19,7 @@
 // library product's rate; 2 x 1024 behind 6144, window 4096: 268 us, where the second round of 256 units leaves
 // 40 of 148 multiprocessors idle. A step takes 6300 cycles of which the products fill 2300: a tile's own chain (products, then 4100 cycles
 // of softmax at a third of the exponential unit's rate, then products) is what bounds it. Steps of the softmax: two
-// passes with the maximum 312 us -> none, packed arithmetic, K's bias taken off the score 288 -> masks as values 278 ->
+// passes with the maximum 312 us -> none, packed arithmetic 288 -> masks as values 278 ->
 // two tiles under one load of the keys 268. Two threads per row (274 us) and two CTAs of one tile (278) were no faster:
 // with several roles' code in turn the instruction cache counts (the fully unrolled form took 343).
 // Probabilities are rounded to fp16 once: 1.41 times the plain form's error; a second product would lengthen the chain.
@@ -147,11 +147,11 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
     extern __shared__ unsigned char raw[];
     __shared__ uint64_t full_k[2], full_v[2], free_k[2], free_v[2], s_ready[2], p_ready[2], pv_done[2], drained;
     __shared__ uint32_t tmem_slot;
-    // Of the steps in flight, per 16-token tile: the factor of its scores, what the bias of int8 codes adds to them per sum
-    // of q, log2 of V's scale, the first key; per step: first and last key, the largest log2 of V's scale.
+    // Of the steps in flight, per 16-token tile: the factor of its scores, log2 of V's scale, the first key; per step: first
+    // and last key, the largest log2 of V's scale.
     // Four of them: K of step i is written when the products with K of step i - 2 are done, while the softmax may
     // still be at step i - 2; it is not at step i - 4, whose probabilities those products' order has waited for.
-    __shared__ float meta_f[4][8], meta_bias[4][8], meta_lv[4][8], step_lv[4];
+    __shared__ float meta_f[4][8], meta_lv[4][8], step_lv[4];
     __shared__ int meta_key0[4][8], step_key0[4], step_key1[4];
     __shared__ int odd_v, odd_page;        // a tail row held an infinity or NaN in V; a page's scale is NaN
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -209,18 +209,6 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
         if (t_mine < tiles) {
         const uint32_t mine = (uint32_t)((warp & 3) * 32) << 16;   // this warp's lanes of tensor memory
         const uint32_t s_at = tmem_s(t_mine) + mine, o_at = tmem_o(t_mine) + mine;
-        float qsum = 0.0f;
-        if (FMT == KIVI_Q8_INT8) {
-            for (int j = 0; j < D / 8; ++j) {
-                const uint4 x = lds128(smem + t_mine * TILE + chunk_at(tid & 127, j));
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const float2 y = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
-                    qsum += y.x + y.y;
-                }
-            }
-        }
         // P = 2^(s f - m) is kept below 2^8 by raising m when a sum says that it may not be: no pass over S for its maximum.
         // In fp16 it carries V's scale relative to 2^vref, an exponent not below any scale's met so far, and 2^6.
         // kQ8Unset: the row has met no key yet.
@@ -262,8 +250,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
                     const float base = vref - kHeadroomLog + (m == kQ8Unset ? 0.0f : m);
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
-                        const float lw = meta_lv[b][2 * c + half], add = fmaf(-qsum, meta_bias[b][2 * c + half], lw - base);
-                        const float f = meta_f[b][2 * c + half];
+                        const float lw = meta_lv[b][2 * c + half], add = lw - base, f = meta_f[b][2 * c + half];
                         const uint64_t ff = pack2(f, f), aa = pack2(add, add);
                         uint64_t acc = pack2(0.0f, 0.0f);
 #pragma unroll
@@ -284,8 +271,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
                     float top = -INFINITY;
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
-                        if (__uint_as_float(s[e]) != kMasked)
-                            top = fmaxf(top, fmaf(__uint_as_float(s[e]), meta_f[b][2 * c + (e >> 4)], -qsum * meta_bias[b][2 * c + (e >> 4)]));
+                        if (__uint_as_float(s[e]) != kMasked) top = fmaxf(top, __uint_as_float(s[e]) * meta_f[b][2 * c + (e >> 4)]);
                     // whole numbers: the factor is a power of two, and what is there already is not rounded again
                     const bool none = !__any_sync(0xffffffffu, top > m);
                     const float mn = fmaxf(m, ceilf(top)), a = fast_exp2(m - mn);
@@ -403,7 +389,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
         for (int i = 0; i < steps && !failed; ++i) {
             const int first = 8 * i, b = i & 3, stage = i % STAGES;
             const int paged = min(8, max(0, v.tiles - first)), there = min(8, u.items - first);   // tiles of pages; of any kind
-            float f = 1.0f, bias = 0.0f, lv = -1000.0f;
+            float f = 1.0f, lv = -1000.0f;
             int key0 = 0x3fffffff;                       // a tile that is not there: no row sees that far
             if (c < paged) {
                 float2 sc = p.cache.scales[(size_t)id * nkv + u.h];
@@ -412,7 +398,6 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
                 f = (sc.x == 0.0f ? 1.0f : sc.x) * p.scale_log2;
                 lv = sc.y == 0.0f ? -1000.0f : log2f(sc.y);
                 key0 = tile_of(first + lane) * 16;
-                if (FMT == KIVI_Q8_INT8) { bias = 128.0f * f; f *= 16777216.0f; }
             } else if (c < there) {
                 f = p.scale_log2; lv = 0.0f;
                 key0 = v.paged + (first + c - v.tiles) * 16;
@@ -436,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
                         k1 = max(k1, __shfl_xor_sync(0xffffffffu, k1, z));
                     }
                     if (c < 8) {
-                        meta_f[b][c] = f; meta_bias[b][c] = bias; meta_key0[b][c] = key0;
+                        meta_f[b][c] = f; meta_key0[b][c] = key0;
                         meta_lv[b][c] = lv == -1000.0f ? fmaxf(lv_top, -100.0f) : lv;
                     }
                     if (c == 0) { step_lv[b] = fmaxf(lv_top, -100.0f); step_key0[b] = k0; step_key1[b] = k1; }
@@ -449,17 +434,8 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
                     const uint4 y = x[which][k];
                     const uint32_t w[4] = {flip ? y.z : y.x, flip ? y.w : y.y, flip ? y.x : y.z, flip ? y.y : y.w};
                     uint4 a, z;
-                    if (FMT == KIVI_Q8_INT8 && which == 0) {
-                        // K: a byte alone is a subnormal, (code + 128) 2^-24 exactly; the softmax takes the bias off the score
-                        const uint32_t h = 0x80808080u;
-                        a = make_uint4(__byte_perm(w[0] ^ h, 0u, 0x4140), __byte_perm(w[0] ^ h, 0u, 0x4342), __byte_perm(w[1] ^ h, 0u, 0x4140),
-                                       __byte_perm(w[1] ^ h, 0u, 0x4342));
-                        z = make_uint4(__byte_perm(w[2] ^ h, 0u, 0x4140), __byte_perm(w[2] ^ h, 0u, 0x4342), __byte_perm(w[3] ^ h, 0u, 0x4140),
-                                       __byte_perm(w[3] ^ h, 0u, 0x4342));
-                    } else {
-                        q8_unpack<FMT>(w[0], a.x, a.y); q8_unpack<FMT>(w[1], a.z, a.w);
-                        q8_unpack<FMT>(w[2], z.x, z.y); q8_unpack<FMT>(w[3], z.z, z.w);
-                    }
+                    q8_unpack<FMT>(w[0], a.x, a.y); q8_unpack<FMT>(w[1], a.z, a.w);
+                    q8_unpack<FMT>(w[2], z.x, z.y); q8_unpack<FMT>(w[3], z.z, z.w);
                     sts128(dst + chunk_at(row, 2 * chunk + (flip ? 1 : 0)), a);
                     sts128(dst + chunk_at(row, 2 * chunk + (flip ? 0 : 1)), z);
                 }

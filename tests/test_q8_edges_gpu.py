@@ -28,11 +28,11 @@ class Prompts(Large):
         self.cache.attend(q, out, max_seq_len=max(self.lens), q_offsets=i32(offsets_of(counts)), max_q_per_seq=max(counts), **kw)
         return out
 
-    def compare(self, q, counts, window=0, sinks=0, half=True, products=1, some=None, bias=0.0):
+    def compare(self, q, counts, window=0, sinks=0, half=True, products=1, some=None):
         at = offsets_of(counts)
         got = self.run(q, counts, half, window=window, sinks=sinks)
         for i in range(len(counts)) if some is None else some:
-            want, bound = qo.attend_block(q[at[i]:at[i + 1]], *self.held(i), window, sinks, products, bias)
+            want, bound = qo.attend_block(q[at[i]:at[i + 1]], *self.held(i), window, sinks, products)
             if half:
                 bound = bound + HALF * want.abs() + 2.0 ** -25
             err = (got[at[i]:at[i + 1]].double() - want).abs()
@@ -51,12 +51,11 @@ def test_prompts_whose_scores_and_v_scales_rise_all_the_time(layout, batch, long
     w.fill(k, v)
     q = (1.0 + 0.05 * torch.randn((sum(w.lens), layout.num_q_heads, d), generator=w.g, device=DEV)).half()
     some = [0, 1, 5, batch - 1]
-    bias = 128.0 * w.scales[0] if layout.fmt == "int8" else 0.0
     for window, sinks, half in ((0, 0, True), (0, 0, False), (70, 3, True), (longest // 2, 40, False)):
-        w.compare(q, w.lens, window, sinks, half, some=some, bias=bias)
+        w.compare(q, w.lens, window, sinks, half, some=some)
     # and falling: the maximum is the first key's, V's reference the first page's
     w.fill(k.flip(0), v.flip(0))
-    w.compare(q, w.lens, 0, 0, True, some=some, bias=bias)
+    w.compare(q, w.lens, 0, 0, True, some=some)
 
 
 @pytest.mark.parametrize("layout,batch,longest", MANY, ids=MANY_IDS)
@@ -71,5 +70,22 @@ def test_probabilities_kept_over_a_large_rise_within_a_step(layout, batch, longe
     v[pos == 64, :, ::2] = 0.0
     w.fill((level / (d ** 0.5 * 1.4427))[:, None, None].expand_as(w.k).contiguous(), v)
     q = torch.ones((sum(w.lens), layout.num_q_heads, d), dtype=torch.float16, device=DEV)
-    bias = 128.0 * w.scales[0] if layout.fmt == "int8" else 0.0
-    w.compare(q, w.lens, half=False, some=[0, batch - 1], bias=bias)
+    w.compare(q, w.lens, half=False, some=[0, batch - 1])
+
+
+@pytest.mark.parametrize("layout,batch,longest", [m for m in MANY if m[0].fmt == "int8"], ids=[x for x, m in zip(MANY_IDS, MANY) if m[0].fmt == "int8"])
+def test_prompts_with_a_loud_key_channel_and_pages_of_zero_keys(layout, batch, longest, native_lib):
+    """A channel that q does not look at sets K's scale, so that a page's other codes are a few steps of it, and all of q
+    has one sign: a score is a small sum whatever 128 sum|q| is. Every third page's K is all zero: scores exactly 0."""
+    w = Prompts(layout, [longest] * batch, 42)
+    k = torch.randn(w.k.shape, generator=w.g, device=DEV)
+    k[..., 0] = 200.0
+    page = w.positions() // layout.block_size
+    k[page % 3 == 2] = 0.0
+    w.fill(k)
+    q = 20.0 + torch.randn((sum(w.lens), layout.num_q_heads, layout.head_dim), generator=w.g, device=DEV)
+    q[..., 0] = 0.0
+    some = [0, batch - 1]
+    w.compare(q.half(), w.lens, some=some)
+    w.compare(q.half(), w.lens, window=40, sinks=3, half=False, some=some)
+    w.compare((q * 8.0).half(), w.lens, half=False, some=some)
