@@ -6,12 +6,13 @@
 // are seen. Per tile of rows:
 //
 //   S[128 x 128] = Q Kc^T     operands in shared memory, accumulator in tensor memory
-//   P = 2^(S f - m) vs'       four warps, a thread per row: no shuffles; P goes back to tensor memory, over S
-//   O[128 x D]  += P Vc       P from tensor memory, Vc from shared memory with the channels as its leading dimension
+//   P = 2^(S f - m) vs'       four warps, a thread per row: no shuffles; P goes back to tensor memory, over S, as two fp16
+//                             numbers (22 bits, as in the kernel for few rows)
+//   O[128 x D]  += P Vc       two products: P from tensor memory, Vc from shared memory, channels as its leading dimension
 //
 // Work is split by warps: 0 .. 3 and 4 .. 7 softmax and epilogue of the two tiles, 8 .. 11 load codes and write them as
 // fp16 into the swizzled tiles (once for both), one thread of warp 12 issues the products. At 256 rows a byte of codes is
-// worth 512 flops, so the tensor pipe (2 * 4 * 128 * 128 * D flops a step) and the exponentials (2 * 128 * 128, 16 a
+// worth 512 flops, so the tensor pipe (2 * 6 * 128 * 128 * D flops a step) and the exponentials (2 * 128 * 128, 16 a
 // cycle) bound it, not HBM; one tile's products run under the other's exponentials. Every wait is bounded: a CTA whose
 // wait gave up counts itself, waits for its products and leaves.
 //
@@ -22,7 +23,8 @@
 // passes with the maximum 312 us -> none, packed arithmetic 288 -> masks as values 278 ->
 // two tiles under one load of the keys 268. Two threads per row (274 us) and two CTAs of one tile (278) were no faster:
 // with several roles' code in turn the instruction cache counts (the fully unrolled form took 343).
-// Probabilities are rounded to fp16 once: 1.41 times the plain form's error; a second product would lengthen the chain.
+// The second half of P: 274 us without it, 321 with it while the next 32 scores were fetched under the present ones (84 to
+// 108 bytes of spills a thread, twice the code in the loop), 267 since scores are fetched when they are due.
 #include "q8_common.cuh"
 
 namespace kivi {
@@ -75,7 +77,7 @@ __device__ __forceinline__ void store16(uint32_t at, const uint32_t (&v)[16]) {
         ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
           "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(at) : "memory");
 }
-// Load and wait in one statement: arithmetic on the registers cannot be moved between the two.
+// Loads wait in the same statement: nothing that uses the registers can be moved between the two.
 __device__ __forceinline__ void load16(uint32_t at, uint32_t (&r)[16]) {
     __syncwarp();
     asm volatile(
@@ -85,24 +87,17 @@ __device__ __forceinline__ void load16(uint32_t at, uint32_t (&r)[16]) {
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(at) : "memory");
 }
-// 32 columns of the thread's row, in two halves: the registers are the caller's after await32 alone, which names them.
-__device__ __forceinline__ void request32(uint32_t at, uint32_t (&r)[32]) {
+__device__ __forceinline__ void load32(uint32_t at, uint32_t (&r)[32]) {
     __syncwarp();
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
           "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
           "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(at) : "memory");
-}
-__device__ __forceinline__ void await32(uint32_t (&r)[32]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
-                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]),
-                   "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]),
-                   "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31]) :: "memory");
 }
 // two fp32 values in one instruction
 __device__ __forceinline__ uint64_t pack2(float x, float y) {
@@ -120,6 +115,14 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+// What fp16 leaves of two values: x - h.x, y - h.y (exact in fp32), packed.
+__device__ __forceinline__ uint32_t rest2(float x, float y, uint32_t h) {
+    const unsigned short minus = 0xBC00;
+    float lo, hi;
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tfma.rn.f32.f16 %0, a, %5, %3;\n\tfma.rn.f32.f16 %1, b, %5, %4;\n\t}"
+        : "=f"(lo), "=f"(hi) : "r"(h), "f"(x), "f"(y), "h"(minus));
+    return pack_half2(lo, hi);
 }
 __device__ __forceinline__ void store_wait() { __syncwarp(); asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void sts128(uint32_t at, uint4 v) {
@@ -238,12 +241,15 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
             }
             // 32 keys: scores to probabilities. What is rare is kept out of the way: this code is run over and over beside
             // two other roles' and its length counted more than its instructions.
-            auto chunk = [&](uint32_t (&s)[32], int c) {
+            auto hide = [&](uint32_t (&s)[32], int c) {
                 if (__builtin_expect(masked, 0)) {
 #pragma unroll
                     for (int e = 0; e < 32; ++e) if (!sees(meta_key0[b][2 * c + (e >> 4)] + (e & 15))) s[e] = __float_as_uint(kMasked);
                 }
-                uint32_t out[16];
+            };
+            auto chunk = [&](uint32_t (&s)[32], int c) {
+                hide(s, c);
+                uint32_t out[16], rest[16];
                 float sum;
                 while (true) {
                     sum = 0.0f;
@@ -261,6 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
                             y = fast_exp2(y);
                             acc = add2(acc, pack2(x, y));
                             out[e / 2] = pack_half2(x, y);
+                            rest[e / 2] = rest2(x, y, out[e / 2]);   // takes the place of the scores, which are in tensor memory still
                         }
                         float x, y;
                         unpack2(acc, x, y);
@@ -268,6 +275,8 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
                     }
                     if (__builtin_expect(!__any_sync(0xffffffffu, !(sum <= 256.0f) || m == kQ8Unset), 1)) break;
                     // the first keys of a row, or scores far above all before them
+                    load32(s_at + 32 * c, s);
+                    hide(s, c);
                     float top = -INFINITY;
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
@@ -284,29 +293,30 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
                     if (i > 0) rescale_o(a);
 #pragma unroll 1
                     for (int k = 0; k < c; ++k) {       // the chunks of P that are there already
-                        uint32_t w[16];
-                        load16(s_at + 16 * k, w);
+                        uint32_t w[16], z[16];
+                        load16(s_at + 32 * k, w);
+                        load16(s_at + 32 * k + 16, z);
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {   // in fp32: the factor alone may lie below fp16's range
                             const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&w[e]));
-                            w[e] = pack_half2(h.x * a, h.y * a);
+                            const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&z[e]));
+                            const float x = (h.x + g.x) * a, y = (h.y + g.y) * a;
+                            w[e] = pack_half2(x, y);
+                            z[e] = rest2(x, y, w[e]);
                         }
-                        store16(s_at + 16 * k, w);
+                        store16(s_at + 32 * k, w);
+                        store16(s_at + 32 * k + 16, z);
                     }
                 }
                 l += sum;
-                store16(s_at + 16 * c, out);            // P over columns of S that have been read
+                store16(s_at + 32 * c, out);            // P in the place of the scores it came from
+                store16(s_at + 32 * c + 16, rest);
             };
-            uint32_t s0[32], s1[32];
-            request32(s_at, s0);
 #pragma unroll 1
-            for (int c = 0; c < 4; c += 2) {
-                await32(s0);
-                request32(s_at + 32 * (c + 1), s1);
-                chunk(s0, c);
-                await32(s1);
-                if (c == 0) request32(s_at + 64, s0);
-                chunk(s1, c + 1);
+            for (int c = 0; c < 4; ++c) {
+                uint32_t x[32];
+                load32(s_at + 32 * c, x);
+                chunk(x, c);
             }
             store_wait();
             fence_before();
@@ -495,8 +505,11 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
                 fence_after();
                 const uint32_t v_at = v_tile + (i % STAGES) * TILE;
 #pragma unroll
-                for (int k = 0; k < kKeys / 16; ++k)   // 16 keys: 8 columns of P, 16 rows of V
-                    product_ts(tmem_o(t), tmem_s(t) + 8 * k, operand(v_at + 2048 * k, kAtom), pv, i > 0 || k > 0);
+                for (int k = 0; k < kKeys / 16; ++k) {   // 16 keys: 8 columns of P, 8 of what fp16 left of it, 16 rows of V
+                    const uint32_t p_at = tmem_s(t) + 32 * (k >> 1) + 8 * (k & 1);
+                    product_ts(tmem_o(t), p_at, operand(v_at + 2048 * k, kAtom), pv, i > 0 || k > 0);
+                    product_ts(tmem_o(t), p_at + 16, operand(v_at + 2048 * k, kAtom), pv, 1);
+                }
                 commit(&pv_done[t]);
                 if (t == tiles - 1) commit(&free_v[i % STAGES]);
                 if (i + 1 == steps) continue;

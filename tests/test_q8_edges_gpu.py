@@ -28,7 +28,7 @@ class Prompts(Large):
         self.cache.attend(q, out, max_seq_len=max(self.lens), q_offsets=i32(offsets_of(counts)), max_q_per_seq=max(counts), **kw)
         return out
 
-    def compare(self, q, counts, window=0, sinks=0, half=True, products=1, some=None):
+    def compare(self, q, counts, window=0, sinks=0, half=True, products=2, some=None):
         at = offsets_of(counts)
         got = self.run(q, counts, half, window=window, sinks=sinks)
         for i in range(len(counts)) if some is None else some:
@@ -89,3 +89,12 @@ def test_prompts_with_a_loud_key_channel_and_pages_of_zero_keys(layout, batch, l
     w.compare(q.half(), w.lens, some=some)
     w.compare(q.half(), w.lens, window=40, sinks=3, half=False, some=some)
     w.compare((q * 8.0).half(), w.lens, half=False, some=some)
+
+
+@pytest.mark.parametrize("layout,batch,longest", MANY, ids=MANY_IDS)
+def test_prompts_are_as_exact_as_single_tokens(layout, batch, longest, native_lib):
+    """Probabilities to 22 bits whichever kernel runs: fp32 outputs within the bound of two fp16 numbers each."""
+    w = Prompts(layout, [longest - 2 * (i % 5) for i in range(batch)], 44)
+    q = torch.randn((sum(w.lens), layout.num_q_heads, layout.head_dim), generator=w.g, device=DEV).half()
+    for window, sinks, half in ((0, 0, False), (0, 0, True), (90, 5, False)):
+        w.compare(q, w.lens, window, sinks, half, some=[0, 3, batch - 1])
