@@ -157,6 +157,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
     __shared__ float meta_f[4][8], meta_lv[4][8], step_lv[4];
     __shared__ int meta_key0[4][8], step_key0[4], step_key1[4];
     __shared__ int odd_v, odd_page;        // a tail row held an infinity or NaN in V; a page's scale is NaN
+    __shared__ uint32_t tail_top[4];       // largest finite magnitude in the tail's V, per loading warp
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int nkv = p.cache.nkv, block = 1 << p.cache.log2b;
     // the last rows first: without a window they have the most keys
@@ -395,6 +396,33 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
         int id = load_id(0), id_next = load_id(1);
         uint32_t start = start_of(id, 0);
         if (AHEAD) { fetch(0, 0, start); fetch(1, 0, start); }
+        // The tail's V enters as a page's does: times a power of two that brings its largest value to 2^7 .. 2^8, whose log2
+        // takes the place of the scale's. As it is, with scale 1, it would push the probabilities of pages of small values
+        // in the same step below fp16's range.
+        float tail_lv = -1000.0f, tail_mul = 1.0f;
+        if (v.tail_tiles) {
+            const __half* tail = p.cache.v_tail + ((size_t)slot * nkv + u.h) * block * D;
+            uint32_t top = 0;
+            for (int e = c; e < (v.end - v.paged) * (D / 8); e += 128) {
+                if (unseen(v.paged + e / (D / 8))) continue;
+                const uint4 y = *reinterpret_cast<const uint4*>(tail + (size_t)e * 8);
+                const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint32_t lo = w[k] & 0x7fffu, hi = w[k] >> 16 & 0x7fffu;
+                    if (lo < 0x7c00u) top = max(top, lo);
+                    if (hi < 0x7c00u) top = max(top, hi);
+                }
+            }
+            top = __reduce_max_sync(0xffffffffu, top);
+            if (lane == 0) tail_top[warp - 8] = top;
+            asm volatile("bar.sync 1, 128;" ::: "memory");   // the loading warps
+            top = max(max(tail_top[0], tail_top[1]), max(tail_top[2], tail_top[3]));
+            if (top) {
+                tail_lv = (float)(ilogbf(__half2float(__ushort_as_half((unsigned short)top))) - 7);
+                tail_mul = exp2f(-tail_lv);
+            }
+        }
 #pragma unroll 1
         for (int i = 0; i < steps && !failed; ++i) {
             const int first = 8 * i, b = i & 3, stage = i % STAGES;
@@ -409,7 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
                 lv = sc.y == 0.0f ? -1000.0f : log2f(sc.y);
                 key0 = tile_of(first + lane) * 16;
             } else if (c < there) {
-                f = p.scale_log2; lv = 0.0f;
+                f = p.scale_log2; lv = tail_lv;
                 key0 = v.paged + (first + c - v.tiles) * 16;
             }
             const uint32_t start_now = start;
@@ -467,6 +495,8 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
                                 if (odd_half(w[z])) odd_v = 1;
                                 if ((w[z] & 0x7c00u) == 0x7c00u) w[z] &= 0xffff0000u;
                                 if ((w[z] & 0x7c000000u) == 0x7c000000u) w[z] &= 0x0000ffffu;
+                                const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&w[z]));
+                                w[z] = pack_half2(x.x * tail_mul, x.y * tail_mul);
                             }
                         }
                         sts128(dst + chunk_at(row, 2 * chunk), make_uint4(w[0], w[1], w[2], w[3]));

@@ -98,3 +98,18 @@ def test_prompts_are_as_exact_as_single_tokens(layout, batch, longest, native_li
     q = torch.randn((sum(w.lens), layout.num_q_heads, layout.head_dim), generator=w.g, device=DEV).half()
     for window, sinks, half in ((0, 0, False), (0, 0, True), (90, 5, False)):
         w.compare(q, w.lens, window, sinks, half, some=[0, 3, batch - 1])
+
+
+@pytest.mark.parametrize("layout,batch,longest", MANY, ids=MANY_IDS)
+@pytest.mark.parametrize("power", [-14, -10, 12])
+def test_prompts_with_a_tail_beside_pages_of_any_magnitude(layout, batch, longest, power, native_lib):
+    """V of magnitude 2^-14 to 2^12, alike in pages and tail rows, then a tail that is 2^6 above or below its pages."""
+    w = Prompts(layout, [longest - 1 - 2 * (i % 6) for i in range(batch)], 45)
+    lens, b = torch.tensor(w.lens, device=DEV), layout.block_size
+    v = torch.randn(w.v.shape, generator=w.g, device=DEV)
+    in_tail = w.positions() >= (lens // b * b).repeat_interleave(lens)
+    q = torch.randn((sum(w.lens), layout.num_q_heads, layout.head_dim), generator=w.g, device=DEV).half()
+    for more in (0, 6, -6) if power < 0 else (0, -6):
+        w.fill(v=v * 2.0 ** power * torch.where(in_tail, 2.0 ** more, 1.0)[:, None, None])
+        w.compare(q, w.lens, 0, 0, False, some=[0, 2, batch - 1])
+        w.compare(q, w.lens, 50, 3, True, some=[1])
