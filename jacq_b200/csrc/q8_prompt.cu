@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
         const uint32_t mine = (uint32_t)((warp & 3) * 32) << 16;   // this warp's lanes of tensor memory
         const uint32_t s_at = tmem_s(t_mine) + mine, o_at = tmem_o(t_mine) + mine;
         // P = 2^(s f - m) is kept below 2^8 by raising m when a sum says that it may not be: no pass over S for its maximum.
-        // In fp16 it carries V's scale relative to 2^vref, an exponent not below any scale's met so far, and 2^6.
+        // In fp16 it carries V's scale relative to 2^vref, an exponent not below any scale's that the row has met, and 2^6.
         // kQ8Unset: the row has met no key yet.
         float m = hi < 0 ? 0.0f : kQ8Unset, l = 0.0f, vref = -1000.0f;
         auto rescale_o = [&](float a) {
@@ -234,9 +234,17 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
             fence_after();
             const int key0 = step_key0[b], key1 = step_key1[b];
             const bool masked = __any_sync(0xffffffffu, key1 > hi || (key0 < lo && key1 >= p.sinks));
-            const float lv = step_lv[b];
-            if (__builtin_expect(lv > vref, 0)) {   // uniform; O of the step before is complete, as S of this one is there
-                const float next = floorf(lv) + 1.0f;
+            float lv = step_lv[b];
+            if (__builtin_expect(masked, 0)) {      // of the tiles that this row sees
+                lv = -1000.0f;
+#pragma unroll 1
+                for (int z = 0; z < 8; ++z) {
+                    const int k0 = meta_key0[b][z];
+                    if (k0 <= hi && (k0 + 15 >= lo || k0 < p.sinks)) lv = fmaxf(lv, meta_lv[b][z]);
+                }
+            }
+            if (__builtin_expect(__any_sync(0xffffffffu, lv > vref), 0)) {   // O of the step before is complete, as S of this one is there
+                const float next = lv > vref ? floorf(lv) + 1.0f : vref;
                 if (i > 0) rescale_o(fast_exp2(vref - next));
                 vref = next;
             }

@@ -113,3 +113,16 @@ def test_prompts_with_a_tail_beside_pages_of_any_magnitude(layout, batch, longes
         w.fill(v=v * 2.0 ** power * torch.where(in_tail, 2.0 ** more, 1.0)[:, None, None])
         w.compare(q, w.lens, 0, 0, False, some=[0, 2, batch - 1])
         w.compare(q, w.lens, 50, 3, True, some=[1])
+
+
+@pytest.mark.parametrize("layout,batch,longest", MANY, ids=MANY_IDS)
+def test_prompt_rows_are_not_touched_by_the_v_scales_of_keys_they_do_not_see(layout, batch, longest, native_lib):
+    """V grows by 2^18 from one token on: rows before it, and rows whose window has left the large ones behind."""
+    w = Prompts(layout, [longest - i % 3 for i in range(batch)], 46)
+    q = torch.randn((sum(w.lens), layout.num_q_heads, layout.head_dim), generator=w.g, device=DEV).half()
+    v, pos = torch.randn(w.v.shape, generator=w.g, device=DEV), w.positions()
+    b = layout.block_size
+    for large in (pos >= 2 * b, (pos < b) | (pos >= 3 * b), pos // b == 1):
+        w.fill(v=v * torch.where(large, 2.0 ** 6, 2.0 ** -12)[:, None, None])
+        w.compare(q, w.lens, 0, 0, False, some=[0, batch - 1])
+        w.compare(q, w.lens, b + 5, 2, False, some=[0, 2])
