@@ -31,7 +31,7 @@ namespace kivi {
 namespace {
 
 constexpr int kRows = 128, kKeys = 128, kThreads = 416;
-constexpr float kMasked = -3.0e38f;    // score of a masked key, before its factor: 2^(factor * this) is 0 for every scale
+constexpr float kMasked = -3.0e38f;    // score of a masked key, before its factor: 2^(factor * this) is 0 for factors of 1e-30 and more
 constexpr float kHeadroomLog = 6.0f;   // log2(kQ8Headroom)
 constexpr int kAtom = 128 * 128;   // bytes of 128 rows of 64 fp16 values, 128-byte swizzled
 
@@ -440,12 +440,12 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
             if (c < paged) {
                 float2 sc = p.cache.scales[(size_t)id * nkv + u.h];
                 if (!(sc.x + sc.y == sc.x + sc.y)) { odd_page = 1; sc = make_float2(1.0f, 0.0f); }   // seen to at the end
-                // a zero scale's codes are zeros too: any other does
-                f = (sc.x == 0.0f ? 1.0f : sc.x) * p.scale_log2;
+                // a sum of products is below 2^33: times a factor as small as this it is 0, and kMasked times it still masks
+                f = fmaxf(sc.x * p.scale_log2, 1e-30f);
                 lv = sc.y == 0.0f ? -1000.0f : log2f(sc.y);
                 key0 = tile_of(first + lane) * 16;
             } else if (c < there) {
-                f = p.scale_log2; lv = tail_lv;
+                f = fmaxf(p.scale_log2, 1e-30f); lv = tail_lv;
                 key0 = v.paged + (first + c - v.tiles) * 16;
             }
             const uint32_t start_now = start;

@@ -126,3 +126,18 @@ def test_prompt_rows_are_not_touched_by_the_v_scales_of_keys_they_do_not_see(lay
         w.fill(v=v * torch.where(large, 2.0 ** 6, 2.0 ** -12)[:, None, None])
         w.compare(q, w.lens, 0, 0, False, some=[0, batch - 1])
         w.compare(q, w.lens, b + 5, 2, False, some=[0, 2])
+
+
+@pytest.mark.parametrize("layout,batch,longest", MANY, ids=MANY_IDS)
+@pytest.mark.parametrize("scale", [1e-38, 1e-33])
+def test_prompts_stay_masked_under_the_smallest_scales(layout, batch, longest, scale, native_lib):
+    """All scores are 0 to working precision: a row is the mean of the values that it sees, and of no other."""
+    w = Prompts(layout, [longest] * batch, 47)
+    q = torch.randn((sum(w.lens), layout.num_q_heads, layout.head_dim), generator=w.g, device=DEV).half()
+    got = w.run(q, w.lens, half=False, scale=scale)[:longest].double()
+    v, per = w.held(0)[1], layout.num_q_heads // layout.num_kv_heads
+    count = torch.arange(1, longest + 1, device=DEV)[:, None, None]
+    want = (v.cumsum(0) / count).repeat_interleave(per, 1)
+    # 2^-22 of each probability and 2^-18 for the sums, as in the oracle's bound
+    bound = 2.0 ** -17 * (v.abs().cumsum(0) / count).repeat_interleave(per, 1) + longest * 2.0 ** -30 * v.abs().max()
+    assert ((got - want).abs() <= bound).all()
