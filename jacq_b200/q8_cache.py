@@ -317,11 +317,20 @@ class Q8Cache:
     def evict(self, page_mass: torch.Tensor, *, budget: int, first: int = 0, recent: int = 0, max_seq_len: int,
               install: bool = True) -> Q8Eviction:
         """``evict_pages`` on this cache's tables and lengths (one row per slot); with ``install`` the results replace
-        them, and ``page_mass`` is updated in place. The pages named in ``freed`` belong to nobody afterwards."""
+        them, and ``page_mass`` is updated in place. The pages named in ``freed`` belong to nobody afterwards.
+
+        The installed tables keep the ids that were entered for the open block and for growth: they move up behind the
+        kept pages. The columns that this empties hold -1, so a block that would complete there is refused and counted
+        until the caller enters a page (``Q8Eviction.block_tables`` has 0 behind the kept pages)."""
         r = evict_pages(self.block_tables, self.seq_lens, page_mass, block_size=self.layout.block_size, budget=budget, first=first,
                         recent=recent, max_seq_len=max_seq_len)
         if install:
-            self.block_tables.copy_(r.block_tables)
+            block, width = self.layout.block_size, self.max_blocks_per_seq
+            kept = (r.seq_lens // block)[:, None]
+            column = torch.arange(width, dtype=torch.int32, device=self.device)
+            source = column + (self.seq_lens // block)[:, None] - kept
+            behind = self.block_tables.gather(1, source.clamp(0, max(width - 1, 0)).long()).masked_fill_(source >= width, -1)
+            self.block_tables.copy_(torch.where(column < kept, r.block_tables, behind))
             self.seq_lens.copy_(r.seq_lens)
             page_mass.copy_(r.page_mass)
         return r

@@ -2,9 +2,9 @@
 import pytest
 import torch
 
-from jacq_b200.q8_cache import Q8Layout
+from jacq_b200.q8_cache import Q8Layout, rejected_indices
 from tests import q8_oracle as qo
-from tests.test_q8_gpu import DEV, HALF, MANY, Large, i32, offsets_of
+from tests.test_q8_gpu import DEV, HALF, MANY, Large, World, i32, offsets_of
 
 pytestmark = pytest.mark.gpu
 
@@ -141,3 +141,53 @@ def test_prompts_stay_masked_under_the_smallest_scales(layout, batch, longest, s
     # 2^-22 of each probability and 2^-18 for the sums, as in the oracle's bound
     bound = 2.0 ** -17 * (v.abs().cumsum(0) / count).repeat_interleave(per, 1) + longest * 2.0 ** -30 * v.abs().max()
     assert ((got - want).abs() <= bound).all()
+
+
+# ------------------------------------------------------------------------------------------------ evictions
+
+def test_an_installed_eviction_keeps_the_pages_entered_for_growth(native_lib):
+    """Ids behind a sequence's complete pages stay its own: every id is kept, freed or still assigned, new blocks go to
+    the ids entered for them, and page 0, which another sequence holds, is not written."""
+    layout, b = Q8Layout(4, 2, 64, 16, "int8"), 16
+    w = World(layout, [12 * b, 12 * b, 12 * b], seed=60, spare=0)
+    tables = torch.randperm(36, generator=w.gen).to(torch.int32).view(3, 12)
+    zero = (tables == 0).nonzero()[0]
+    tables[zero[0], zero[1]], tables[1, 2] = tables[1, 2].clone(), 0      # page 0: the third page of sequence 1
+    w.cache.set_block_tables(tables)
+    w.feed([7 * b + 5, 9 * b, 3 * b + 1])
+    mass = torch.rand((3, 2, 12), generator=w.gen)
+    mass[1, :, 2] = 9.0                                                   # kept
+    r = w.cache.evict(mass.to(DEV), budget=4, first=1, recent=1, max_seq_len=9 * b)
+    after = w.cache.block_tables.cpu()
+    for i, full in enumerate((7, 9, 3)):
+        kept = min(4, full)
+        freed = r.freed[i, :int(r.freed_counts[i])].tolist()
+        assert torch.equal(after[i, :kept], r.block_tables[i, :kept].cpu()) and int(r.block_tables[i, kept:].abs().max()) == 0
+        assert after[i, kept:12 - full + kept].tolist() == tables[i, full:].tolist()
+        assert (after[i, 12 - full + kept:] == -1).all()
+        assert sorted(after[i, :12 - full + kept].tolist() + freed) == sorted(tables[i].tolist())
+    assert 0 in after[1, :4]
+    codes, scales = (x.clone() for x in (w.cache.tensors.K_PAGES.view(torch.int8)[0], w.cache.tensors.SCALES[0]))
+    keep = [qo.evict(n // b, mass[i], 4, 1, 1) for i, n in enumerate(w.lens())]
+    for i, (k, v) in enumerate(w.rows):
+        rows = [p * b + j for p in keep[i] for j in range(b)] + list(range(k.shape[0] // b * b, k.shape[0]))
+        w.rows[i] = (k[rows], v[rows])
+    w.check_contents()
+    w.feed([2 * b, 2 * b + 3, b - 1])                                     # complete blocks in the pages entered before
+    w.check_contents()
+    assert torch.equal(codes, w.cache.tensors.K_PAGES.view(torch.int8)[0]) and torch.equal(scales, w.cache.tensors.SCALES[0])
+    # past the pages that were entered: refused and counted, and no page is written
+    before, pages = rejected_indices(), [t.clone() for t in w.cache.tensors[:3]]
+    rows = w.randn(8 * b, 2, 64).to(DEV)
+    w.cache.write(rows, rows, i32([0, 0, 8 * b, 8 * b]), max_new_per_seq=8 * b, max_start_seq_len=12 * b, start_seq_lens=w.cache.seq_lens)
+    assert rejected_indices() == before + 1
+    assert all(torch.equal(x.view(torch.uint8), y.view(torch.uint8)) for x, y in zip(pages, w.cache.tensors))
+
+
+def test_an_installed_eviction_that_evicts_nothing_changes_no_table(native_lib):
+    layout = Q8Layout(4, 2, 64, 16, "e4m3")
+    w = World(layout, [100, 60], seed=61)
+    w.feed([50, 60])
+    tables = w.cache.block_tables.clone()
+    w.cache.evict(torch.ones((2, 2, w.cache.max_blocks_per_seq), device=DEV), budget=50, max_seq_len=100)
+    assert torch.equal(tables, w.cache.block_tables) and w.cache.seq_lens.tolist() == [50, 60]
