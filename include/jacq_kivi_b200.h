@@ -320,14 +320,15 @@ int kivi_b200_q8_attention(const kivi_q8_geometry* geom, const kivi_q8_cache* ca
  *   new_tables [batch, max_blocks_per_seq]: 0 behind the kept pages;  new_lens [batch]
  *   new_mass [batch, NKV, mass_width]: the kept pages' columns and the open block's, 0 behind them
  *   freed [batch, max_blocks_per_seq]: ids of the evicted pages in order, -1 behind them;  freed_counts [batch]
- * mass_width * block_size >= max_seq_len; lengths are clamped to 0 .. max_seq_len. */
+ * mass_width * block_size >= max_seq_len. A sequence whose length lies outside 0 .. max_seq_len goes through unchanged,
+ * its table, masses and length copied and nothing freed, and is counted. */
 int kivi_b200_q8_evict(int num_kv_heads, int block_size, const int32_t* block_tables, int max_blocks_per_seq,
                        const int32_t* seq_lens, const float* page_mass, int mass_width, int batch, int max_seq_len,
                        int budget, int first, int recent, int32_t* new_tables, int32_t* new_lens, float* new_mass,
                        int32_t* freed, int32_t* freed_counts, cudaStream_t stream);
 
-/* Sequences (write, read) and ids (attention) refused since the library was loaded on the current device; 0 in any
- * healthy run. Synchronises the device. */
+/* Sequences (all calls) and page and slot ids (attention, read) refused since the library was loaded on the current
+ * device; 0 in any healthy run. Synchronises the device. */
 int kivi_b200_q8_rejected_indices(uint32_t* count_out);
 
 /* CTAs of the attention kernel for many query rows whose waits on shared-memory barriers, all of them bounded, gave up

@@ -189,10 +189,11 @@ extern "C" int kivi_b200_q8_evict(int num_kv_heads, int block_size, const int32_
 
 extern "C" int kivi_b200_q8_rejected_indices(uint32_t* count_out) {
     if (!count_out) return KIVI_ERR_NULL_POINTER;
-    unsigned int a = 0, b = 0, c = 0;
-    if (q8_cache_rejected(&a) != cudaSuccess || q8_attention_rejected(&b) != cudaSuccess || q8_prompt_rejected(&c) != cudaSuccess)
+    unsigned int a = 0, b = 0, c = 0, d = 0;
+    if (q8_cache_rejected(&a) != cudaSuccess || q8_attention_rejected(&b) != cudaSuccess || q8_prompt_rejected(&c) != cudaSuccess ||
+        q8_evict_rejected(&d) != cudaSuccess)
         return KIVI_ERR_CUDA;
-    *count_out = a + b + c;
+    *count_out = a + b + c + d;
     return KIVI_OK;
 }
 

@@ -31,6 +31,7 @@ __device__ __forceinline__ int q8_slot(const Q8Seqs& s, int i) { return s.slots 
 cudaError_t q8_cache_rejected(unsigned int* count);
 cudaError_t q8_attention_rejected(unsigned int* count);
 cudaError_t q8_prompt_rejected(unsigned int* count);
+cudaError_t q8_evict_rejected(unsigned int* count);
 
 // Two codes (the low 16 bits of `codes`) as a pair of fp16 values; every e4m3 value is an fp16 value.
 __device__ __forceinline__ uint32_t q8_e4m3_pair(uint16_t codes) {

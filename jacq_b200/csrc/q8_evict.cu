@@ -2,7 +2,8 @@
 // tables, masses and freed ids that follow.
 //
 // Per sequence: rank = fp32(sum over kv heads of page_mass, in 64 bits), keep the protected pages and the `budget`
-// minus those highest-ranking others (equal: lowest index first). One CTA per sequence holds the ranks as ordered
+// minus those highest-ranking others (equal: lowest index first). A sequence whose length lies outside the bounds goes
+// through as it is: cutting it would lose the pages behind the bound. One CTA per sequence holds the ranks as ordered
 // 32-bit keys in shared memory, finds the smallest kept key by a four-pass radix selection, and closes the kept pages
 // up with a running prefix count. Bound by latency: a few thousand keys, each read once from HBM and written once.
 // Measured: 4 sequences of 2048 tokens 8.8 us, 128 of 9000 .. 32768 tokens 13.8 us (2.6 us of data); with one atomic per
@@ -14,6 +15,8 @@ namespace {
 
 constexpr int kThreads = 1024;
 constexpr int kMaxKeys = 48 * 1024;   // pages of a sequence the shared memory holds a 4-byte key for
+
+__device__ unsigned int g_q8_evict_rejected;
 
 // Larger floats have larger keys; -0 equals 0; NaN is 0, below -infinity.
 __device__ __forceinline__ uint32_t key_of(float x) {
@@ -50,8 +53,14 @@ __global__ void __launch_bounds__(kThreads) q8_evict_kernel(const Q8EvictParams 
     int* freed = p.freed + (size_t)seq * p.width;
     const float* mass = p.mass + (size_t)seq * p.nkv * p.mass_width;
     float* new_mass = p.new_mass + (size_t)seq * p.nkv * p.mass_width;
-    const int len = min(max(p.lens[seq], 0), p.max_seq);
-    const int full = min(len >> p.log2b, p.width), open = len & ((1 << p.log2b) - 1);
+    const int len = p.lens[seq];
+    if (len < 0 || len > p.max_seq) {     // (max_seq's pages fit the table and the masses)
+        for (int i = tid; i < p.width; i += kThreads) { new_table[i] = table[i]; freed[i] = -1; }
+        for (size_t i = tid; i < (size_t)p.nkv * p.mass_width; i += kThreads) new_mass[i] = mass[i];
+        if (tid == 0) { p.new_lens[seq] = len; p.freed_counts[seq] = 0; atomicAdd(&g_q8_evict_rejected, 1u); }
+        return;
+    }
+    const int full = len >> p.log2b, open = len & ((1 << p.log2b) - 1);
     const bool all = full <= p.budget;
     const int lo = min(p.first, full), hi = max(lo, full - p.recent);   // candidates [lo, hi)
     uint32_t threshold = 0;
@@ -146,6 +155,8 @@ __global__ void __launch_bounds__(kThreads) q8_evict_kernel(const Q8EvictParams 
 }
 
 }  // namespace
+
+cudaError_t q8_evict_rejected(unsigned int* count) { return cudaMemcpyFromSymbol(count, g_q8_evict_rejected, sizeof(*count)); }
 
 int q8_evict_max_pages() { return kMaxKeys; }
 

@@ -346,8 +346,8 @@ def _check_mass(mass: torch.Tensor, batch: int, nkv: int | None, index: int) -> 
 def evict_pages(block_tables: torch.Tensor, seq_lens: torch.Tensor, page_mass: torch.Tensor, *, block_size: int, budget: int,
                 first: int = 0, recent: int = 0, max_seq_len: int) -> Q8Eviction:
     """Keep ``budget`` complete pages of every sequence that has more: its first ``first`` and last ``recent`` ones and, of
-    the others, those with the largest ``page_mass [batch, NKV, width]`` over all kv heads (ties: the lowest page). The
-    inputs stay as they are. Works on the tables of any paged cache whose pages are self-contained."""
+    the others, those with the largest ``page_mass [batch, NKV, width]`` over all kv heads (ties: the lowest page). A
+    sequence whose length lies outside 0 .. ``max_seq_len`` goes through unchanged and is counted. The inputs stay as they are. Works on the tables of any paged cache whose pages are self-contained."""
     index = block_tables.get_device()
     if index < 0:
         raise RuntimeError("evict_pages needs CUDA tensors; its kernel has no CPU path")

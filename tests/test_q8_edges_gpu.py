@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from jacq_b200.q8_cache import Q8Layout, rejected_indices
+from jacq_b200.q8_cache import Q8Layout, evict_pages, rejected_indices
 from tests import q8_oracle as qo
 from tests.test_q8_gpu import DEV, HALF, MANY, Large, World, i32, offsets_of
 
@@ -191,3 +191,28 @@ def test_an_installed_eviction_that_evicts_nothing_changes_no_table(native_lib):
     tables = w.cache.block_tables.clone()
     w.cache.evict(torch.ones((2, 2, w.cache.max_blocks_per_seq), device=DEV), budget=50, max_seq_len=100)
     assert torch.equal(tables, w.cache.block_tables) and w.cache.seq_lens.tolist() == [50, 60]
+
+
+def test_evictions_let_lengths_outside_the_bounds_through(native_lib):
+    """A sequence longer than max_seq_len, or of negative length: nothing is cut, freed or moved, and it is counted."""
+    width, gen = 20, torch.Generator().manual_seed(62)
+    lens = [160, 161, 20 * 16, -1, 0, 20 * 16 + 5]
+    tables = torch.randperm(6 * width, generator=gen).to(torch.int32).view(6, width)
+    mass = torch.rand((6, 2, width), generator=gen)
+    before = rejected_indices()
+    r = evict_pages(tables.to(DEV), i32(lens), mass.to(DEV), block_size=16, budget=4, first=1, recent=1, max_seq_len=160)
+    assert rejected_indices() == before + 4
+    assert r.seq_lens.tolist() == [64, 161, 320, -1, 0, 325]
+    assert r.freed_counts.tolist() == [6, 0, 0, 0, 0, 0]
+    for i in (1, 2, 3, 5):
+        assert torch.equal(r.block_tables[i].cpu(), tables[i]) and torch.equal(r.page_mass[i].cpu(), mass[i])
+        assert (r.freed[i] == -1).all()
+    # and so does an installed one
+    layout = Q8Layout(4, 2, 64, 16, "int8")
+    w = World(layout, [200, 90], seed=63)
+    w.feed([200, 90])
+    tables, mass = w.cache.block_tables.clone(), torch.rand((2, 2, w.cache.max_blocks_per_seq), device=DEV)
+    kept = mass.clone()
+    r = w.cache.evict(mass, budget=3, max_seq_len=100)
+    assert torch.equal(w.cache.block_tables[0], tables[0]) and w.cache.seq_lens.tolist() == [200, 58] and torch.equal(mass[0], kept[0])
+    assert int(r.freed_counts[1]) == 2
