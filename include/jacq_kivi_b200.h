@@ -301,8 +301,8 @@ size_t kivi_b200_q8_attention_workspace_bytes(const kivi_q8_geometry* geom, int 
  * zeros. out_f16 or out_f32 [total_q, NH, D], contiguous; exactly one is not NULL.
  * page_mass (or NULL) f32 [batch, NKV, mass_width], single-token calls only (q_offsets NULL): entry [i, h, p] grows by the
  * softmax weight that the query heads of kv head h gave the tokens of logical page p; mass_width * B >= max_seq_len.
- * Lengths are on the device: a longer one than max_seq_len counts as max_seq_len, a negative one as 0; page and slot
- * ids outside the pools are read as 0 and counted; a sequence whose q rows lie outside 0 .. total_q, or are more than
+ * Lengths are on the device: a longer one than max_seq_len is taken as max_seq_len, a negative one as 0, and counted; page
+ * and slot ids outside the pools are read as 0 and counted; a sequence whose q rows lie outside 0 .. total_q, or are more than
  * max_q_per_seq, is skipped (its output rows are left) and counted.
  * The workspace belongs to the call until it is done: calls that may run at the same time need one each. Results do not
  * depend on what it holds, and for given sizes repeat bit for bit. */

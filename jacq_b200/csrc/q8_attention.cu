@@ -155,10 +155,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>()) q8_attentio
     const Unit u = make_unit(p, unit, R);
     const int seq = u.seq, h = u.h, rb = u.rb, len = u.len, n = u.n, row0 = u.row0, rows = u.rows, items = u.items;
     const View& v = u.v;
-    if (rb * R >= rows) {                        // uniform over the cluster
-        if (u.refused && h == 0 && rb == 0 && part == 0 && threadIdx.x == 0) atomicAdd(&g_q8_attn_rejected, 1u);
-        return;
-    }
+    if (u.counted && h == 0 && rb == 0 && part == 0 && threadIdx.x == 0) atomicAdd(&g_q8_attn_rejected, 1u);
+    if (rb * R >= rows) return;                  // uniform over the cluster
     const int i0 = min(part * p.chunk, items), i1 = min(i0 + p.chunk, items);
     if (p.cluster == 0 && i0 == i1 && part > 0) return;   // the merge knows how many parts have something
 

@@ -143,13 +143,15 @@ struct Unit {
     View v;
     int items;          // tiles of the page part and of the tail
     bool refused;       // its query rows do not lie inside the launch's
+    bool counted;       // refused, or its length had to be brought into the launch's bounds
 };
 __device__ __forceinline__ Unit make_unit(const Q8AttnParams& p, int unit, int r_per_block) {
     Unit u;
     u.rb = unit % p.row_blocks + p.row_block0;
     unit /= p.row_blocks;
     u.h = unit % p.cache.nkv; u.seq = unit / p.cache.nkv;
-    u.len = min(max(p.seq.lens[u.seq], 0), p.max_seq);
+    const int len = p.seq.lens[u.seq];
+    u.len = min(max(len, 0), p.max_seq);
     u.row0 = u.seq; u.n = 1;
     u.refused = false;
     if (p.q_offsets) {
@@ -157,6 +159,7 @@ __device__ __forceinline__ Unit make_unit(const Q8AttnParams& p, int unit, int r
         u.n = p.q_offsets[u.seq + 1] - u.row0;
         if (u.row0 < 0 || u.n < 0 || u.n > p.max_q || u.row0 > p.total_q - u.n) { u.n = 0; u.refused = true; }
     }
+    u.counted = u.refused || u.len != len;
     u.rows = u.n * p.qpk;
     const int first = u.rb * r_per_block, last = min(first + r_per_block, u.rows) - 1;
     u.v = make_view(p, u.len, u.n, first / p.qpk, max(last, 0) / p.qpk);

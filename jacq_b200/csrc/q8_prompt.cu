@@ -164,10 +164,8 @@ __global__ void __launch_bounds__(kThreads, 1) q8_prompt_kernel(const Q8AttnPara
     const int at_block = blockIdx.x % p.row_blocks;
     const Unit u = make_unit(p, blockIdx.x - at_block + (p.row_blocks - 1 - at_block), TILES * kRows);
     const int row_base = u.rb * TILES * kRows;
-    if (row_base >= u.rows) {
-        if (u.refused && u.h == 0 && u.rb == 0 && tid == 0) atomicAdd(&g_q8_prompt_rejected, 1u);
-        return;
-    }
+    if (u.counted && u.h == 0 && u.rb == 0 && tid == 0) atomicAdd(&g_q8_prompt_rejected, 1u);
+    if (row_base >= u.rows) return;
     const View& v = u.v;
     const int steps = (u.items + 7) >> 3;
     const int tiles = row_base + kRows < u.rows ? TILES : 1;       // tiles with rows in them

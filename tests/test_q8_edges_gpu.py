@@ -216,3 +216,27 @@ def test_evictions_let_lengths_outside_the_bounds_through(native_lib):
     r = w.cache.evict(mass, budget=3, max_seq_len=100)
     assert torch.equal(w.cache.block_tables[0], tables[0]) and w.cache.seq_lens.tolist() == [200, 58] and torch.equal(mass[0], kept[0])
     assert int(r.freed_counts[1]) == 2
+
+
+# ------------------------------------------------------------------------------------------------ lengths, ids, bounds
+
+@pytest.mark.parametrize("many", [False, True])
+def test_attention_counts_lengths_outside_the_bounds(many, native_lib):
+    """In both kernels a length above max_seq_len answers as max_seq_len, a negative one as 0, and each is counted once."""
+    layout, batch, longest = MANY[0]
+    w = Prompts(layout, [longest] * batch, 64)
+    lens = [longest] * batch
+    lens[1], lens[4], lens[7] = longest + 1, -5, 1 << 29
+    clamped = [min(max(t, 0), longest) for t in lens]
+    n = longest if many else 1
+    q = torch.randn((n * batch, layout.num_q_heads, layout.head_dim), generator=w.g, device=DEV).half()
+    kw = dict(max_seq_len=longest, q_offsets=i32([n * i for i in range(batch + 1)]), max_q_per_seq=n) if many else dict(max_seq_len=longest)
+    before = rejected_indices()
+    good = w.cache.attend(q, seq_lens=i32(clamped), **kw)
+    assert rejected_indices() == before
+    assert torch.equal(w.cache.attend(q, seq_lens=i32(lens), **kw), good) and rejected_indices() == before + 3
+    assert int(good[4 * n:5 * n].abs().max()) == 0
+    if not many:
+        mass = torch.zeros((batch, layout.num_kv_heads, w.cache.max_blocks_per_seq), device=DEV)
+        w.cache.attend(q, seq_lens=i32(lens), page_mass=mass, **kw)
+        assert rejected_indices() == before + 6
