@@ -104,8 +104,9 @@ extern "C" int kivi_b200_q8_cache_read(const kivi_q8_geometry* geom, const kivi_
 
 namespace {
 constexpr int kNoWindow = 0x7fffffff;
-int window_of(int window) { return window == 0 ? kNoWindow : window; }
-// Grid size of a call: (sequence, kv head, block of 8 query rows) units cut into at most 16 parts.
+// A window of max_seq_len tokens or more hides none; as a number it would overflow in positions before the first token.
+int window_of(int window, int max_seq) { return window == 0 || window >= max_seq ? kNoWindow : window; }
+// Grid size of a call: (sequence, kv head, block of 8 query rows) units cut into at most 32 parts.
 bool q8_grid_fits(const kivi_q8_geometry* g, int batch, int max_q) {
     const int64_t rows = (int64_t)max_q * (g->num_q_heads / g->num_kv_heads);
     return rows < (1 << 24) && (int64_t)batch * g->num_kv_heads * ((rows + 7) / 8) < (1LL << 27);
@@ -117,7 +118,7 @@ extern "C" size_t kivi_b200_q8_attention_workspace_bytes(const kivi_q8_geometry*
     if (check_q8_geometry(geom) != KIVI_OK || batch < 1 || batch > kQ8MaxBatch || max_q_per_seq < 1 || max_seq_len < 0 ||
         max_seq_len > kQ8MaxLen || window < 0 || sinks < 0 || !q8_grid_fits(geom, batch, max_q_per_seq)) return 0;
     return q8_attention_workspace(geom->num_kv_heads, geom->num_q_heads / geom->num_kv_heads, geom->head_dim, geom->block_size, batch, max_q_per_seq,
-                                  max_seq_len, window_of(window), sinks, with_mass != 0);
+                                  max_seq_len, window_of(window, max_seq_len), sinks, with_mass != 0);
 }
 
 extern "C" int kivi_b200_q8_attention(const kivi_q8_geometry* geom, const kivi_q8_cache* cache, const kivi_f16* q,
@@ -145,7 +146,7 @@ extern "C" int kivi_b200_q8_attention(const kivi_q8_geometry* geom, const kivi_q
     p.q = reinterpret_cast<const __half*>(q); p.q_stride = q_stride; p.q_offsets = q_offsets;
     p.total_q = total_q; p.max_q = max_q_per_seq; p.max_seq = max_seq_len;
     p.qpk = geom->num_q_heads / geom->num_kv_heads;
-    p.window = window_of(window); p.sinks = sinks;
+    p.window = window_of(window, max_seq_len); p.sinks = sinks;
     const float s = scale > 0.0f ? scale : (geom->head_dim == 64 ? 0.125f : geom->head_dim == 256 ? 0.0625f : 0.08838834764831845f);
     p.scale_log2 = s * 1.4426950408889634f;
     p.out = out_f32; p.out_h = reinterpret_cast<__half*>(out_f16);

@@ -240,3 +240,12 @@ def test_attention_counts_lengths_outside_the_bounds(many, native_lib):
         mass = torch.zeros((batch, layout.num_kv_heads, w.cache.max_blocks_per_seq), device=DEV)
         w.cache.attend(q, seq_lens=i32(lens), page_mass=mass, **kw)
         assert rejected_indices() == before + 6
+
+
+@pytest.mark.parametrize("window", [(1 << 31) - 2, (1 << 31) - 1, 1 << 30])
+def test_the_largest_windows_hide_nothing_from_runs_longer_than_their_sequence(window, native_lib):
+    w = World(Q8Layout(4, 2, 128, 16, "int8"), [40], seed=65)
+    w.feed([40])
+    q = w.randn(60, 4, 128)                       # tokens -20 .. 39
+    want = w.attend(q, [60])
+    assert torch.equal(w.attend(q, [60], window=window), want) and torch.equal(w.attend(q, [60], window=window, sinks=(1 << 31) - 1), want)
