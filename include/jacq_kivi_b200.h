@@ -245,7 +245,8 @@ int kivi_b200_gemm_wait_failures(uint32_t* failures_out);
  * quantised once, from its fp16 rows, when its last token arrives, so no value is ever rounded twice.
  *   scale = max|x| * fp32(1/127) (e4m3: fp32(1/448)), code = x / scale rounded to nearest even
  * An all-zero block has scale 0. A block that holds an infinity or a NaN gets scale NaN and zero codes: every
- * query that sees one of its tokens yields NaN, queries that do not are unaffected. */
+ * query that sees one of its tokens yields NaN, queries that do not are unaffected. In a tail row such a value of V
+ * makes its channel NaN for the queries that see it. */
 enum kivi_q8_format { KIVI_Q8_INT8 = 0, KIVI_Q8_E4M3 = 1 };
 
 typedef struct kivi_q8_geometry {

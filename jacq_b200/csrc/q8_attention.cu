@@ -486,8 +486,14 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>()) q8_attentio
                     }
                 }
             uint32_t pb[1][NT][4];
-            const float one = 1.0f;
-            softmax(std::integral_constant<int, 1>(), s, &p.scale_log2, &one, &key0, item, 1, pb);
+            const float unit_scale = 1.0f;
+            softmax(std::integral_constant<int, 1>(), s, &p.scale_log2, &unit_scale, &key0, item, 1, pb);
+            uint32_t seen = 0;                      // bit 4 nt + e: whether score e's row sees its key
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) seen |= (s[0][nt][e] != -INFINITY ? 1u : 0u) << (4 * nt + e);
+            auto ones = [&](int bit) { return movmatrix_trans((seen >> bit & 1u) * 0x3c00u + (seen >> (bit + 1) & 1u) * 0x3c000000u); };
 #pragma unroll
             for (int e = 0; e < T::MT / 4; ++e) {   // 8 channels of a token per 16-byte word: output tiles 4 e .. 4 e + 3
                 const int chan = D == 64 ? 8 * g : 16 * g + 8 * (e & 1) + 128 * (e >> 1);
@@ -512,7 +518,8 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>()) q8_attentio
                 pairs(x[0], x[1], 0);
                 pairs(x[2], x[3], 2);
                 // An infinity or NaN in V must reach the rows that see its token and no other, but 0 * NaN is NaN: such
-                // elements leave the product, and a second product counts the weight that fell on them.
+                // elements leave the product, and a second product counts those that a row sees (not their weight, which may
+                // have underflowed).
                 const bool any_odd = __any_sync(0xffffffffu, odd);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
@@ -530,7 +537,7 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>()) q8_attentio
                         if (!FOLD) product(o[nt][4 * e + i], a[i][0], a[i][1], a[i][2], a[i][3], pb[0][nt][2], pb[0][nt][3]);
                         if (any_odd) {
                             float hit[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            product(hit, bad[0], bad[1], bad[2], bad[3], pb[0][nt][0], pb[0][nt][1]);
+                            product(hit, bad[0], bad[1], bad[2], bad[3], ones(4 * nt), ones(4 * nt + 2));
 #pragma unroll
                             for (int k = 0; k < 4; ++k) if (hit[k] != 0.0f) o[nt][4 * e + i][k] = __int_as_float(0x7fc00000);
                         }

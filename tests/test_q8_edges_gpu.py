@@ -249,3 +249,25 @@ def test_the_largest_windows_hide_nothing_from_runs_longer_than_their_sequence(w
     q = w.randn(60, 4, 128)                       # tokens -20 .. 39
     want = w.attend(q, [60])
     assert torch.equal(w.attend(q, [60], window=window), want) and torch.equal(w.attend(q, [60], window=window, sinks=(1 << 31) - 1), want)
+
+
+@pytest.mark.parametrize("layout", [Q8Layout(8, 2, 128, 32, "int8"), Q8Layout(6, 1, 64, 64, "e4m3"), Q8Layout(12, 1, 256, 16, "int8")],
+                         ids=["128", "64", "256"])
+def test_a_nan_in_a_visible_tail_row_shows_whatever_its_weight(layout, native_lib):
+    """Its key scores e^-60 below the others: the weight underflows, a NaN times it does not."""
+    b, d = layout.block_size, layout.head_dim
+    t = 2 * b + 10
+    w = World(layout, [t], seed=66)
+    k, v = w.randn(t, layout.num_kv_heads, d), w.randn(t, layout.num_kv_heads, d)
+    k[t - 4] = -60.0 / d ** 0.5
+    v[t - 4, 0, 5] = float("nan")
+    v[t - 4, 0, 6] = float("-inf")
+    w.feed([t], k, v)
+    per = layout.num_q_heads // layout.num_kv_heads
+    for n, window in ((1, 0), (1, 4), (1, 3), (7, 0), (7, 3)):
+        got = w.attend(torch.ones((n, layout.num_q_heads, d)).half(), None if n == 1 else [n], window=window)
+        bad = torch.zeros(got.shape, dtype=torch.bool)
+        for i, at in enumerate(range(t - n, t)):                        # token t - 4 is seen from itself on, as long as the window
+            if at >= t - 4 and (window == 0 or t - 4 > at - window):
+                bad[i, :per, 5:7] = True
+        assert torch.equal(got.isnan(), bad), (n, window)
