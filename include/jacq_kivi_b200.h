@@ -281,6 +281,19 @@ int kivi_b200_q8_cache_write(const kivi_q8_geometry* geom, const kivi_q8_cache* 
                              int batch, int total_new, int max_new_per_seq, int max_start_seq_len,
                              cudaStream_t stream);
 
+/* The calls here take tables and lengths by sequence of the batch. Where they are stored by slot, this gathers them: row i
+ * of out_tables [batch, max_blocks_per_seq] becomes block_tables[slot_ids[i]], and out_lens[i] becomes
+ * seq_lens[slot_ids[i]], or seq_lens[i] with lens_by_slot 0. num_rows: rows of block_tables (and of seq_lens, by slot). A
+ * slot id outside 0 .. num_rows - 1 yields page ids and a length of -1, which the other calls refuse and count. */
+int kivi_b200_q8_gather_slots(const int32_t* block_tables, int max_blocks_per_seq, const int32_t* seq_lens, int lens_by_slot,
+                              int num_rows, const int32_t* slot_ids, int batch, int32_t* out_tables, int32_t* out_lens,
+                              cudaStream_t stream);
+
+/* After a write: seq_lens[slot_ids[i]] grows by new_offsets[i + 1] - new_offsets[i]; ids outside 0 .. num_rows - 1 are
+ * left out. */
+int kivi_b200_q8_advance_slots(int32_t* seq_lens, int num_rows, const int32_t* slot_ids, const int32_t* new_offsets, int batch,
+                               cudaStream_t stream);
+
 /* The values the cache holds, as fp16: rows row_offsets[i] .. row_offsets[i+1]-1 of k_out / v_out
  * ([total_rows, NKV, D], contiguous) receive tokens first_rows[i] .. of sequence i, which holds seq_lens[i] tokens.
  * Rows behind the sequence's last token become zeros; the rows of sequences the call rejects (as above) are left. */

@@ -128,6 +128,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "kivi_b200_silu_mul": (c_int, [_P, _P, c_int, c_int, _P]),
     "kivi_b200_argmax": (c_int, [_P, _P, c_int, c_int, _P, c_size_t, _P]),
     "kivi_b200_q8_validate_geometry": (c_int, [ctypes.POINTER(KiviQ8Geometry)]),
+    "kivi_b200_q8_gather_slots": (c_int, [_P, c_int, _P, c_int, c_int, _P, c_int, _P, _P, _P]),
+    "kivi_b200_q8_advance_slots": (c_int, [_P, c_int, _P, _P, c_int, _P]),
     "kivi_b200_q8_cache_write": (c_int, [ctypes.POINTER(KiviQ8Geometry), ctypes.POINTER(KiviQ8CacheStruct), _P, _P, c_int64,
                                          c_int64, _P, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, _P]),
     "kivi_b200_q8_cache_read": (c_int, [ctypes.POINTER(KiviQ8Geometry), ctypes.POINTER(KiviQ8CacheStruct), _P, c_int, _P, _P,

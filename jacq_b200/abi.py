@@ -45,7 +45,8 @@ V2_SYMBOLS = (
     "kivi_b200_bias_rope", "kivi_b200_silu_mul", "kivi_b200_argmax",
     "kivi_b200_p2p_region_bytes", "kivi_b200_p2p_region_create", "kivi_b200_p2p_region_open",
     "kivi_b200_p2p_region_close", "kivi_b200_p2p_region_destroy", "kivi_b200_p2p_status",
-    "kivi_b200_q8_validate_geometry", "kivi_b200_q8_cache_write", "kivi_b200_q8_cache_read",
+    "kivi_b200_q8_validate_geometry", "kivi_b200_q8_gather_slots", "kivi_b200_q8_advance_slots",
+    "kivi_b200_q8_cache_write", "kivi_b200_q8_cache_read",
     "kivi_b200_q8_attention_workspace_bytes", "kivi_b200_q8_attention", "kivi_b200_q8_evict",
     "kivi_b200_q8_rejected_indices", "kivi_b200_q8_wait_failures",
 )

@@ -56,6 +56,25 @@ using namespace kivi;
 
 extern "C" int kivi_b200_q8_validate_geometry(const kivi_q8_geometry* geom) { return check_q8_geometry(geom); }
 
+extern "C" int kivi_b200_q8_gather_slots(const int32_t* block_tables, int max_blocks_per_seq, const int32_t* seq_lens, int lens_by_slot,
+                                         int num_rows, const int32_t* slot_ids, int batch, int32_t* out_tables, int32_t* out_lens,
+                                         cudaStream_t stream) {
+    if (batch < 0 || batch > kQ8MaxBatch || max_blocks_per_seq < 0 || num_rows < 0) return KIVI_ERR_RANGE;
+    if (batch == 0) return KIVI_OK;
+    if (!slot_ids || !out_lens || (!seq_lens && num_rows) || (max_blocks_per_seq && (!out_tables || (!block_tables && num_rows))))
+        return KIVI_ERR_NULL_POINTER;
+    return launch_q8_gather(block_tables, max_blocks_per_seq, seq_lens, lens_by_slot != 0, num_rows, slot_ids, batch, out_tables,
+                            out_lens, stream) == cudaSuccess ? KIVI_OK : KIVI_ERR_CUDA;
+}
+
+extern "C" int kivi_b200_q8_advance_slots(int32_t* seq_lens, int num_rows, const int32_t* slot_ids, const int32_t* new_offsets,
+                                          int batch, cudaStream_t stream) {
+    if (batch < 0 || batch > kQ8MaxBatch || num_rows < 0) return KIVI_ERR_RANGE;
+    if (batch == 0 || num_rows == 0) return KIVI_OK;
+    if (!seq_lens || !slot_ids || !new_offsets) return KIVI_ERR_NULL_POINTER;
+    return launch_q8_advance(seq_lens, num_rows, slot_ids, new_offsets, batch, stream) == cudaSuccess ? KIVI_OK : KIVI_ERR_CUDA;
+}
+
 extern "C" int kivi_b200_q8_cache_write(const kivi_q8_geometry* geom, const kivi_q8_cache* cache, const kivi_f16* new_k,
                                         const kivi_f16* new_v, int64_t k_stride, int64_t v_stride,
                                         const int32_t* block_tables, int max_blocks_per_seq, const int32_t* start_seq_lens,

@@ -220,6 +220,19 @@ __global__ void __launch_bounds__(256) q8_read_kernel(const Q8ReadParams p) {
     }
 }
 
+// Rows of per-slot tables and lengths for a batch: one CTA a sequence, bound by its launch.
+__global__ void __launch_bounds__(128) q8_gather_kernel(const int* tables, int width, const int* lens, bool by_slot, int rows,
+                                                        const int* slots, int* out_tables, int* out_lens) {
+    const int i = blockIdx.x, slot = slots[i];
+    const bool ok = index_in_pool(slot, rows);
+    for (int c = threadIdx.x; c < width; c += 128) out_tables[(size_t)i * width + c] = ok ? tables[(size_t)slot * width + c] : -1;
+    if (threadIdx.x == 0) out_lens[i] = ok ? lens[by_slot ? slot : i] : -1;
+}
+__global__ void __launch_bounds__(128) q8_advance_kernel(int* lens, int rows, const int* slots, const int* offsets, int batch) {
+    const int i = blockIdx.x * 128 + threadIdx.x;
+    if (i < batch && index_in_pool(slots[i], rows)) atomicAdd(lens + slots[i], offsets[i + 1] - offsets[i]);
+}
+
 template <int D>
 cudaError_t write_d(const Q8WriteParams& p, int fmt, dim3 grid, int threads, int wpb, cudaStream_t stream) {
     if (fmt == KIVI_Q8_INT8) q8_write_kernel<D, KIVI_Q8_INT8><<<grid, threads, 0, stream>>>(p, wpb);
@@ -234,6 +247,17 @@ cudaError_t read_d(const Q8ReadParams& p, int fmt, dim3 grid, cudaStream_t strea
 }
 
 }  // namespace
+
+cudaError_t launch_q8_gather(const int* tables, int width, const int* lens, bool by_slot, int rows, const int* slots, int batch,
+                             int* out_tables, int* out_lens, cudaStream_t stream) {
+    q8_gather_kernel<<<batch, 128, 0, stream>>>(tables, width, lens, by_slot, rows, slots, out_tables, out_lens);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_q8_advance(int* lens, int rows, const int* slots, const int* offsets, int batch, cudaStream_t stream) {
+    q8_advance_kernel<<<(batch + 127) / 128, 128, 0, stream>>>(lens, rows, slots, offsets, batch);
+    return cudaGetLastError();
+}
 
 cudaError_t launch_q8_write(const Q8WriteParams& p, int d, int fmt, cudaStream_t stream) {
     const int block = 1 << p.cache.log2b, wpb = block / 16, warps = wpb > 4 ? wpb : 4;

@@ -181,6 +181,9 @@ struct Q8EvictParams {
     int nkv, log2b, batch, max_seq, budget, first, recent;
     int* new_tables; int* new_lens; float* new_mass; int* freed; int* freed_counts;
 };
+cudaError_t launch_q8_gather(const int* tables, int width, const int* lens, bool by_slot, int rows, const int* slots, int batch,
+                             int* out_tables, int* out_lens, cudaStream_t stream);
+cudaError_t launch_q8_advance(int* lens, int rows, const int* slots, const int* offsets, int batch, cudaStream_t stream);
 cudaError_t launch_q8_write(const Q8WriteParams& p, int d, int fmt, cudaStream_t stream);
 cudaError_t launch_q8_read(const Q8ReadParams& p, int d, int fmt, cudaStream_t stream);
 cudaError_t launch_q8_attention(const Q8AttnParams& p, int d, int fmt, void* workspace, cudaStream_t stream);

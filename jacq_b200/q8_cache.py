@@ -155,6 +155,7 @@ class Q8Cache:
         self._geom_ref, self._cache_ref = ctypes.byref(self._geom), ctypes.byref(self._struct)
         lib = _native.lib()
         self._write, self._read, self._attention = lib.kivi_b200_q8_cache_write, lib.kivi_b200_q8_cache_read, lib.kivi_b200_q8_attention
+        self._gather, self._advance = lib.kivi_b200_q8_gather_slots, lib.kivi_b200_q8_advance_slots
         self._workspace_of = lib.kivi_b200_q8_attention_workspace_bytes
         self._workspace_bytes: dict[tuple, int] = {}   # by the sizes of a call; the plan behind them is host arithmetic
 
@@ -164,23 +165,37 @@ class Q8Cache:
         self.block_tables.zero_()
         self.block_tables[: tables.shape[0], : tables.shape[1]] = tables
 
+    def _call(self, where: str, fn, *args) -> None:
+        if self._index == _current_device():
+            rc = fn(*args, _raw_stream(self._index))
+            if rc:
+                _native.check(rc, where)
+        else:
+            _elsewhere(self._index, where, fn, *args)
+
     def _rows(self, batch: int, slot_ids, lens):
         """Pointers of the batch's block-table rows, lengths and slots, and the tensors to keep alive: tables and lengths
-        are stored per slot, the library indexes them per batch row."""
-        tables = self.block_tables
-        slots = 0
-        if slot_ids is not None:
-            slots = _int32(slot_ids, "slot_ids", self._index)
-            if slot_ids.numel() != batch:
-                raise RuntimeError(f"slot_ids holds {slot_ids.numel()} entries for a batch of {batch}")
-            tables = tables.index_select(0, slot_ids)
-            if lens is None:
-                lens = self.seq_lens.index_select(0, slot_ids)
-        elif lens is None:
+        are stored per slot, the library indexes them per batch row. The gather refuses slots that are not there."""
+        tables, by_slot = self.block_tables, lens is None
+        if by_slot:
             lens = self.seq_lens
-        if tables.shape[0] < batch or lens.numel() < batch:
-            raise RuntimeError(f"a batch of {batch} exceeds the {tables.shape[0]} block-table rows / {lens.numel()} lengths")
-        return tables.data_ptr(), _int32(lens, "sequence lengths", self._index), slots, (tables, lens)
+        at = _int32(lens, "sequence lengths", self._index)
+        if slot_ids is None:
+            if tables.shape[0] < batch or lens.numel() < batch:
+                raise RuntimeError(f"a batch of {batch} exceeds the {tables.shape[0]} block-table rows / {lens.numel()} lengths")
+            return tables.data_ptr(), at, 0, (tables, lens)
+        slots = _int32(slot_ids, "slot_ids", self._index)
+        if slot_ids.numel() != batch:
+            raise RuntimeError(f"slot_ids holds {slot_ids.numel()} entries for a batch of {batch}")
+        rows = tables.shape[0]
+        if by_slot:
+            rows = min(rows, lens.numel())
+        elif lens.numel() < batch:
+            raise RuntimeError(f"a batch of {batch} exceeds the {lens.numel()} lengths")
+        picked, lengths = tables.new_empty((batch, self.max_blocks_per_seq)), tables.new_empty((batch,))
+        args = (tables.data_ptr(), self.max_blocks_per_seq, at, int(by_slot), rows, slots, batch, picked.data_ptr(), lengths.data_ptr())
+        self._call("kivi_b200_q8_gather_slots", self._gather, *args)
+        return picked.data_ptr(), lengths.data_ptr(), slots, (picked, lengths)
 
     def _token_rows(self, t: torch.Tensor, name: str, heads: int) -> tuple[int, int]:
         """Checks ``[tokens, heads, head_dim]`` fp16 rows that are contiguous within a token; tokens, stride in elements."""
@@ -221,11 +236,11 @@ class Q8Cache:
             _elsewhere(index, "kivi_b200_q8_cache_write", self._write, geom, cache, new_k.data_ptr(), new_v.data_ptr(), ks, vs, tables,
                        self.max_blocks_per_seq, starts, offsets, slots, n, total, max_new_per_seq, max_start_seq_len)
         if advance and start_seq_lens is None:
-            counts = new_offsets[1:] - new_offsets[:-1]
             if slot_ids is None:
-                self.seq_lens[:n] += counts
+                self.seq_lens[:n] += new_offsets[1:] - new_offsets[:-1]
             else:
-                self.seq_lens.index_add_(0, slot_ids, counts)
+                rows = min(self.block_tables.shape[0], self.seq_lens.numel())
+                self._call("kivi_b200_q8_advance_slots", self._advance, self.seq_lens.data_ptr(), rows, slots, offsets, n)
 
     def read(self, row_offsets: torch.Tensor, first_rows: torch.Tensor, seq_lens: torch.Tensor | None = None, *, total: int,
              max_rows_per_seq: int, slot_ids: torch.Tensor | None = None, k_out: torch.Tensor | None = None,

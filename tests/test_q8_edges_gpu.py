@@ -271,3 +271,32 @@ def test_a_nan_in_a_visible_tail_row_shows_whatever_its_weight(layout, native_li
             if at >= t - 4 and (window == 0 or t - 4 > at - window):
                 bad[i, :per, 5:7] = True
         assert torch.equal(got.isnan(), bad), (n, window)
+
+
+def test_slots_that_are_not_there_are_refused_by_every_call(native_lib):
+    """Slot ids outside the tables: nothing is written or advanced, rows stay, attention gives zeros; each is counted."""
+    layout = Q8Layout(4, 2, 64, 16, "int8")
+    w = World(layout, [90, 90, 90], seed=67)
+    w.feed([40, 50, 64])
+    ids = i32([2, -1, 0, 3, 1 << 30])
+    k, q = w.randn(5, 2, 64).to(DEV), w.randn(5, 4, 64).to(DEV)
+    before = rejected_indices()
+    good = w.cache.attend(q[[0, 2]], max_seq_len=90, slot_ids=i32([2, 0]))
+    got = w.cache.attend(q, max_seq_len=90, slot_ids=ids)
+    assert torch.equal(got[[0, 2]], good) and int(got[[1, 3, 4]].abs().max()) == 0 and rejected_indices() == before + 3
+    got = w.cache.attend(q, max_seq_len=90, slot_ids=ids, seq_lens=i32([64, 40, 40, 40, 40]))     # the caller's lengths
+    assert torch.equal(got[[0, 2]], good) and int(got[[1, 3, 4]].abs().max()) == 0 and rejected_indices() == before + 6
+    out = [torch.full((5, 2, 64), 3.0, dtype=torch.float16, device=DEV) for _ in range(2)]
+    w.cache.read(i32([0, 1, 2, 3, 4, 5]), i32([5] * 5), total=5, max_rows_per_seq=1, slot_ids=ids, k_out=out[0], v_out=out[1])
+    assert (out[0][[1, 3, 4]] == 3.0).all() and not (out[0][[0, 2]] == 3.0).any() and rejected_indices() == before + 9
+    w.cache.write(k, k, i32([0, 1, 2, 3, 4, 5]), max_new_per_seq=1, max_start_seq_len=90, slot_ids=ids)
+    assert w.cache.seq_lens.tolist() == [41, 50, 65] and rejected_indices() == before + 12
+    w.rows = [(torch.cat([a, b]), torch.cat([c, b])) for (a, c), b in zip(w.rows, (k[2:3].cpu(), k[:0].cpu(), k[:1].cpu()))]
+    w.check_contents()
+    graph, lens, ends = torch.cuda.CUDAGraph(), w.cache.seq_lens.clone(), i32([0, 1, 2, 3, 4, 5])
+    with torch.cuda.graph(graph):
+        w.cache.write(k, k, ends, max_new_per_seq=1, max_start_seq_len=90, slot_ids=ids)
+        got = w.cache.attend(q, max_seq_len=90, slot_ids=ids)
+    graph.replay()
+    assert (w.cache.seq_lens - lens).tolist() == [1, 0, 1]
+    assert torch.equal(got[[0, 2]], w.cache.attend(q[[0, 2]], max_seq_len=90, slot_ids=i32([2, 0])))

@@ -1,0 +1,23 @@
+"""Refusals and bookkeeping of the 8-bit cache that need no GPU, beside those of ``tests/test_q8_host.py``."""
+import pytest
+
+OK, NULL, RANGE = 0, 1, 3
+FAKE = 1 << 20      # stands for a device pointer; never dereferenced on the host
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(batch=-1), RANGE), (dict(batch=65536), RANGE), (dict(width=-1), RANGE), (dict(rows=-1), RANGE), (dict(slots=0), NULL),
+    (dict(tables=0), NULL), (dict(lens=0), NULL), (dict(out_tables=0), NULL), (dict(out_lens=0), NULL), (dict(batch=0), OK)])
+def test_gather_refusals(native_lib, change, status):
+    a = dict(tables=FAKE, width=8, lens=FAKE, by_slot=1, rows=4, slots=FAKE, batch=2, out_tables=FAKE, out_lens=FAKE)
+    a.update(change)
+    assert native_lib.kivi_b200_q8_gather_slots(*a.values(), 0) == status
+
+
+@pytest.mark.parametrize("change,status", [
+    (dict(batch=-1), RANGE), (dict(batch=65536), RANGE), (dict(rows=-1), RANGE), (dict(lens=0), NULL), (dict(slots=0), NULL),
+    (dict(offsets=0), NULL), (dict(batch=0), OK), (dict(rows=0), OK)])
+def test_advance_refusals(native_lib, change, status):
+    a = dict(lens=FAKE, rows=4, slots=FAKE, offsets=FAKE, batch=2)
+    a.update(change)
+    assert native_lib.kivi_b200_q8_advance_slots(*a.values(), 0) == status
