@@ -157,7 +157,7 @@ class Q8Cache:
         self._write, self._read, self._attention = lib.kivi_b200_q8_cache_write, lib.kivi_b200_q8_cache_read, lib.kivi_b200_q8_attention
         self._gather, self._advance = lib.kivi_b200_q8_gather_slots, lib.kivi_b200_q8_advance_slots
         self._workspace_of = lib.kivi_b200_q8_attention_workspace_bytes
-        self._workspace_bytes: dict[tuple, int] = {}   # by the sizes of a call; the plan behind them is host arithmetic
+        self._workspace_bytes: dict[tuple, int] = {}   # by the sizes of a call
 
     def set_block_tables(self, tables: torch.Tensor) -> None:
         """Install block tables ``[<= num_slots, <= max_blocks_per_seq]`` (int32; host or device)."""
@@ -272,6 +272,15 @@ class Q8Cache:
                        first, n, total, max_rows_per_seq, k_out.data_ptr(), v_out.data_ptr())
         return k_out, v_out
 
+    def _ask_workspace(self, sizes: tuple) -> int:
+        """Bytes for a call of these sizes, by the plan for this cache's device; the last sizes asked for are kept."""
+        with torch.cuda.device(self._index):
+            size = self._workspace_of(self._geom_ref, *sizes)
+        if len(self._workspace_bytes) >= 64:   # a batch that grows by a token a step never asks for the same sizes again
+            self._workspace_bytes.clear()
+        self._workspace_bytes[sizes] = size
+        return size
+
     def attend(self, q: torch.Tensor, out: torch.Tensor | None = None, *, max_seq_len: int, window: int = 0, sinks: int = 0,
                scale: float | None = None, q_offsets: torch.Tensor | None = None, max_q_per_seq: int = 1,
                page_mass: torch.Tensor | None = None, slot_ids: torch.Tensor | None = None,
@@ -308,7 +317,7 @@ class Q8Cache:
         sizes = (batch, max_q_per_seq, max_seq_len, window, sinks, page_mass is not None)
         size = self._workspace_bytes.get(sizes)
         if size is None:
-            size = self._workspace_bytes[sizes] = self._workspace_of(self._geom_ref, *sizes)
+            size = self._ask_workspace(sizes)
         workspace, at = None, 0
         if size:   # of this call alone: the allocator hands it on in stream order, or keeps it for a graph under capture
             workspace = torch.empty(size, dtype=torch.uint8, device=self.device)

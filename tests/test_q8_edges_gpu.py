@@ -300,3 +300,18 @@ def test_slots_that_are_not_there_are_refused_by_every_call(native_lib):
     graph.replay()
     assert (w.cache.seq_lens - lens).tolist() == [1, 0, 1]
     assert torch.equal(got[[0, 2]], w.cache.attend(q[[0, 2]], max_seq_len=90, slot_ids=i32([2, 0])))
+
+
+def test_a_growing_context_leaves_no_growing_state(native_lib):
+    w = World(Q8Layout(8, 2, 64, 16, "int8"), [900], seed=68)
+    w.feed([900])
+    q = w.randn(1, 8, 64).to(DEV)
+    mass = torch.zeros((1, 2, w.cache.max_blocks_per_seq), device=DEV)
+    lens, seen = i32([300]), set()
+    want = w.cache.attend(q, max_seq_len=300, seq_lens=lens)
+    for t in range(300, 800):
+        got = w.cache.attend(q, max_seq_len=t, seq_lens=lens, page_mass=mass)
+        # other parts, other orders of fp32 sums of 300 weights and values below 8: 2^-18 each, and masses do not enter
+        assert t % 100 or float((got - want).abs().max()) <= 8 * 2.0 ** -17
+        seen.add(len(w.cache._workspace_bytes))
+    assert max(seen) <= 64
