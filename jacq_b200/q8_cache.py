@@ -290,12 +290,14 @@ class Q8Cache:
         ``q [tokens, NH, D]`` (fp16, token rows may be strided): one token per sequence, or with ``q_offsets`` rows
         ``q_offsets[i]:q_offsets[i+1]``, at most ``max_q_per_seq``, the last ones of sequence i. Token i sees token
         j <= i if ``j < sinks`` or ``j > i - window``; ``window=0`` is no window. ``out`` is fp32, or fp16 when an fp16
-        tensor is passed. ``page_mass`` (fp32 ``[batch, NKV, width]``, single tokens only; row i belongs to row i of the
+        tensor is passed; rows that belong to no sequence, or to one that is refused, are left as they are (zeros without
+        ``out``). ``page_mass`` (fp32 ``[batch, NKV, width]``, single tokens only; row i belongs to row i of the
         batch, whatever its slot) grows by the weight every page got. ``scale`` defaults to 1 / sqrt(D). A length above
         ``max_seq_len`` is taken as ``max_seq_len``, a negative one as 0; both are counted (``rejected_indices``)."""
         total, stride = self._token_rows(q, "q", self.layout.num_q_heads)
-        if out is None:
-            out = torch.empty(q.shape, dtype=torch.float32, device=self.device)
+        if out is None:   # with offsets, rows of no sequence and of one that the device refuses are not written: zeros
+            make = torch.empty if q_offsets is None else torch.zeros
+            out = make(q.shape, dtype=torch.float32, device=self.device)
         half = out.dtype is torch.float16
         if not (half or out.dtype is torch.float32) or out.shape != q.shape or not out.is_contiguous() or out.get_device() != self._index:
             raise TypeError("out must be a contiguous torch.float32 or float16 tensor shaped like q")

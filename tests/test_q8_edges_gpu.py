@@ -315,3 +315,19 @@ def test_a_growing_context_leaves_no_growing_state(native_lib):
         assert t % 100 or float((got - want).abs().max()) <= 8 * 2.0 ** -17
         seen.add(len(w.cache._workspace_bytes))
     assert max(seen) <= 64
+
+
+def test_rows_that_nobody_writes_are_zeros_in_an_output_of_the_calls_own(native_lib):
+    """Rows behind the last sequence, before the first, and of a sequence that is refused."""
+    w = World(Q8Layout(4, 2, 64, 16, "int8"), [30, 30, 30], seed=69)
+    w.feed([30, 30, 30])
+    q = w.randn(12, 4, 64).to(DEV)
+    ends = i32([2, 4, 10, 11])                   # rows 0, 1 and 11 belong to nobody; the second sequence has six, four are stated
+    given = torch.full(q.shape, 5.0, device=DEV)
+    w.cache.attend(q, given, max_seq_len=30, q_offsets=ends, max_q_per_seq=4)
+    for _ in range(4):                           # the allocator's old blocks hold something
+        torch.full(q.shape, float("nan"), device=DEV)
+        got = w.cache.attend(q, max_seq_len=30, q_offsets=ends, max_q_per_seq=4)
+        nobody = (given == 5.0).all(-1).all(-1)
+        assert nobody.tolist() == [True] * 2 + [False] * 2 + [True] * 6 + [False, True]
+        assert int(got[nobody].abs().max()) == 0 and torch.equal(got[~nobody], given[~nobody])
