@@ -404,3 +404,11 @@ def rejected_indices() -> int:
     out = ctypes.c_uint32(0)
     _native.check(_native.lib().kivi_b200_q8_rejected_indices(ctypes.byref(out)), "kivi_b200_q8_rejected_indices")
     return int(out.value)
+
+
+def wait_failures() -> int:
+    """CTAs of the attention kernel for many query rows that gave up a bounded wait on the current device since the library
+    was loaded (their output is undefined); 0 in any healthy run."""
+    out = ctypes.c_uint32(0)
+    _native.check(_native.lib().kivi_b200_q8_wait_failures(ctypes.byref(out)), "kivi_b200_q8_wait_failures")
+    return int(out.value)

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from jacq_b200.q8_cache import Q8Layout, evict_pages, rejected_indices
+from jacq_b200.q8_cache import Q8Layout, evict_pages, rejected_indices, wait_failures
 from tests import q8_oracle as qo
 from tests.test_q8_gpu import DEV, HALF, MANY, Large, World, i32, offsets_of
 
@@ -331,3 +331,7 @@ def test_rows_that_nobody_writes_are_zeros_in_an_output_of_the_calls_own(native_
         nobody = (given == 5.0).all(-1).all(-1)
         assert nobody.tolist() == [True] * 2 + [False] * 2 + [True] * 6 + [False, True]
         assert int(got[nobody].abs().max()) == 0 and torch.equal(got[~nobody], given[~nobody])
+
+
+def test_no_wait_gave_up(native_lib):
+    assert wait_failures() == 0

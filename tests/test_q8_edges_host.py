@@ -1,6 +1,8 @@
 """Refusals and bookkeeping of the 8-bit cache that need no GPU, beside those of ``tests/test_q8_host.py``."""
 import pytest
 
+from jacq_b200 import _native, q8_cache
+
 OK, NULL, RANGE = 0, 1, 3
 FAKE = 1 << 20      # stands for a device pointer; never dereferenced on the host
 
@@ -21,3 +23,19 @@ def test_advance_refusals(native_lib, change, status):
     a = dict(lens=FAKE, rows=4, slots=FAKE, offsets=FAKE, batch=2)
     a.update(change)
     assert native_lib.kivi_b200_q8_advance_slots(*a.values(), 0) == status
+
+
+def test_wait_failures_reads_the_librarys_counter(native_lib, monkeypatch):
+    class Fake:
+        def kivi_b200_q8_wait_failures(self, out):
+            out._obj.value = 3
+            return self.status
+
+    fake = Fake()
+    monkeypatch.setattr(_native, "lib", lambda: fake)
+    fake.status = 0
+    assert q8_cache.wait_failures() == 3
+    monkeypatch.setattr(_native, "check", lambda rc, where: (_ for _ in ()).throw(RuntimeError(where)) if rc else None)
+    fake.status = 9
+    with pytest.raises(RuntimeError, match="wait_failures"):
+        q8_cache.wait_failures()
