@@ -346,9 +346,11 @@ class Q8Cache:
         """``evict_pages`` on this cache's tables and lengths (one row per slot); with ``install`` the results replace
         them, and ``page_mass`` is updated in place. The pages named in ``freed`` belong to nobody afterwards.
 
+        ``page_mass`` is ``[slots, NKV, width]``: where ``attend`` ran on some slots only, its rows go to their slots'.
         The installed tables keep the ids that were entered for the open block and for growth: they move up behind the
         kept pages. The columns that this empties hold -1, so a block that would complete there is refused and counted
         until the caller enters a page (``Q8Eviction.block_tables`` has 0 behind the kept pages)."""
+        _check_mass(page_mass, self.block_tables.shape[0], self.layout.num_kv_heads, self._index)
         r = evict_pages(self.block_tables, self.seq_lens, page_mass, block_size=self.layout.block_size, budget=budget, first=first,
                         recent=recent, max_seq_len=max_seq_len)
         if install:

@@ -335,3 +335,13 @@ def test_rows_that_nobody_writes_are_zeros_in_an_output_of_the_calls_own(native_
 
 def test_no_wait_gave_up(native_lib):
     assert wait_failures() == 0
+
+
+def test_an_eviction_wants_the_caches_own_masses(native_lib):
+    w = World(Q8Layout(4, 2, 64, 16, "int8"), [64, 64], seed=70)
+    w.feed([64, 64])
+    tables = w.cache.block_tables.clone()
+    for shape in ((2, 1, 4), (2, 3, 4), (1, 2, 4)):
+        with pytest.raises(RuntimeError, match="page_mass"):
+            w.cache.evict(torch.zeros(shape, device=DEV), budget=1, max_seq_len=64)
+    assert torch.equal(tables, w.cache.block_tables) and w.cache.seq_lens.tolist() == [64, 64]
