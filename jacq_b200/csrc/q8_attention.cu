@@ -282,9 +282,10 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>()) q8_attentio
                     float x = (odd ? b : a) + __shfl_xor_sync(0xffffffffu, odd ? a : b, 4);
                     x += __shfl_xor_sync(0xffffffffu, x, 8);
                     x += __shfl_xor_sync(0xffffffffu, x, 16);
+                    // a column that holds no row leaves 0, whatever 0 times an infinite key made of it
                     if (g < 2 && i < live)
                         p.page_ws[((size_t)(seq * nkv + h) * p.ws_tiles + item + i) * R + 8 * nt + 2 * t + g] =
-                            make_float2(x, g ? m[nt][1] : m[nt][0]);
+                            make_float2((g ? hi[nt][1] : hi[nt][0]) < 0 ? 0.0f : x, g ? m[nt][1] : m[nt][0]);
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {

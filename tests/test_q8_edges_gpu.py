@@ -345,3 +345,25 @@ def test_an_eviction_wants_the_caches_own_masses(native_lib):
         with pytest.raises(RuntimeError, match="page_mass"):
             w.cache.evict(torch.zeros(shape, device=DEV), budget=1, max_seq_len=64)
     assert torch.equal(tables, w.cache.block_tables) and w.cache.seq_lens.tolist() == [64, 64]
+
+
+@pytest.mark.parametrize("heads", [1, 3, 5, 11])
+def test_an_infinite_key_of_no_weight_leaves_the_masses_finite(heads, native_lib):
+    """K's tail holds -infinity where q is positive: weight 0. Query rows a unit has room for and nobody fills are 0, and
+    0 times infinity is no number."""
+    layout = Q8Layout(2 * heads, 2, 64, 32, "int8")
+    w = World(layout, [48], seed=71)
+    k, v = w.randn(48, 2, 64), w.randn(48, 2, 64)
+    k[40, :, 3] = float("-inf")
+    w.feed([48], k, v)
+    q = w.randn(1, 2 * heads, 64)
+    q[..., 3] = q[..., 3].abs() + 0.1
+    mass = torch.zeros((1, 2, 2), device=DEV)
+    out = w.attend(q, page_mass=mass)
+    held = w.held()[0]
+    keep = [t for t in range(48) if t != 40]
+    s = torch.einsum("hd,thd->ht", q[0].double(), held[0].repeat_interleave(heads, 1)[keep]) / 8.0
+    p = torch.zeros((2 * heads, 48), dtype=torch.float64)
+    p[:, keep] = torch.softmax(s, 1)
+    want = torch.nn.functional.pad(p, (0, 16)).view(2, heads, 2, 32).sum((1, 3))
+    assert out.isfinite().all() and ((mass[0].cpu().double() - want).abs() <= 2.0 ** -14 * want + 1e-12).all()
