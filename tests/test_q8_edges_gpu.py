@@ -218,6 +218,31 @@ def test_evictions_let_lengths_outside_the_bounds_through(native_lib):
     assert int(r.freed_counts[1]) == 2
 
 
+# ------------------------------------------------------------------------------------------------ writer
+
+@pytest.mark.parametrize("layout", [Q8Layout(8, 2, 128, 16, "int8"), Q8Layout(3, 3, 64, 32, "e4m3"), Q8Layout(4, 2, 256, 128, "int8")], ids=["16", "32", "128"])
+def test_the_writer_leaves_tail_rows_behind_the_last_token(layout, native_lib):
+    """A call writes the rows of its own tokens that stay open and no other row of the slot, nor another slot's."""
+    b = layout.block_size
+    w = World(layout, [4 * b] * 5, seed=72)
+    mark = 0x7abc                                  # a NaN that no arithmetic leaves
+    tails = (w.cache.tensors.K_TAIL, w.cache.tensors.V_TAIL)
+    for tail in tails:
+        tail.view(torch.int16).fill_(mark)
+    written = [0] * 5                              # rows of the slot that have ever been written
+    for counts in ([0, 1, b - 1, b, b + 3], [0, b - 2, 0, 1, 2 * b - 6], [0, 2, 2, 0, 1]):
+        before = w.lens()
+        w.feed(counts)
+        for i, (old, n) in enumerate(zip(before, counts)):
+            end = (old + n) % b
+            if n:
+                written[i] = max(written[i], end) if (old + n) // b > old // b else max(written[i], old % b + n)
+            for tail in tails:
+                rows = tail[i].view(torch.int16).cpu()
+                assert (rows[:, written[i]:] == mark).all() and (end == 0 or not (rows[:, :end] == mark).all(-1).any())
+    w.check_contents()
+
+
 # ------------------------------------------------------------------------------------------------ lengths, ids, bounds
 
 @pytest.mark.parametrize("many", [False, True])
