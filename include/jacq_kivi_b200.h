@@ -240,6 +240,8 @@ int kivi_b200_gemm_wait_failures(uint32_t* failures_out);
  *   scales            f32   [num_blocks, NKV, 2]      K scale, V scale
  *   k_tail, v_tail    f16   [num_slots, NKV, B, D]    the tokens of a sequence's last, incomplete block
  *
+ * Pages that a caller fills itself hold finite codes (e4m3: no 0x7f, 0xff) and scales that are 0, positive or NaN, with
+ * zero codes under a scale of 0 or NaN, as the writer leaves them.
  * Token j of a sequence is row j % B of logical page j / B. A sequence of T tokens holds T / B complete pages in
  * 8 bits (block table entries 0 .. T / B - 1) and T % B rows, 0 .. T % B - 1, of its tail slot in fp16: a block is
  * quantised once, from its fp16 rows, when its last token arrives, so no value is ever rounded twice.

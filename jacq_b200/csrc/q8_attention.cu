@@ -196,7 +196,11 @@ __global__ void __launch_bounds__(kWarps * 32, ctas_of<D, kWarps>()) q8_attentio
         m[nt][0] = m[nt][1] = kQ8Unset;
         l[nt][0] = l[nt][1] = 0.0f;
     }
-    // V's scales enter the fp16 probabilities relative to vref, a power of two not below any met so far (0: none yet)
+    // V's scales enter the fp16 probabilities relative to vref, a power of two not below any met so far (0: none yet). One
+    // for all columns: where rows of a run see different pages, a page whose V scale is 2^r times the others' leaves the rows
+    // that do not see it probabilities off by 2^(r - 31) of the largest: as much as an fp16 output's rounding at r = 20. A
+    // reference per column costs 82.7 -> 101.2 us at 24 x 8 tokens behind 8000 and up to 5 % for single tokens, whose
+    // columns all see the same.
     float vref = 0.0f, vmul = 0.0f;
     const float second = FOLD && t >= 2 ? 1.0f : 0.0f;
 
@@ -791,7 +795,9 @@ struct Plan {
 // multiprocessor runs its queue in rounds of as many CTAs as fit. Parts are joined in a cluster (about 1 us, parts 2, 4
 // or 8) while all clusters are resident at once -- 16 units of 512 tokens, head_dim 64: 6.8 us against 8.2 with the
 // merge kernel -- and by the merge kernel beyond that (256 units of ragged lengths in 2 parts: 63 us against 56, as
-// clusters wait for all of their CTAs' slots). With one unit per multiprocessor or fewer, eight-warp CTAs with deeper
+// clusters wait for all of their CTAs' slots). All sequences are cut by the longest one's tiles: in a ragged batch the
+// longest sequence's parts decide the time while others' places are empty. The figures here are all the model was fitted
+// to; it was not measured on a second set of calls. With one unit per multiprocessor or fewer, eight-warp CTAs with deeper
 // rings (8 units of 32768 tokens: 24.7 us against 26.6).
 constexpr double kStart = 4.0, kClusterUs = 1.0, kMergeUs = 3.0;
 constexpr long long kMostParts = 16384;
@@ -832,13 +838,12 @@ void plan_parts(Plan& q, int d) {
 
 // Whether the kernel for many rows is the faster one. It takes 3.1, 3.8 and 4.6 us (head_dim 64, 128, 256) for 128 keys of
 // its 256 (128) rows on every multiprocessor; the other one 0.40, 0.60 and 1.3 ns for 16 keys of 16 rows. At head_dim
-// 128, 8 sequences of 8192 tokens, 8 kv heads: 128 rows each 276 us against 181, 256 rows 287 against 409, 512 rows
-// 282 against 766. Of 36 calls between both kernels' ranges a margin
-// of 1.1 on the model chose two better than 1.25 and one worse; over 36 others, drawn afterwards, it takes 1.5 % more
-// than the faster kernel of each call, 1.25 takes 3.1 %, always the one for few rows 15 %, always the other 27 %
-// (geometric means). It gains on long contexts (256, 2 x 123 tokens, window 1654, 8/32 heads: 117 us -> 80) and loses 1
-// to 6 us on small calls (128, 4 x 104 tokens, 2/14 heads: 18.5 -> 24.0). Known misses: 64, 3 x 150 tokens behind 5163,
-// 3/36 heads, 182 us against 128; 256, 2 x 68 behind 6104, 8/40 heads, 256 against 210.
+// 128, 8 sequences of 8192 tokens, 8 kv heads: 128 rows each 272 us against 192, 256 rows 280 against 482, 512 rows
+// 281 against 934. Over two sets of 36 calls between both kernels' ranges it takes 1.0 and 2.0 % more than the faster
+// kernel of each call, always the one for few rows 15 and 11 %, always the other 29 and 25 % (geometric means). It loses 3
+// to 8 us on small calls (128, 4 x 104 tokens, 2/14 heads: 15.8 -> 23.3), and misses one large one: 64, 3 x 150 tokens
+// behind 5163, 3/36 heads, 180 us against 139. It knows the largest count of the batch only: single tokens beside a prompt
+// go with the prompt, in units of 256 rows of which they fill a few; a caller that has many makes two calls.
 bool many_rows(int d, int batch, int nkv, long long rows, int tiles) {
     const int per = d == 256 ? 128 : 256;
     const double step_us = d == 64 ? 3.1 : d == 128 ? 3.8 : 4.6, tile_us = (d == 64 ? 0.40 : d == 128 ? 0.60 : 1.3) * 1e-3;

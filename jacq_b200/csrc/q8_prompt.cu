@@ -16,15 +16,17 @@
 // cycle) bound it, not HBM; one tile's products run under the other's exponentials. Every wait is bounded: a CTA whose
 // wait gave up counts itself, waits for its products and leaves.
 //
-// Measured: 8 x 1024 query tokens behind 8192, 32/8 heads, no window: 1.64 ms, 627 TFLOP/s (e4m3 647), 0.37 of a large
-// library product's rate; 2 x 1024 behind 6144, window 4096: 268 us, where the second round of 256 units leaves
-// 40 of 148 multiprocessors idle. A step takes 6300 cycles of which the products fill 2300: a tile's own chain (products, then 4100 cycles
-// of softmax at a third of the exponential unit's rate, then products) is what bounds it. Steps of the softmax: two
-// passes with the maximum 312 us -> none, packed arithmetic 288 -> masks as values 278 ->
-// two tiles under one load of the keys 268. Two threads per row (274 us) and two CTAs of one tile (278) were no faster:
-// with several roles' code in turn the instruction cache counts (the fully unrolled form took 343).
-// The second half of P: 274 us without it, 321 with it while the next 32 scores were fetched under the present ones (84 to
-// 108 bytes of spills a thread, twice the code in the loop), 267 since scores are fetched when they are due.
+// Measured: 8 x 1024 query tokens behind 8192, 32/8 heads, no window: 1.65 ms, 624 TFLOP/s of the formula's 4 D flops a
+// pair (e4m3 646), 0.37 and 0.38 of a large library product's rate, which the second product's half again is not counted
+// in; head_dim 64: 381, 256 with 16/4 heads: 456. 2 x 1024 behind 6144, window 4096: 268 to 277 us in different runs, where
+// the second round of 256 units leaves 40 of 148 multiprocessors idle: the tensor pipe is busy 35 % of the time, the
+// exponentials' unit 31 %, the issue slots 41 %, so what bounds it is a tile's own chain (products, softmax, products).
+// Steps of the softmax: two passes with the maximum 312 us -> none, packed arithmetic 288 -> masks as values 278 -> two
+// tiles under one load of the keys 268. Two threads per row (274 us) and two CTAs of one tile (278) were no faster: with
+// several roles' code in turn the instruction cache counts (the fully unrolled form took 343). The second half of P: 274 us
+// without it, 321 with it while the next 32 scores were fetched under the present ones (84 to 108 bytes of spills a thread,
+// twice the code in the loop), 267 since scores are fetched when they are due; an exponent for the tail 269, V's reference
+// per row 272.
 #include "q8_common.cuh"
 
 namespace kivi {
