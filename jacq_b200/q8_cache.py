@@ -6,7 +6,8 @@ sequence's last, incomplete page stay in fp16 tail rows until the page fills up,
 and semantics are those of ``include/jacq_kivi_b200.h`` (section q8).
 
 ``Q8Cache`` owns (or is laid over) one layer's tensors, block tables and sequence lengths, all on the device; each
-method is one library call on the current stream and nothing synchronises with the host. The reference has no 8-bit
+method is one library call on the current stream (slot ids take one more to gather tables and lengths, and a write one to
+advance the lengths) and nothing synchronises with the host. The reference has no 8-bit
 cache, no window and, for its page-drop mechanism, no eviction policy.
 
 torch is plumbing here (device memory, streams); all arithmetic is in libjacq_kivi_b200.so.
